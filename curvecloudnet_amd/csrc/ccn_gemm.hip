@@ -1414,9 +1414,8 @@ __global__ __launch_bounds__(PR_TPB, 2) void gemm_glds_pair_kernel(const float* 
         // a handful of VALU instructions of the NEXT group's transform.  A wave issues in order and the matrix pipe takes
         // one MFMA per 64 cycles, so VALU work placed between MFMAs is free, VALU work behind all sixteen is not (first
         // form: transform after the group's MFMAs, 10-25 % slower than the plain product).
-        // (round 5: TWO K components per call in packed form -- v_pk_fma_f32, v_pk_mul_f32 and two v_max_f32 per block instead
-        // of fma / mul / cmp / cndmask + the VCC hazard's wait states per element: 8 vector instructions per call where the
-        // round-2 form issued 16 + 8 s_nop.  max(v, v * neg) == (v > 0 ? v : v * neg) for 0 <= neg <= 1, the entry point checks it.)
+        // (TWO K components per call: fma, mul and max per element instead of fma / mul / cmp / cndmask + the VCC hazard's wait
+        // states; the build keeps packed fp32 instructions out, the step takes the same time with and without them: 103.9 ms.  max(v, v * neg) == (v > 0 ? v : v * neg) for 0 <= neg <= 1, the entry point checks it.)
         const f32x2 neg2 = {xf_neg, xf_neg};
         auto xform_pair = [&](int par, int c2) {
           __builtin_amdgcn_sched_barrier(0);
@@ -1612,7 +1611,7 @@ __global__ __launch_bounds__(PR_TPB, 2) void gemm_glds_pair_kernel(const float* 
           } else
           if (colstats != nullptr) {
             // column statistics only where a BatchNorm follows (a data-gradient launch skips 128 vector instructions per tile
-            // and wave), two accumulator registers per packed instruction (v_pk_add_f32 / v_pk_fma_f32)
+            // and wave), two accumulator registers at a time
             f32x2 p1 = {0.f, 0.f}, p2 = {0.f, 0.f};
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {

@@ -113,8 +113,8 @@ __global__ __launch_bounds__(TN_TPB, 2) void gemm_tn_glds_kernel(const float* __
         xsh[c] = xf_shift[k];
       }
     }
-    // (branch-free; bits of act(b * scale + shift), ReLU's zero may be -0.0.  Round 5: packed -- v_pk_fma_f32, v_pk_mul_f32 and
-    // two v_max_f32 instead of two each of fma / mul / cmp / cndmask + the VCC hazard's wait states; max(v, v * neg) equals
+    // (branch-free; bits of act(b * scale + shift), ReLU's zero may be -0.0.  Fma, mul and max per element instead
+    // of fma / mul / cmp / cndmask + the VCC hazard's wait states; max(v, v * neg) equals
     // (v > 0 ? v : v * neg) for 0 <= neg <= 1, which the entry point checks.)
     const f32x2 xsc2 = {xsc[0], xsc[1]}, xsh2 = {xsh[0], xsh[1]}, neg2 = {xf_neg, xf_neg};
     auto xform = [&](f32x2& b) {

@@ -24,7 +24,8 @@ NOP = re.compile(r"^\s*s_nop\s+(\d+)")
 def scan(path):
     with tempfile.TemporaryDirectory() as tmp:
         out = os.path.join(tmp, "k.s")
-        subprocess.run(["hipcc", "-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-S", "--cuda-device-only", "-o", out,
+        subprocess.run(["hipcc", "-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Xclang", "-target-feature",
+                        "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", "-o", out,
                         path], check=True, stderr=subprocess.DEVNULL)
         lines = open(out).read().splitlines()
     bad = []
