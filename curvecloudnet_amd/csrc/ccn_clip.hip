@@ -1,0 +1,366 @@
+// The global norm of many gradients, their clipping, and the Adam update that clips as it goes.
+//
+//   norm = sqrt(sum g^2)  |  sum |g|  |  max |g|    over every value of every tensor,   scale = min(1, max_norm / (norm + 1e-6))
+// Squares and sums are held in 64 bits: a square of any fp32 value is far inside their range, so no value is too large or too small
+// for the norm.  Every workgroup writes one partial result and every reader adds the partial results in the same order: the norm has
+// the same bits in every run.  The tensors' addresses and sizes travel in the kernel's arguments (CLIP_MAX tensors per launch), so a
+// captured launch holds them by value.
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "ccn_common.h"
+
+namespace {
+
+constexpr int CLIP_TPB = 256;
+constexpr int CLIP_MAX = 160;                      // tensors of one launch: 20 bytes of arguments each
+constexpr int CLIP_PART_MAX = 1024;                // workgroups of one launch of the norm, each with a partial result
+constexpr int64_t CLIP_CHUNK = 16384;              // values that a workgroup takes at a time
+
+struct ClipTable {
+  void* ptr[CLIP_MAX];
+  int64_t size[CLIP_MAX];
+  uint8_t dtype[CLIP_MAX];
+  int first[CLIP_MAX + 1];                         // chunks in front of tensor i
+  int n;
+};
+static_assert(sizeof(ClipTable) < 3584, "kernel arguments");
+
+enum { NORM_SUM = 1, NORM_TWO = 2, NORM_MAX = 3 };
+
+template <int KIND>
+__device__ __forceinline__ double clip_term(float v) {
+  return KIND == NORM_TWO ? (double)v * (double)v : fabs((double)v);
+}
+// (a NaN stays: fmax would drop it)
+template <int KIND>
+__device__ __forceinline__ double clip_join(double a, double b) {
+  if (KIND != NORM_MAX) return a + b;
+  return a != a ? a : (b > a || b != b ? b : a);
+}
+__device__ __forceinline__ double clip_shfl_xor(double v, int d) { return __shfl_xor(v, d, 64); }
+
+template <int KIND>
+__device__ __forceinline__ double clip_block(double v, double* red) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = clip_join<KIND>(v, clip_shfl_xor(v, d));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+  for (int k = 1; k < CLIP_TPB / 64; ++k) v = clip_join<KIND>(v, red[k]);
+  __syncthreads();
+  return v;
+}
+
+// The tensor that chunk c belongs to.
+__device__ __forceinline__ int clip_find(const ClipTable& t, int c) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int KIND, int T>
+__device__ __forceinline__ double clip_sum(const void* p, int64_t beg, int64_t end) {
+  double v = 0.0;
+  for (int64_t i = beg + threadIdx.x; i < end; i += CLIP_TPB) v = clip_join<KIND>(v, clip_term<KIND>(ld_el<T>(p, i)));
+  return v;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(CLIP_TPB) void grad_norm_kernel(const ClipTable t, double* __restrict__ partial) {
+  __shared__ double red[CLIP_TPB / 64];
+  double v = 0.0;
+  for (int c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
+    const int i = clip_find(t, c);
+    const int64_t beg = (int64_t)(c - t.first[i]) * CLIP_CHUNK, end = min(beg + CLIP_CHUNK, t.size[i]);
+    const double u = t.dtype[i] == 0 ? clip_sum<KIND, 0>(t.ptr[i], beg, end)
+                     : t.dtype[i] == 1 ? clip_sum<KIND, 1>(t.ptr[i], beg, end) : clip_sum<KIND, 2>(t.ptr[i], beg, end);
+    v = clip_join<KIND>(v, u);
+  }
+  v = clip_block<KIND>(v, red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = v;
+}
+
+// Every thread of the workgroup gets the norm, from the partial results in a fixed order.
+template <int KIND>
+__device__ __forceinline__ double clip_total(const double* __restrict__ partial, int n, double* red) {
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n; i += CLIP_TPB) v = clip_join<KIND>(v, partial[i]);
+  v = clip_block<KIND>(v, red);
+  return KIND == NORM_TWO ? sqrt(v) : v;
+}
+__device__ __forceinline__ float clip_scale(double norm, double max_norm) {
+  const double s = max_norm / (norm + 1e-6);
+  return s != s ? NAN : s < 1.0 ? (float)s : 1.f;       // (a NaN norm makes every gradient NaN; an infinite one makes them 0)
+}
+
+template <int KIND>
+__global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double* __restrict__ partial, int n,
+                                                                   float* __restrict__ norm) {
+  __shared__ double red[CLIP_TPB / 64];
+  const double v = clip_total<KIND>(partial, n, red);
+  if (threadIdx.x == 0) *norm = (float)v;
+}
+
+template <int T>
+__device__ __forceinline__ void clip_apply(void* p, int64_t beg, int64_t end, float scale) {
+  for (int64_t i = beg + threadIdx.x; i < end; i += CLIP_TPB) st_el<T>(p, i, ld_el<T>(p, i) * scale);
+}
+
+template <int KIND>
+__global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, const double* __restrict__ partial, int n,
+                                                             double max_norm, float* __restrict__ norm) {
+  __shared__ double red[CLIP_TPB / 64];
+  const double v = clip_total<KIND>(partial, n, red);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+  const float scale = clip_scale(v, max_norm);
+  if (scale == 1.f) return;
+  for (int c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
+    const int i = clip_find(t, c);
+    const int64_t beg = (int64_t)(c - t.first[i]) * CLIP_CHUNK, end = min(beg + CLIP_CHUNK, t.size[i]);
+    if (t.dtype[i] == 0) clip_apply<0>(t.ptr[i], beg, end, scale);
+    else if (t.dtype[i] == 1) clip_apply<1>(t.ptr[i], beg, end, scale);
+    else clip_apply<2>(t.ptr[i], beg, end, scale);
+  }
+}
+
+// ---- Adam over several runs of parameters with the gradients scaled on the way
+constexpr int ADAM_MAX = 64;
+
+struct AdamTable {
+  float* p[ADAM_MAX];
+  const float* g[ADAM_MAX];
+  float* m[ADAM_MAX];
+  float* v[ADAM_MAX];
+  int64_t size[ADAM_MAX];
+  int first[ADAM_MAX + 1];
+  int n;
+};
+static_assert(sizeof(AdamTable) < 3584, "kernel arguments");
+
+__global__ __launch_bounds__(CLIP_TPB) void adam_clip_kernel(const AdamTable t, const double* __restrict__ partial, int n,
+                                                             double max_norm, float* __restrict__ norm, float beta1_rest,
+                                                             float beta2, float beta2_rest, float step_size, float inv_bc2_sqrt,
+                                                             float eps, float weight_decay) {
+  __shared__ double red[CLIP_TPB / 64];
+  const double total = clip_total<NORM_TWO>(partial, n, red);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+  const float scale = clip_scale(total, max_norm);
+  for (int c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
+    int i = 0;
+    while (t.first[i + 1] <= c) ++i;
+    const int64_t beg = (int64_t)(c - t.first[i]) * CLIP_CHUNK, end = min(beg + CLIP_CHUNK, t.size[i]);
+    for (int64_t k = beg + threadIdx.x; k < end; k += CLIP_TPB) {
+      const float pk = t.p[i][k], grad = t.g[i][k] * scale + weight_decay * pk;
+      const float mk = t.m[i][k] + (grad - t.m[i][k]) * beta1_rest;
+      const float vk = t.v[i][k] * beta2 + beta2_rest * grad * grad;
+      t.m[i][k] = mk;
+      t.v[i][k] = vk;
+      t.p[i][k] = pk - step_size * (mk / (sqrtf(vk) * inv_bc2_sqrt + eps));
+    }
+  }
+}
+
+int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype, int64_t n, bool writes, const char* who) {
+  CCN_REQUIRE(n >= 0 && n < (1 << 24) && (n == 0 || (ptr && size)), "%s: n=%lld, or a null table", who, (long long)n);
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t el = dtype && dtype[i] ? 2 : 4;
+    CCN_REQUIRE(!dtype || (dtype[i] >= 0 && dtype[i] <= 2), "%s: tensor %lld: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", who,
+                (long long)i, dtype ? dtype[i] : 0);
+    CCN_REQUIRE(size[i] >= 0 && size[i] < ((int64_t)1 << 36), "%s: tensor %lld has %lld values", who, (long long)i, (long long)size[i]);
+    CCN_REQUIRE(size[i] == 0 || (ptr[i] && (uintptr_t)ptr[i] % el == 0), "%s: tensor %lld: null or not aligned to its type", who,
+                (long long)i);
+  }
+  if (!writes) return CCN_OK;
+  bool ordered = true;                               // tensors of one buffer come in order, or in reverse: looked at before sorting
+  std::vector<std::pair<uintptr_t, uintptr_t>> span;
+  try {
+    span.reserve((size_t)n);
+  } catch (...) {
+    ccn_set_error("%s: out of host memory", who);
+    return CCN_ERR_ARG;
+  }
+  for (int64_t i = 0; i < n; ++i) {
+    if (size[i] == 0) continue;
+    const uintptr_t a = (uintptr_t)ptr[i], b = a + (uintptr_t)size[i] * (dtype && dtype[i] ? 2 : 4);
+    ordered = ordered && (span.empty() || span.back().first <= a);
+    span.emplace_back(a, b);
+  }
+  if (!ordered) std::sort(span.begin(), span.end());
+  for (size_t i = 1; i < span.size(); ++i)
+    CCN_REQUIRE(span[i - 1].second <= span[i].first, "%s: two of the tensors share memory (the same one given twice?)", who);
+  return CCN_OK;
+}
+
+int clip_chunks(int64_t size) { return (int)((size + CLIP_CHUNK - 1) / CLIP_CHUNK); }
+
+// The tables of the launches that a list of tensors takes: f(table) for each.
+template <typename F>
+int clip_tables(const void* const* ptr, const int64_t* size, const int32_t* dtype, int64_t n, F f) {
+  ClipTable t;
+  t.n = 0;
+  t.first[0] = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    if (size[i] == 0) continue;
+    t.ptr[t.n] = const_cast<void*>(ptr[i]);
+    t.size[t.n] = size[i];
+    t.dtype[t.n] = (uint8_t)(dtype ? dtype[i] : 0);
+    t.first[t.n + 1] = t.first[t.n] + clip_chunks(size[i]);
+    if (++t.n == CLIP_MAX) {
+      if (int rc = f(t)) return rc;
+      t.n = 0;
+    }
+  }
+  return t.n ? f(t) : CCN_OK;
+}
+
+// The partial results of the norm: *count of them, at `partial`.
+int clip_norm_launches(const void* const* ptr, const int64_t* size, const int32_t* dtype, int64_t n, int kind, double* partial,
+                       int* count, hipStream_t s) {
+  *count = 0;
+  return clip_tables(ptr, size, dtype, n, [&](const ClipTable& t) {
+    const int chunks = t.first[t.n], grid = chunks < CLIP_PART_MAX ? chunks : CLIP_PART_MAX;
+    double* const to = partial + *count;
+    if (kind == NORM_TWO) hipLaunchKernelGGL(grad_norm_kernel<NORM_TWO>, dim3(grid), dim3(CLIP_TPB), 0, s, t, to);
+    else if (kind == NORM_SUM) hipLaunchKernelGGL(grad_norm_kernel<NORM_SUM>, dim3(grid), dim3(CLIP_TPB), 0, s, t, to);
+    else hipLaunchKernelGGL(grad_norm_kernel<NORM_MAX>, dim3(grid), dim3(CLIP_TPB), 0, s, t, to);
+    *count += grid;
+    return CCN_OK;
+  });
+}
+
+}  // namespace
+
+extern "C" size_t ccn_grad_norm_workspace_bytes(int64_t n) {
+  if (n < 0) return 0;
+  const int64_t launches = (n + CLIP_MAX - 1) / CLIP_MAX;
+  return ccn_align256((size_t)(launches < 1 ? 1 : launches) * CLIP_PART_MAX * sizeof(double));
+}
+
+extern "C" int ccn_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, void* ws,
+                             size_t ws_bytes, float* norm, void* stream) {
+  if (int rc = clip_check(grads, sizes, dtypes, n, false, "grad_norm")) return rc;
+  CCN_REQUIRE(kind >= NORM_SUM && kind <= NORM_MAX, "grad_norm: kind %d is not 1 (sum), 2 (two) or 3 (max)", kind);
+  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "grad_norm: null norm or workspace");
+  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
+    ccn_set_error("grad_norm: workspace %zu < %zu bytes", ws_bytes, ccn_grad_norm_workspace_bytes(n));
+    return CCN_ERR_WORKSPACE;
+  }
+  double* const partial = (double*)ws;
+  int count = 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (int rc = clip_norm_launches(grads, sizes, dtypes, n, kind, partial, &count, s)) return rc;
+  if (kind == NORM_TWO) hipLaunchKernelGGL(grad_norm_final_kernel<NORM_TWO>, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, norm);
+  else if (kind == NORM_SUM) hipLaunchKernelGGL(grad_norm_final_kernel<NORM_SUM>, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, norm);
+  else hipLaunchKernelGGL(grad_norm_final_kernel<NORM_MAX>, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, norm);
+  CCN_LAUNCH_OK("grad_norm");
+  return CCN_OK;
+}
+
+extern "C" int ccn_grad_clip(void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, double max_norm,
+                             void* ws, size_t ws_bytes, float* norm, void* stream) {
+  if (int rc = clip_check(grads, sizes, dtypes, n, true, "grad_clip")) return rc;
+  CCN_REQUIRE(kind >= NORM_SUM && kind <= NORM_MAX, "grad_clip: kind %d is not 1 (sum), 2 (two) or 3 (max)", kind);
+  CCN_REQUIRE(max_norm >= 0.0, "grad_clip: max_norm %g", max_norm);
+  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "grad_clip: null norm or workspace");
+  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
+    ccn_set_error("grad_clip: workspace %zu < %zu bytes", ws_bytes, ccn_grad_norm_workspace_bytes(n));
+    return CCN_ERR_WORKSPACE;
+  }
+  double* const partial = (double*)ws;
+  int count = 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (int rc = clip_norm_launches(grads, sizes, dtypes, n, kind, partial, &count, s)) return rc;
+  if (count == 0) {
+    hipLaunchKernelGGL(grad_norm_final_kernel<NORM_SUM>, dim3(1), dim3(CLIP_TPB), 0, s, partial, 0, norm);
+    CCN_LAUNCH_OK("grad_clip");
+    return CCN_OK;
+  }
+  float* out = norm;
+  const int rc = clip_tables(grads, sizes, dtypes, n, [&](const ClipTable& t) {
+    const int chunks = t.first[t.n], grid = chunks < 4 * CLIP_PART_MAX ? chunks : 4 * CLIP_PART_MAX;
+    if (kind == NORM_TWO)
+      hipLaunchKernelGGL(grad_clip_kernel<NORM_TWO>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
+    else if (kind == NORM_SUM)
+      hipLaunchKernelGGL(grad_clip_kernel<NORM_SUM>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
+    else
+      hipLaunchKernelGGL(grad_clip_kernel<NORM_MAX>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
+    out = nullptr;
+    return CCN_OK;
+  });
+  if (rc) return rc;
+  CCN_LAUNCH_OK("grad_clip");
+  return CCN_OK;
+}
+
+extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, float* const* exp_avgs, float* const* exp_avg_sqs,
+                             const int64_t* sizes, int64_t n, double lr, double beta1, double beta2, double eps,
+                             double weight_decay, int64_t step, double max_norm, void* ws, size_t ws_bytes, float* norm, void* stream) {
+  CCN_REQUIRE(step >= 1, "adam_clip: step=%lld", (long long)step);
+  CCN_REQUIRE(n >= 0 && (n == 0 || (params && grads && exp_avgs && exp_avg_sqs && sizes)), "adam_clip: n=%lld, or a null table",
+              (long long)n);
+  CCN_REQUIRE(max_norm >= 0.0, "adam_clip: max_norm %g", max_norm);
+  if (int rc = clip_check((const void* const*)grads, sizes, nullptr, n, false, "adam_clip")) return rc;
+  std::vector<const void*> all;
+  std::vector<int64_t> every;
+  try {                                              // nothing that is written may share memory with anything else that is used
+    for (int64_t i = 0; i < n; ++i)
+      for (const void* p : {(const void*)params[i], (const void*)grads[i], (const void*)exp_avgs[i], (const void*)exp_avg_sqs[i]}) {
+        CCN_REQUIRE(size_t(p) % 16 == 0, "adam_clip: buffers must be 16-byte aligned");
+        all.push_back(p);
+        every.push_back(sizes[i]);
+      }
+  } catch (...) {
+    ccn_set_error("adam_clip: out of host memory");
+    return CCN_ERR_ARG;
+  }
+  if (int rc = clip_check(all.data(), every.data(), nullptr, 4 * n, true, "adam_clip")) return rc;
+  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "adam_clip: null norm or workspace");
+  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
+    ccn_set_error("adam_clip: workspace %zu < %zu bytes", ws_bytes, ccn_grad_norm_workspace_bytes(n));
+    return CCN_ERR_WORKSPACE;
+  }
+  double* const partial = (double*)ws;
+  int count = 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (int rc = clip_norm_launches((const void* const*)grads, sizes, nullptr, n, NORM_TWO, partial, &count, s)) return rc;
+  if (count == 0) {
+    hipLaunchKernelGGL(grad_norm_final_kernel<NORM_TWO>, dim3(1), dim3(CLIP_TPB), 0, s, partial, 0, norm);
+    CCN_LAUNCH_OK("adam_clip");
+    return CCN_OK;
+  }
+  // bias corrections and 1 - beta in double on the host (1 - 0.999 from a beta in 32 bits is off by 1.3e-5 of itself)
+  const double bc1 = 1.0 - pow(beta1, (double)step), bc2 = 1.0 - pow(beta2, (double)step);
+  const float step_size = (float)(lr / bc1), inv_bc2_sqrt = (float)(1.0 / sqrt(bc2));
+  float* out = norm;
+  AdamTable t;
+  t.n = 0;
+  t.first[0] = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    if (sizes[i] > 0) {
+      t.p[t.n] = params[i];
+      t.g[t.n] = grads[i];
+      t.m[t.n] = exp_avgs[i];
+      t.v[t.n] = exp_avg_sqs[i];
+      t.size[t.n] = sizes[i];
+      t.first[t.n + 1] = t.first[t.n] + clip_chunks(sizes[i]);
+      ++t.n;
+    }
+    if (t.n == ADAM_MAX || (i == n - 1 && t.n > 0)) {
+      const int chunks = t.first[t.n], grid = chunks < 4 * CLIP_PART_MAX ? chunks : 4 * CLIP_PART_MAX;
+      hipLaunchKernelGGL(adam_clip_kernel, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out,
+                         (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), step_size, inv_bc2_sqrt, (float)eps,
+                         (float)weight_decay);
+      out = nullptr;
+      t.n = 0;
+    }
+  }
+  CCN_LAUNCH_OK("adam_clip");
+  return CCN_OK;
+}

@@ -5,8 +5,13 @@ The Lovasz-softmax term is evaluated for all classes at once: one segmented desc
 matrix (device radix sort), two row-wise prefix sums, and a masked mean over the classes present -- no ``.sum() == 0``
 sync per class (the reference does 20 of them on KITTI).
 """
+from typing import NamedTuple, Optional
+
 import torch
 import torch.nn.functional as F
+
+from . import ops
+from ._lib import require_gpu
 
 
 def lovasz_softmax_flat(probas, labels, classes="present"):
@@ -30,6 +35,62 @@ def lovasz_softmax_flat(probas, labels, classes="present"):
         return per_class.mean()
     present = (total[:, 0] > 0).to(probas.dtype)
     return (per_class * present).sum() / present.sum()
+
+
+class Scores(NamedTuple):
+    """What token_logprobs returns; the last two are None where no alternatives were asked for."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: Optional[torch.Tensor]
+    top_index: Optional[torch.Tensor]
+
+
+def token_logprobs(logits, target, top=0, ignore_index=-100):
+    """Log-probability of a given class in every row of ``logits`` (..., C), the row's entropy, and its ``top`` best alternatives,
+    in one pass over the logits (ccn_logprob_fwd); differentiable with respect to the logits in logprob, entropy and top_logprob.
+
+    logits: fp32, bf16 or fp16, any strides (columns that are not adjacent are copied).  target: int64 (or int32) of shape (...).
+    top: 0 ... min(64, C).  Returns ``Scores``: logprob (...), entropy (...), top_logprob (..., top) in fp32 and top_index (...,
+    top) in int64, best first, equal logits by ascending class.
+
+    ``target == ignore_index``: logprob 0, no gradient from it; entropy and alternatives are the row's all the same.  Any other
+    target outside [0, C): NaN, in logprob and (where logprob takes part in the loss) in the row's gradient.  Logits of -inf are
+    classes without probability; a row of nothing else has logprob -inf, entropy 0 and gradient 0 but for the given class's own.
+    The gradient has the logits' type, its rows 16-byte aligned (their stride padded where C is odd)."""
+    if logits.dtype not in ops.LOGIT_DTYPES:
+        raise TypeError("token_logprobs: logits are %s; fp32, bf16 or fp16 is wanted" % logits.dtype)
+    if target.dtype not in (torch.int64, torch.int32):
+        raise TypeError("token_logprobs: target is %s; int64 or int32 is wanted" % target.dtype)
+    if target.is_cuda and logits.is_cuda and target.device != logits.device:
+        raise ValueError("token_logprobs: logits on %s, target on %s" % (logits.device, target.device))
+    if logits.dim() == 0 or logits.size(-1) == 0 or logits.size(-1) >= 1 << 31:
+        raise ValueError("token_logprobs: logits of shape %s have no classes, or too many" % (tuple(logits.shape),))
+    shape, c = logits.shape[:-1], logits.size(-1)
+    if target.shape != shape:
+        raise ValueError("token_logprobs: logits of shape %s want a target of shape %s, got %s"
+                         % (tuple(logits.shape), tuple(shape), tuple(target.shape)))
+    top = int(top)
+    if top < 0 or top > min(ops.TOP_MAX, c):
+        raise ValueError("token_logprobs: top=%d; 0 to %d is wanted" % (top, min(ops.TOP_MAX, c)))
+    rows = target.numel()
+    if rows >= 1 << 31:
+        raise ValueError("token_logprobs: %d rows" % rows)
+    require_gpu(logits, target)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, c) if rows else logits.reshape(0, c)
+    # (one row: its stride is never used, and torch may report any)
+    if (x.stride(1) != 1 and c > 1) or (rows > 1 and x.stride(0) < c):
+        x = x.contiguous()
+    target = target.reshape(-1).to(torch.int64).contiguous()
+    with torch.cuda.device(logits.device):
+        if torch.is_grad_enabled() and logits.requires_grad:
+            out = ops.TokenLogProbs.apply(x, target, top, int(ignore_index))
+        else:
+            out = ops.logprob_forward(x.detach(), target, top, int(ignore_index), stats=False)[:4]
+    if len(shape) == 1:
+        return Scores(*out)
+    logprob, entropy, best, index = out
+    return Scores(logprob.view(shape), entropy.view(shape), best.view(*shape, top) if top else None,
+                  index.view(*shape, top) if top else None)
 
 
 def seg_loss_kitti(pred, gt, ignore=0, use_lovasz=False, class_weights=None):

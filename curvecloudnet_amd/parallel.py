@@ -6,7 +6,10 @@ The reference has no distributed code at all; this is th
 section 8(e).  BatchNorm statistics stay per rank (a rank's result equals the reference run on
 that rank's sub-batch).  Works with the gloo backend on CPU tensors too (used by the tests).
 """
+import array
 import contextlib
+import ctypes
+import math
 import os
 
 import torch
@@ -236,6 +239,143 @@ class GradientAllReduce:
         return sum(f.numel() * f.element_size() for f, _, _ in self.buckets)
 
 
+_GRAD_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}
+
+
+def _norm_kind(norm_type, who):
+    kind = _NORM_KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError("%s: norm_type %r; 1, 2 or inf is wanted" % (who, norm_type))
+    return kind
+
+
+def _bound(max_norm, who):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("%s: max_norm is %r" % (who, max_norm))
+    return max_norm
+
+
+def _dense(t):
+    """Whether the values of ``t`` fill one run of memory, in whatever order of the dimensions."""
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.size()) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class _Tensors:
+    """The tables that the norm's entry points read on the host: addresses, sizes and types of tensors of one device."""
+
+    def __init__(self, tensors, who):
+        if any(t.layout is not torch.strided for t in tensors):
+            raise TypeError("%s: sparse tensors are not built" % who)
+        try:
+            codes = [_GRAD_DTYPES[t.dtype] for t in tensors]
+        except KeyError as e:
+            raise TypeError("%s: %s; fp32, bf16 or fp16 is wanted" % (who, e.args[0])) from None
+        for t in tensors:
+            if not t.is_contiguous() and not _dense(t):
+                raise ValueError("%s: a tensor of strides %s does not fill its memory" % (who, tuple(t.stride())))
+        places = set(map(torch.Tensor.get_device, tensors))
+        if -1 in places:
+            raise RuntimeError("curvecloudnet_amd ops run on the GPU only (got a cpu tensor); there is no CPU path")
+        if len(places) != 1:
+            raise ValueError("%s: tensors on %d devices; one is wanted" % (who, len(places)))
+        self.place = places.pop()
+        sizes = [t.numel() for t in tensors]
+        self.n = len(tensors)
+        self.nbytes = sum(n * (4, 2, 2)[k] for n, k in zip(sizes, codes))
+        self.keep = [array.array("q", (t.data_ptr() for t in tensors)), array.array("q", sizes), array.array("i", codes)]
+        self.ptrs, self.sizes, self.codes = (ctypes.c_void_p(a.buffer_info()[0]) for a in self.keep)
+
+
+def _norm_call(entry, tables, *args):
+    from ._lib import call, lib, ptr, workspace
+    with torch.cuda.device(tables.place):
+        dev = torch.device("cuda", tables.place)
+        nbytes = lib().ccn_grad_norm_workspace_bytes(tables.n)
+        ws, norm = workspace(nbytes, dev), torch.empty((), dtype=torch.float32, device=dev)
+        call(entry, *args, ptr(ws), nbytes, ptr(norm), work_rows=tables.nbytes)
+    return norm
+
+
+def grad_norm(tensors, norm_type=2.0):
+    """The norm of all values of all ``tensors`` (fp32, bf16 or fp16, of one GPU) as ONE vector: an fp32 scalar on the device, summed
+    in 64 bits in a fixed order (ccn_grad_norm).  norm_type: 1, 2 or inf.  The gradients of a GradientAllReduce are already reduced
+    after ``finish()``: every rank computes the same norm and no collective is needed."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    kind = _norm_kind(norm_type, "grad_norm")
+    if not tensors:
+        return torch.zeros(())
+    _join_wgrad()
+    t = _Tensors(tensors, "grad_norm")
+    return _norm_call("grad_norm", t, t.ptrs, t.sizes, t.codes, t.n, kind)
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """``torch.nn.utils.clip_grad_norm_`` in one call of the library (ccn_grad_clip): every gradient of ``parameters`` is multiplied
+    in place by min(1, max_norm / (norm + 1e-6)); returns the norm before clipping, an fp32 scalar on the device.  The product is taken in
+    32 bits and rounded once to the gradient's type.  A norm that is not finite gives what the formula gives (0 or NaN), or raises with
+    ``error_if_nonfinite`` (which waits for the GPU) before anything is scaled.  Gradients that share memory are refused."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    kind, max_norm = _norm_kind(norm_type, "clip_grad_norm_"), _bound(max_norm, "clip_grad_norm_")
+    if not grads:
+        return torch.zeros(())
+    _join_wgrad()
+    t = _Tensors(grads, "clip_grad_norm_")
+    if error_if_nonfinite:
+        norm = _norm_call("grad_norm", t, t.ptrs, t.sizes, t.codes, t.n, kind)
+        if not math.isfinite(float(norm)):
+            raise RuntimeError("clip_grad_norm_: the norm of the gradients is %r" % float(norm))
+    norm = _norm_call("grad_clip", t, t.ptrs, t.sizes, t.codes, t.n, kind, max_norm)
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, max_norm=None):
+    """One ``torch.optim.Adam`` update, in place, of several contiguous 16-byte aligned fp32 tensors (the flat buckets of FlatAdam).
+    ``max_norm``: the gradients' global norm is bounded as by clip_grad_norm_, but each is scaled as it is read (ccn_adam_clip): they keep
+    their values, and the read and write of a separate clipping pass are saved.  Returns the norm before clipping (an fp32 scalar on the
+    device), or None without ``max_norm``.  ``step``: the 1-based count of this update."""
+    lists = [list(v) for v in (params, grads, exp_avgs, exp_avg_sqs)]
+    step, max_norm = int(step), None if max_norm is None else _bound(max_norm, "adam_step_")
+    if step < 1:
+        raise ValueError("adam_step_: step %d; the first update is step 1" % step)
+    if len(set(map(len, lists))) != 1:
+        raise ValueError("adam_step_: %d parameters, %d gradients, %d and %d moments" % tuple(map(len, lists)))
+    if not lists[0]:
+        return None if max_norm is None else torch.zeros(())
+    for v in lists:
+        if any(t.dtype != torch.float32 for t in v):
+            raise TypeError("adam_step_: fp32 tensors are wanted")
+        if [t.numel() for t in v] != [t.numel() for t in lists[0]] or not all(map(torch.Tensor.is_contiguous, v)):
+            raise ValueError("adam_step_: the tensors of a parameter are contiguous and of one size")
+    tables = [_Tensors(v, "adam_step_") for v in lists]
+    for t in tables:
+        if t.place != tables[0].place:
+            raise ValueError("adam_step_: the tensors of a parameter are on one device")
+        if any(p % 16 for p in t.keep[0]):
+            raise ValueError("adam_step_: a tensor does not start at a multiple of 16 bytes")
+    return _adam(tables, step, lr, betas, eps, weight_decay, max_norm)
+
+
+def _adam(tables, step, lr, betas, eps, weight_decay, max_norm):
+    p, g, m, v = tables
+    rest = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), step)         # (as both entries take them)
+    _join_wgrad()
+    if max_norm is not None:
+        return _norm_call("adam_clip", g, p.ptrs, g.ptrs, m.ptrs, v.ptrs, g.sizes, g.n, *rest, max_norm)
+    from ._lib import call
+    with torch.cuda.device(g.place):
+        for at in zip(*(t.keep[0] for t in tables), g.keep[1]):
+            call("adam_step", *map(ctypes.c_void_p, at[:4]), at[4], *rest)
+
+
 class FlatAdam(torch.optim.Optimizer):
     """``torch.optim.Adam`` (the reference harness' optimiser, src/main.py:56) over the flat buckets of a
     ``GradientAllReduce``: the parameters of a bucket are re-homed into one contiguous buffer laid out like
@@ -249,11 +389,16 @@ class FlatAdam(torch.optim.Optimizer):
     preemption checkpoints (src/main.py:131-141) are interchangeable with the reference's and do not depend on the
     bucket size.
 
+    ``max_norm``: every step bounds the global norm of the gradients (adam_step_); ``grad_norm`` is then the last step's norm before
+    clipping, a scalar on the device.  It is no part of the state dict, whose format stays ``torch.optim.Adam``'s.
+
     Build it after the module sits on its device; ``module.to(...)`` afterwards would detach the views.
     """
 
-    def __init__(self, sync, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
+    def __init__(self, sync, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, max_norm=None):
         self.sync = sync
+        self.max_norm = None if max_norm is None else _bound(max_norm, "FlatAdam")
+        self.grad_norm = None
         defaults = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False,
                         foreach=None, capturable=False, differentiable=False, fused=None)
         self.steps = 0
@@ -284,6 +429,11 @@ class FlatAdam(torch.optim.Optimizer):
         _join_wgrad()
         self.steps += 1
         g = self.param_groups[0]
+        if self.max_norm is not None:
+            flat = list(zip(*((pflat, gflat, m, v) for (gflat, _, _), (pflat, m, v) in zip(self.sync.buckets, self.flat))))
+            self.grad_norm = adam_step_(*flat, self.steps, lr=g["lr"], betas=g["betas"], eps=g["eps"],
+                                        weight_decay=g["weight_decay"], max_norm=self.max_norm)
+            return loss
         for (gflat, _, _), (pflat, m, v) in zip(self.sync.buckets, self.flat):
             call("adam_step", ptr(pflat), ptr(gflat), ptr(m), ptr(v), gflat.numel(), float(g["lr"]), float(g["betas"][0]),
                  float(g["betas"][1]), float(g["eps"]), float(g["weight_decay"]), self.steps)

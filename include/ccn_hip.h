@@ -702,6 +702,38 @@ int ccn_nll_loss_bwd(const float* logits, int64_t ld, const int64_t* target, con
 int ccn_adam_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, int64_t n, float lr, float beta1,
                   float beta2, float eps, float weight_decay, int64_t step, void* stream);
 
+/* Log-probabilities of given classes, the entropy of every row, its best alternatives, and their gradient.
+ * logits: rows x C of `dtype` (0 = fp32, 1 = bf16, 2 = fp16), row stride ld elements (any alignment of the type).  Outputs fp32.
+ * fwd: logprob (rows) of target (0 where target == ignore_index, NaN for another target outside [0, C)), entropy (rows), stats
+ * (2 x rows, nullable: what bwd needs), top_logprob / top_index (rows x top, the `top` largest logits, equal ones by ascending
+ * class; top <= 64, top <= C).  A row of -inf only: logprob -inf, entropy 0.
+ * bwd: dlogits (`dtype`, row stride ldd) = d / d logits of sum(g_logprob logprob) + sum(g_entropy entropy) + sum(g_top top_logprob);
+ * g_logprob and g_entropy are read at row * their stride (0: one value for all rows) and may be null, g_top is rows x top.
+ * Deterministic.  ws: ccn_logprob_workspace_bytes of device memory (0: none needed). */
+size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top);
+int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index,
+                    int top, float* logprob, float* entropy, float* stats, float* top_logprob, int64_t* top_index, void* ws,
+                    size_t ws_bytes, void* stream);
+int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index,
+                    int top, const int64_t* top_index, const float* stats, const float* entropy, const float* g_logprob,
+                    int64_t g_logprob_stride, const float* g_entropy, int64_t g_entropy_stride, const float* g_top, void* dlogits,
+                    int64_t ldd, void* stream);
+
+/* The global norm of n gradients and their clipping.  grads / sizes / dtypes are HOST arrays (addresses of device buffers, their
+ * lengths in values, 0 = fp32 | 1 = bf16 | 2 = fp16; dtypes may be null: all fp32); they are read before the call returns.  kind: 1 =
+ * sum of magnitudes, 2 = square root of the sum of squares, 3 = largest magnitude.  norm: fp32 device scalar, the norm BEFORE
+ * clipping.  clip: every value times min(1, max_norm / (norm + 1e-6)), in place; tensors that share memory are refused.
+ * adam_clip: torch.optim.Adam(amsgrad=False, maximize=False) over n runs of parameters (fp32, 16-byte aligned) with the gradients
+ * scaled the same way as they are read; they are not written.  Norms are summed in double in a fixed order.  ws: ccn_grad_norm_workspace_bytes(n) of device memory. */
+size_t ccn_grad_norm_workspace_bytes(int64_t n);
+int ccn_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, void* ws,
+                  size_t ws_bytes, float* norm, void* stream);
+int ccn_grad_clip(void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, double max_norm, void* ws,
+                  size_t ws_bytes, float* norm, void* stream);
+int ccn_adam_clip(float* const* params, const float* const* grads, float* const* exp_avgs, float* const* exp_avg_sqs,
+                  const int64_t* sizes, int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay,
+                  int64_t step, double max_norm, void* ws, size_t ws_bytes, float* norm, void* stream);
+
 /* ================================================================================================================
  * The entry points SURVEY.md section 8(b) lists as the minimum C-ABI of the hot path (ccn_contract.hip).  Each is a FIXED
  * composition of the kernels declared above, for a host that does not want to sequence them itself; the Python mirror

@@ -1,0 +1,450 @@
+"""loss.token_logprobs on the GPU against its definition in 64 bits: sizes around every border of the kernels, types, strides, masks,
+refused targets, gradients, streams and graphs.
+
+Tolerances, derived.  u = 2^-24 is half a step of fp32, L = ln C.  A weight exp(x - m) carries |x - m| u from the difference's
+rounding, as much again from the product with log2 e, and 2 u from the exponential; a thread adds at most max(64, C / 256) of them one
+after another and a tree of at most 12 levels joins the threads.  S is therefore off by (n + 14 + 2 (|x - m| averaged over p)) u, the
+average being at most L + 1, so log S, a log-probability l and the entropy are off by at most
+    E(v) = u (n + 64 + 4 |v|) (1 + L),   n = max(64, C / 256)
+(the factor 1 + L only the entropy needs, whose W / S is at most L in size).  p is off by a factor of 1 + E(l) + |l| u + 2 u, and a
+gradient by that on its smooth part, u on every sum, and half a step of its own type (half a subnormal step of fp16, 2^-25, at least).
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+
+
+def _score(*a, **k):
+    from curvecloudnet_amd.loss import token_logprobs
+    return token_logprobs(*a, **k)
+
+
+def _definition(x, target, top, ignore=-100):
+    """64 bits, on the CPU: logprob, entropy, top_logprob, top_index, all log-probabilities."""
+    x = x.detach().cpu().double()
+    target = target.cpu().long()
+    best = x.amax(1, keepdim=True)                      # (subtracted first: log C is lost beside the lowest values even in 64 bits)
+    off = x - best
+    empty = torch.isneginf(x).all(1, keepdim=True)
+    logp = torch.where(empty, -math.inf, off - off.exp().sum(1, keepdim=True).log())
+    odd = torch.isnan(x).any(1, keepdim=True) | torch.isposinf(x).any(1, keepdim=True)
+    logp = torch.where(odd, math.nan, logp)
+    p = logp.exp()
+    entropy = -torch.where(p == 0, 0.0, p * logp).sum(1)
+    inside = (target >= 0) & (target < x.size(1))
+    given = logp.gather(1, torch.where(inside, target, 0)[:, None]).squeeze(1)
+    logprob = torch.where(target == ignore, 0.0, torch.where(inside, given, math.nan))
+    order = torch.sort(torch.where(torch.isnan(x), math.inf, x + 0.0), dim=1, descending=True, stable=True).indices
+    # (a NaN comes before an infinity)
+    order = order.gather(1, torch.sort(torch.isnan(x).gather(1, order).int(), dim=1, descending=True, stable=True).indices)[:, :top]
+    return logprob, entropy, logp.gather(1, order), order, logp
+
+
+def _gradient(logp, entropy, target, order, g_lp, g_h, g_top, ignore=-100):
+    target = target.cpu().long()
+    scored = target != ignore
+    inside = (target >= 0) & (target < logp.size(1))
+    g = torch.where(scored, g_lp.cpu().double(), 0.0)
+    g = torch.where(scored & ~inside, math.nan, g)
+    total = g.clone()
+    onehot = torch.zeros_like(logp)
+    onehot.scatter_add_(1, torch.where(inside, target, 0)[:, None], torch.where(inside, g, 0.0)[:, None])
+    if g_top is not None:
+        total = total + g_top.cpu().double().sum(1)
+        onehot.scatter_add_(1, order, g_top.cpu().double())
+    p = logp.exp()
+    smooth = torch.where(p == 0, 0.0, -p * (total[:, None] + g_h.cpu().double()[:, None] * (logp + entropy[:, None])))
+    return smooth, onehot, total
+
+
+def _e(v, c):
+    return U * (max(64, c / 256) + 64 + 4 * v.abs()) * (1 + math.log(c))
+
+
+def _near(a, ref, tol, what):
+    a, ref = a.detach().cpu().double(), ref.double()
+    ref = torch.where(ref < -3.5e38, -math.inf, ref)                    # (below the range of the outputs' type)
+    assert a.shape == ref.shape, what
+    same = (a == ref) | (torch.isnan(a) & torch.isnan(ref))
+    off = (a - ref).abs()
+    bad = ~(same | (off <= tol))
+    assert not bool(bad.any()), "%s: %d values off, worst %.3g, first at %s: %r for %r" % (
+        what, int(bad.sum()), float(off[bad].max()), bad.nonzero()[0].tolist(), float(a[bad][0]), float(ref[bad][0]))
+
+
+def _check(x, target, top, ignore=-100, r=None):
+    r = _score(x, target, top=top, ignore_index=ignore) if r is None else r
+    lp, h, best, order, logp = _definition(x, target, top, ignore)
+    c = x.size(1)
+    assert r.logprob.dtype == r.entropy.dtype == torch.float32
+    _near(r.logprob, lp, _e(lp, c), "logprob")
+    _near(r.entropy, h, _e(h, c), "entropy")
+    if top:
+        assert r.top_index.dtype == torch.int64
+        assert torch.equal(r.top_index.cpu(), order), "alternatives"
+        _near(r.top_logprob, best, _e(best, c), "alternatives' log-probabilities")
+    else:
+        assert r.top_logprob is None and r.top_index is None
+    return lp, h, best, order, logp
+
+
+def _check_gradient(x, target, top, ignore=-100, seed=1, use=(True, True, True)):
+    gen = torch.Generator().manual_seed(seed)
+    rows, c = x.shape
+    g_lp, g_h = torch.randn(rows, generator=gen) * use[0], torch.randn(rows, generator=gen) * use[1]
+    g_top = torch.randn(rows, top, generator=gen) if top and use[2] else None
+    leaf = x.detach().requires_grad_(True)
+    r = _score(leaf, target, top=top, ignore_index=ignore)
+    _, h, _, order, logp = _check(x, target, top, ignore, r)
+    outs, gs = [], []
+    for on, out, g in zip(use, (r.logprob, r.entropy, r.top_logprob), (g_lp, g_h, g_top)):
+        if on and out is not None:
+            outs.append(out)
+            gs.append(g.to(DEV))
+    (d,) = torch.autograd.grad(outs, leaf, gs)
+    assert d.dtype == x.dtype and d.shape == x.shape
+    smooth, onehot, total = _gradient(logp, h, target, order, g_lp, g_h, g_top, ignore)
+    ref = smooth + onehot
+    lsafe = torch.where(torch.isinf(logp), 0.0, logp)
+    p = logp.exp()
+    factor = _e(lsafe, c) + U * (lsafe.abs() + 4)
+    gh = g_h.double()[:, None].abs()
+    sums = total[:, None].abs() + (g_lp.abs().double()[:, None] + (0 if g_top is None else g_top.abs().double().sum(1, keepdim=True)))
+    tol = p * (sums + gh * (lsafe.abs() + h[:, None].abs())) * (factor + 70 * U)            # (up to 64 gradients in one sum)
+    tol = tol + p * gh * (_e(lsafe, c) + _e(h, c)[:, None])
+    tol = tol + U * (onehot.abs() + ref.abs()) * 66
+    tol = tol + ref.abs() * torch.finfo(x.dtype).eps / 2 + (2.0 ** -25 if x.dtype == torch.float16 else 0.0)
+    # (weights below the smallest normal number are zero)
+    tol = tol + (sums + gh * 200) * 2.0 ** -126
+    _near(d, ref, torch.nan_to_num(tol, nan=0.0), "gradient")
+    return d
+
+
+def _logits(rows, c, dtype, seed=0, spread=3.0, pad=0, shift=0):
+    gen = torch.Generator().manual_seed(seed + 7 * rows + c)
+    wide = (torch.randn(rows, c + pad + shift, generator=gen) * spread).to(dtype).to(DEV)
+    return wide[:, shift: shift + c]
+
+
+def _target(rows, c, seed=0):
+    return torch.randint(0, c, (rows,), generator=torch.Generator().manual_seed(seed + rows + c)).to(DEV)
+
+
+SIZES = [(1, 1), (1, 2), (2, 1), (3, 5), (257, 20), (1000, 20), (64, 55), (513, 55), (5, 63), (5, 64), (5, 65), (70, 66), (7, 127),
+         (9, 255), (9, 256), (9, 257), (33, 300), (5, 511), (5, 513), (4, 1000), (4, 1023), (4, 1025), (3, 2047), (3, 2048), (3, 2049),
+         (2, 4095), (2, 4097), (2, 8191), (2, 8193), (3, 16385), (1, 32769), (1, 50021), (2, 65535), (2, 65537), (300, 4099), (1, 262144),
+         (1, 300007)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,c", SIZES)
+def test_scores_and_gradient_over_sizes(rows, c, dtype):
+    x, t = _logits(rows, c, dtype), _target(rows, c)
+    for top in sorted({0, min(c, 1), min(c, 5), min(c, 20)}):
+        _check(x, t, top)
+    _check_gradient(x, t, 0)
+    _check_gradient(x, t, min(c, 5))
+
+
+@pytest.mark.parametrize("rows,c", [(3, 64), (40, 64), (3, 65), (3, 100), (2, 2048), (3, 9000), (1, 70000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_many_alternatives(rows, c, dtype):
+    x, t = _logits(rows, c, dtype), _target(rows, c)
+    for top in (31, 32, 33, 63, 64):
+        _check(x, t, top)
+    _check_gradient(x, t, 64)
+
+
+def test_every_class_is_an_alternative():
+    for rows, c in ((1, 1), (5, 2), (300, 20), (7, 33), (3, 64)):
+        x, t = _logits(rows, c, torch.float32), _target(rows, c)
+        lp, _, _, order, _ = _check(x, t, c)
+        assert torch.equal(order.sort(1).values, torch.arange(c).expand(rows, c))
+        _check_gradient(x, t, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("c", [20, 64, 65, 1500, 5000, 40000])
+def test_strides_and_alignments(c, dtype):
+    rows, top = 5, 4
+    t = _target(rows, c)
+    for pad, shift in ((1, 0), (0, 1), (3, 5), (8, 0), (7, 3)):
+        x = _logits(rows, c, dtype, pad=pad, shift=shift)
+        assert x.stride(0) == c + pad + shift
+        _check_gradient(x, t, top)
+    flat = _logits(1, rows * c + 3, dtype)[0]
+    for k in range(4):
+        _check_gradient(flat[k: k + rows * c].view(rows, c), t, top)
+    x = _logits(c, rows, dtype).t()                                     # columns that are not adjacent
+    assert x.stride() == (1, rows)
+    _check_gradient(x, t, top)
+    _check(_logits(1, c, dtype).expand(rows, c), t, top)               # one row for all
+    _check(_logits(2 * rows, c, dtype)[::2], t, top)
+    _check(_logits(2 * rows, c, dtype).flip(0)[1::2], t, top)
+
+
+def test_shapes_and_target_types():
+    x, t = _logits(24, 30, torch.float32), _target(24, 30)
+    lp, h, best, order, _ = _definition(x, t, 3)
+    r = _score(x.view(2, 3, 4, 30), t.view(2, 3, 4).to(torch.int32), top=3)
+    assert r.logprob.shape == r.entropy.shape == (2, 3, 4) and r.top_logprob.shape == r.top_index.shape == (2, 3, 4, 3)
+    _check(x, t, 3, r=type(r)(r.logprob.view(-1), r.entropy.view(-1), r.top_logprob.view(-1, 3), r.top_index.view(-1, 3)))
+    one = _score(x[5], t[5], top=3)
+    assert one.logprob.shape == () and one.top_index.shape == (3,)
+    assert torch.equal(one.top_index.cpu(), order[5]) and float(one.logprob) == float(r.logprob.view(-1)[5])
+    # a slice of a larger batch, an axis moved: no copy of the caller's is needed
+    y = _logits(6 * 9, 30, torch.float32).view(6, 9, 30)[1:5, 2:8].requires_grad_(True)
+    k = _target(24, 30).view(4, 6)
+    s = _score(y, k)
+    (d,) = torch.autograd.grad(s.logprob.sum(), y)
+    ref = torch.softmax(y.detach().double(), -1)
+    ref = torch.nn.functional.one_hot(k, 30).double() - ref
+    _near(d, ref.cpu(), 300 * U, "gradient of a slice")
+    for shape in ((0, 30), (2, 0, 30)):
+        e = torch.empty(shape, device=DEV, requires_grad=True)
+        s = _score(e, torch.empty(shape[:-1], dtype=torch.int64, device=DEV), top=2)
+        assert s.logprob.shape == shape[:-1] and s.top_index.shape == shape[:-1] + (2,)
+        (d,) = torch.autograd.grad(s.logprob.sum() + s.top_logprob.sum(), e)
+        assert d.shape == shape
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("c", [7, 64, 65, 700, 3000, 20000, 70001])
+def test_equal_logits_come_by_class(c, dtype):
+    rows, top = 6, min(c, 33)
+    t = _target(rows, c)
+    x = torch.zeros(rows, c, dtype=dtype, device=DEV)
+    x[1] = -5.0
+    x[2, ::2] = -0.0                                                    # -0 and 0 are equal
+    x[3] = torch.arange(c, device=DEV).div(max(1, c // 4), rounding_mode="floor").to(dtype)
+    x[4] = torch.arange(c, device=DEV).div(max(1, c // 4), rounding_mode="floor").flip(0).to(dtype)
+    x[5] = (torch.arange(c, device=DEV) % 3).to(dtype)
+    _check_gradient(x, t, top)
+    _check(x, t, min(c, 64))
+
+
+@pytest.mark.parametrize("c", [64, 65, 2048, 5000, 40000])
+def test_ordered_rows(c):
+    """Rising, falling and one-lane-heavy rows: the alternatives lie next to one another, at the end, at the start, or a stride apart."""
+    x = torch.empty(5, c, device=DEV)
+    x[0] = torch.arange(c, device=DEV) * (30.0 / c)
+    x[1] = x[0].flip(0)
+    x[2] = torch.where(torch.arange(c, device=DEV) % 64 == 13, 20.0, 0.0) + x[0] * 0.01
+    x[3] = torch.where(torch.arange(c, device=DEV) % 256 == 7, 20.0, 0.0) - x[0] * 0.01
+    x[4] = torch.where((torch.arange(c, device=DEV) >= c // 2) & (torch.arange(c, device=DEV) < c // 2 + 64), 25.0, 0.0) + x[0] * 0.1
+    for top in (1, 20, 64):
+        _check(x, _target(5, c), top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("c", [5, 20, 64, 65, 1000, 5001, 40000])
+def test_masked_rows(c, dtype):
+    rows, top, low = 12, 5, torch.finfo(dtype).min
+    x = _logits(rows, c, dtype).clone()
+    t = _target(rows, c)
+    x[0] = -math.inf                                                    # nothing left
+    x[1] = low                                                          # the type's lowest value throughout: uniform
+    x[2] = -math.inf
+    x[2, c - 1] = 1.5                                                   # one class left
+    x[3] = low
+    x[3, 0] = torch.finfo(dtype).max                                    # the widest difference
+    x[4, : c // 2] = -math.inf
+    x[5, c // 2:] = low
+    x[6] = -math.inf
+    x[6, 0], x[6, c - 1] = low, low
+    x[7, 1::2] = -math.inf
+    t[2], t[3], t[8] = c - 1, 0, -100
+    t[9] = c - 1
+    x[9, c - 1] = -math.inf                                             # the given class has no probability
+    x[10] = -math.inf
+    t[10] = -100
+    r = _score(x, t, top=top)
+    assert float(r.logprob[0]) == -math.inf and float(r.entropy[0]) == 0.0 and float(r.logprob[8]) == 0.0
+    assert r.top_index[0].tolist() == list(range(top)) and float(r.logprob[9]) == -math.inf
+    _check(x, t, top)
+    d = _check_gradient(x, t, top)
+    assert bool(torch.isfinite(d).all())
+    d = _check_gradient(x, t, 0)
+    assert float(d[10].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("c", [5, 64, 65, 1000, 5001, 40000])
+def test_nan_and_infinity_stay_in_their_rows(c):
+    rows = 6
+    x, t = _logits(rows, c, torch.float32).clone(), _target(rows, c)
+    x[1, c // 2] = math.nan
+    x[2, c - 1] = math.inf
+    x[3] = math.nan
+    x[4, 0], x[4, c - 1], x[4, c // 2] = math.inf, math.inf, -math.inf
+    r = _score(x, t, top=4)
+    assert torch.isnan(r.logprob[1:5]).all() and torch.isnan(r.entropy[1:5]).all() and torch.isnan(r.top_logprob[1:5]).all()
+    _check(x, t, 4)
+    leaf = x.clone().requires_grad_(True)
+    (d,) = torch.autograd.grad(_score(leaf, t).logprob.sum(), leaf)
+    assert torch.isfinite(d[[0, 5]]).all() and torch.isnan(d[1:5]).any(1).all()
+
+
+def test_targets_that_are_not_scored():
+    for c in (20, 65, 3000):
+        rows = 9
+        x, t = _logits(rows, c, torch.float32), _target(rows, c)
+        t[1], t[2], t[3], t[4], t[5] = -100, c, -1, 2 ** 40, -2 ** 62
+        r = _score(x, t, top=2)
+        assert float(r.logprob[1]) == 0.0 and torch.isnan(r.logprob[2:6]).all() and torch.isfinite(r.entropy).all()
+        _check(x, t, 2)
+        leaf = x.detach().requires_grad_(True)
+        (d,) = torch.autograd.grad(_score(leaf, t).logprob.sum(), leaf)
+        assert float(d[1].abs().max()) == 0.0 and torch.isnan(d[2:6]).any(1).all() and torch.isfinite(d[[0, 6, 7, 8]]).all()
+        (d,) = torch.autograd.grad(_score(leaf, t).entropy.sum(), leaf)                 # (a bad target is no part of the entropy)
+        assert torch.isfinite(d).all()
+        # a class of the range that is not scored
+        t = _target(rows, c) % 3
+        _check_gradient(x, t, 2, ignore=0)
+
+
+@pytest.mark.parametrize("use", [(True, False, False), (False, True, False), (False, False, True), (True, False, True)])
+@pytest.mark.parametrize("c", [20, 500, 9001])
+def test_gradient_of_each_output_alone(c, use):
+    _check_gradient(_logits(11, c, torch.float32), _target(11, c), 6, use=use)
+
+
+def test_the_given_class_among_the_alternatives_and_gradients_broadcast():
+    for c in (20, 700, 5000):
+        x = _logits(8, c, torch.bfloat16)
+        t = x.float().argmax(1)
+        _check_gradient(x, t, 3)
+        leaf = x.detach().requires_grad_(True)
+        r = _score(leaf, t, top=3)
+        loss = -r.logprob.mean() + 0.5 * r.entropy.mean() + r.top_logprob.mean()        # (gradients of stride 0)
+        (a,) = torch.autograd.grad(loss, leaf)
+        r = _score(leaf, t, top=3)
+        n = float(x.size(0))
+        (b,) = torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], leaf,
+                                   [torch.full_like(r.logprob, -1 / n), torch.full_like(r.entropy, 0.5 / n),
+                                    torch.full_like(r.top_logprob, 1 / (3 * n))])
+        assert torch.equal(a, b)
+
+
+def test_gradient_against_differences():
+    """Central differences of the definition in 64 bits: their own error, h^2 / 6 times the third derivative, is below 1e-8; the
+    kernel's is at most p (n + 64 + 4 |l| + ...) u times gradients of up to 4, in all less than 4e-5."""
+    x, t = _logits(2, 9, torch.float32, spread=1.0), _target(2, 9)
+    gen = torch.Generator().manual_seed(5)
+    g = [torch.randn(2, generator=gen), torch.randn(2, generator=gen), torch.randn(2, 3, generator=gen)]
+
+    def value(y):
+        lp, h, best, _, _ = _definition(y, t, 3)
+        return float((lp * g[0]).sum() + (h * g[1]).sum() + (best * g[2]).sum())
+
+    leaf = x.detach().requires_grad_(True)
+    r = _score(leaf, t, top=3)
+    (d,) = torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], leaf, [v.to(DEV) for v in g])
+    step, base = 1e-4, x.cpu().double()
+    for i in range(2):
+        for j in range(9):
+            up, down = base.clone(), base.clone()
+            up[i, j] += step
+            down[i, j] -= step
+            assert abs((value(up) - value(down)) / (2 * step) - float(d[i, j])) < 4e-5, (i, j)
+
+
+def test_rows_behind_a_long_way():
+    """Rows that start more than 2^31 values behind the first."""
+    ld, c = (1 << 30) + 24, 100
+    base = torch.empty(2 * ld + 5000, dtype=torch.bfloat16, device=DEV)
+    for classes in (c, 5000):
+        x = base.as_strided((3, classes), (ld, 1))
+        x.copy_(_logits(3, classes, torch.bfloat16))
+        assert 2 * ld > 2 ** 31
+        _check_gradient(x, _target(3, classes), 5)
+
+
+def test_many_rows():
+    """More rows than workgroups fit at once, checked against torch on the device."""
+    for rows, c, dtype in ((400070, 20, torch.float32), (70001, 130, torch.bfloat16), (9001, 2500, torch.float16)):
+        gen = torch.Generator(device=DEV).manual_seed(c)
+        x = (torch.randn(rows, c, generator=gen, device=DEV) * 3).to(dtype).requires_grad_(True)
+        t = torch.randint(0, c, (rows,), generator=gen, device=DEV)
+        r = _score(x, t, top=2)
+        logp = torch.log_softmax(x.detach().double(), 1)
+        lp = logp.gather(1, t[:, None]).squeeze(1)
+        _near(r.logprob, lp.cpu(), _e(lp, c).cpu(), "logprob")
+        (d,) = torch.autograd.grad(r.logprob.sum(), x)
+        ref = torch.nn.functional.one_hot(t, c).double() - logp.exp()
+        tol = 400 * U + ref.abs() * (torch.finfo(dtype).eps / 2) + 2.0 ** -25
+        assert bool(((d.double() - ref).abs() <= tol).all())
+
+
+def test_same_bits_every_time_and_two_streams_at_once():
+    x, t = _logits(37, 40001, torch.bfloat16), _target(37, 40001)
+    y, k = _logits(5000, 20, torch.float32), _target(5000, 20)
+    first = [_score(x, t, top=9), _score(y, k, top=3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            a = _score(x, t, top=9)
+        b = _score(y, k, top=3)
+        torch.cuda.current_stream().wait_stream(side)
+        for got, want in zip((a, b), first):
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_captured_forward_and_backward():
+    """Two graphs captured from the same code, replayed in turn with eager work and new logits between the replays."""
+    cases = []
+    for rows, c, dtype in ((50, 20, torch.float32), (3, 50021, torch.bfloat16), (40, 3000, torch.float16)):
+        x = _logits(rows, c, dtype).clone().requires_grad_(True)
+        t = _target(rows, c)
+        g = torch.randn(rows, device=DEV)
+
+        def step(x=x, t=t, g=g):
+            r = _score(x, t, top=4)
+            (d,) = torch.autograd.grad([r.logprob, r.entropy], x, [g, g])
+            return [v.detach() for v in (*r, d)]                        # (no autograd graph outlives a step)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        cases.append((graph, out, step, x))
+    for turn in range(4):
+        for graph, out, step, x in cases:
+            with torch.no_grad():
+                x.copy_(torch.randn(x.shape, device=DEV) * (turn + 1))
+            want = step()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+
+
+def test_rows_beside_the_outputs_stay():
+    """The gradient's padding columns and the rows of the outputs' neighbours are not written."""
+    from curvecloudnet_amd._lib import call, ptr
+    for rows, c, dtype, code in ((5, 7, torch.float32, 0), (5, 65, torch.float16, 2), (2, 5001, torch.bfloat16, 1)):
+        x, t = _logits(rows, c, dtype), _target(rows, c)
+        f = [torch.full((rows + 2,), 7.0, device=DEV) for _ in range(2)]
+        stats, best = torch.full((rows + 2, 2), 7.0, device=DEV), torch.full((rows + 2, 3), 7.0, device=DEV)
+        index = torch.full((rows + 2, 3), 7, dtype=torch.int64, device=DEV)
+        from curvecloudnet_amd._lib import lib, workspace
+        n = lib().ccn_logprob_workspace_bytes(rows, c, 3)
+        call("logprob_fwd", ptr(x), code, x.stride(0), ptr(t), rows, c, -100, 3, ptr(f[0][1:]), ptr(f[1][1:]), ptr(stats[1:]),
+             ptr(best[1:]), ptr(index[1:]), ptr(workspace(n, DEV)), n)
+        for v in f + [stats, best, index]:
+            assert bool((v[0] == 7).all()) and bool((v[-1] == 7).all())
+        _check(x, t, 3, r=type(_score(x, t))(f[0][1:-1], f[1][1:-1], best[1:-1], index[1:-1]))
+        d = torch.full((rows + 2, c + 5), 7.0, dtype=dtype, device=DEV)
+        g = torch.ones(rows, device=DEV)
+        call("logprob_bwd", ptr(x), code, x.stride(0), ptr(t), rows, c, -100, 0, None, ptr(stats[1:]), ptr(f[1][1:]), ptr(g), 1,
+             None, 0, None, ptr(d[1:]), d.stride(0))
+        assert bool((d[0] == 7).all()) and bool((d[-1] == 7).all()) and bool((d[:, c:] == 7).all())
+        assert bool((d[1:-1, :c] != 7).all())
