@@ -11,6 +11,8 @@
 // Rows that no formula covers: every logit -inf -> logprob -inf, entropy 0, gradient 0 (but for the one-hot terms); a NaN or
 // +inf anywhere -> NaN everywhere (a NaN counts as the largest logit among the alternatives).  target == ignore_index -> logprob 0
 // and no gradient from it; any other target outside [0, C) -> NaN for both, and nothing is read there.
+#include <limits.h>
+
 #include "ccn_common.h"
 
 namespace {
@@ -18,10 +20,15 @@ namespace {
 constexpr int LP_TPB = 256;
 constexpr int LP_TOP_MAX = 64;
 constexpr float LP_LOG2E = 1.44269504088896340736f;
+constexpr float LP_FAR = -1000.f;           // differences below it weigh nothing; -inf, and -inf - -inf, become it
 
-// e^d for d <= 0.  The product with log2(e) is off by at most |d| 2^-24 relative, which a weight of e^d turns into less than
-// 2^-25 of the row's sum; results below 2^-126 are zero.
+// e^d for LP_FAR <= d <= 0.  The product with log2(e) is off by at most |d| 2^-24 relative, which a weight of e^d turns into less
+// than 2^-25 of the row's sum; results below 2^-126 are zero.
 __device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * LP_LOG2E); }
+// v - base of a logit that may be -inf or NaN.  A NaN or +inf is not carried here: the row's maximum tells (lp_finish).
+__device__ __forceinline__ float lp_diff(float v, float base) { return fmaxf(v - base, LP_FAR); }
+// (of two values one of which is NaN: NaN)
+__device__ __forceinline__ float lp_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // Order of the alternatives as unsigned numbers: larger logit first, NaN above all, -0 equal to 0; then the lower class.
 __device__ __forceinline__ uint64_t lp_key(float v, uint32_t c) {
@@ -36,94 +43,464 @@ __device__ __forceinline__ float lp_key_value(uint64_t k) {
 }
 __device__ __forceinline__ int64_t lp_key_class(uint64_t k) { return (int64_t)(uint32_t)~(uint32_t)k; }
 
-// The row's results from its statistics.
+// The row's results from its statistics.  m: the maximum, NaN where a logit is.
 struct LpRow {
   float base, log_total, entropy;           // logprob of a logit v: (v - base) - log_total
 };
 __device__ __forceinline__ LpRow lp_finish(float m, float total, float weighted) {
   LpRow r;
-  if (total == 0.f) {                       // every logit -inf
+  if (m == -INFINITY) {                     // every logit -inf
     r.base = 0.f;
     r.log_total = INFINITY;                 // (x - base) - log_total = -inf for every class
     r.entropy = 0.f;
+  } else if (!(m < INFINITY)) {
+    r.base = 0.f;
+    r.log_total = r.entropy = NAN;
   } else {
-    r.base = m == -INFINITY ? 0.f : m;
+    r.base = m;
     r.log_total = logf(total);
     r.entropy = r.log_total - weighted / total;
   }
   return r;
 }
 
+// 16 bytes of a row, at any alignment of the type.
+typedef uint32_t lp_u32x4 __attribute__((ext_vector_type(4)));
+template <int T> struct LpVec;
+template <> struct LpVec<0> {
+  static constexpr int N = 4;
+  static constexpr uint32_t FILL = 0xff800000u;      // -inf
+  typedef lp_u32x4 mem __attribute__((aligned(4)));
+};
+template <> struct LpVec<1> {
+  static constexpr int N = 8;
+  static constexpr uint32_t FILL = 0xff80ff80u;
+  typedef lp_u32x4 mem __attribute__((aligned(2)));
+};
+template <> struct LpVec<2> {
+  static constexpr int N = 8;
+  static constexpr uint32_t FILL = 0xfc00fc00u;
+  typedef lp_u32x4 mem __attribute__((aligned(2)));
+};
 template <int T>
-__global__ __launch_bounds__(LP_TPB) void logprob_fwd_kernel(const void* __restrict__ x, int64_t ld,
-                                                             const int64_t* __restrict__ target, int C, int64_t ignore, int top,
-                                                             float* __restrict__ logprob, float* __restrict__ entropy,
-                                                             float2* __restrict__ stats, float* __restrict__ top_logprob,
-                                                             int64_t* __restrict__ top_index) {
-  __shared__ float red[2][LP_TPB / 64];
-  __shared__ uint64_t kred[LP_TPB / 64];
-  const int64_t row = blockIdx.x, at = row * ld;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  float m = -INFINITY;
-  for (int c = threadIdx.x; c < C; c += LP_TPB) m = fmaxf(m, ld_el<T>(x, at + c));
+__device__ __forceinline__ float lp_el(const lp_u32x4& r, int i) {
+  if (T == 0) return __uint_as_float(r[i]);
+  if (T == 1) return __uint_as_float((i & 1) ? (r[i >> 1] & 0xffff0000u) : (r[i >> 1] << 16));
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i >> 1] >> (16 * (i & 1))));
+}
+template <int T>
+__device__ __forceinline__ lp_u32x4 lp_load(const void* __restrict__ x, int64_t at) {
+  constexpr int B = T == 0 ? 4 : 2;
+  return *reinterpret_cast<const typename LpVec<T>::mem*>(reinterpret_cast<const char*>(x) + at * B);
+}
+// ... of which only the first n values are the row's: the others are -inf and not read.
+template <int T>
+__device__ __forceinline__ lp_u32x4 lp_load_part(const void* __restrict__ x, int64_t at, int n) {
+  constexpr int V = LpVec<T>::N;
+  lp_u32x4 r = {LpVec<T>::FILL, LpVec<T>::FILL, LpVec<T>::FILL, LpVec<T>::FILL};
+  if (n >= V) return lp_load<T>(x, at);
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  if (lane == 0) red[0][w] = m;
-  __syncthreads();
-  for (int k = 0; k < LP_TPB / 64; ++k) m = fmaxf(m, red[0][k]);
-  __syncthreads();
-  const float base = m == -INFINITY ? 0.f : m;
-  float total = 0.f, weighted = 0.f;
-  for (int c = threadIdx.x; c < C; c += LP_TPB) {
-    const float d = ld_el<T>(x, at + c) - base, e = lp_exp(d);
-    total += e;
-    weighted += e > 0.f ? e * d : 0.f;
-  }
+  for (int i = 0; i < V; ++i)
+    if (i < n) {
+      if (T == 0) {
+        r[i] = reinterpret_cast<const uint32_t*>(x)[at + i];
+      } else {
+        const uint32_t v = reinterpret_cast<const uint16_t*>(x)[at + i];
+        r[i >> 1] = (i & 1) ? ((r[i >> 1] & 0xffffu) | (v << 16)) : ((r[i >> 1] & 0xffff0000u) | v);
+      }
+    }
+  return r;
+}
+
+// (what was computed from the values is computed again where it is rarely needed, and not kept in registers until then)
+template <int N>
+__device__ __forceinline__ void lp_forget(lp_u32x4 (&raw)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(raw[j]));
+}
+
+// ---- sorted lists of 64 keys, one to a lane, descending
+
+__device__ __forceinline__ uint64_t lp_shfl_xor(uint64_t v, int d) { return __shfl_xor((unsigned long long)v, d, 64); }
+
+__device__ __forceinline__ uint64_t lp_sort64(uint64_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d >= 1; d >>= 1) {
+      const uint64_t o = lp_shfl_xor(v, d);
+      const bool larger = ((lane & size) == 0) == ((lane & d) == 0);
+      v = (o > v) == larger ? o : v;
+    }
+  return v;
+}
+// The 64 largest of two lists: the larger of each pair (i, 63 - i) are they, and fall and rise; six steps put them in order.
+__device__ __forceinline__ uint64_t lp_merge64(uint64_t a, uint64_t b) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t o = __shfl((unsigned long long)b, 63 - lane, 64);
+  uint64_t v = a > o ? a : o;
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) {
-    total += __shfl_xor(total, d, 64);
-    weighted += __shfl_xor(weighted, d, 64);
+    const uint64_t p = lp_shfl_xor(v, d);
+    v = (p > v) == ((lane & d) == 0) ? p : v;
   }
+  return v;
+}
+// Lane k - 1 of the lane values in descending order (NaN first), as a value.
+__device__ __forceinline__ float lp_kth_lane(float m, int k) {
+  const int lane = threadIdx.x & 63;
+  int v = __float_as_int(m + 0.0f);
+  if (m != m) v = 0x7f800001;
+  v ^= (v >> 31) & 0x7fffffff;
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d >= 1; d >>= 1) {
+      const int o = __shfl_xor(v, d, 64);
+      const bool larger = ((lane & size) == 0) == ((lane & d) == 0);
+      v = larger ? max(v, o) : min(v, o);
+    }
+  v = __shfl(v, k - 1, 64);
+  v ^= (v >> 31) & 0x7fffffff;
+  return __int_as_float(v);
+}
+
+// ---- rows of more than 64 classes: NW waves hold NW * 2048 logits of a row at a time in registers (32 a thread), take their maximum,
+// and add weights relative to the maximum so far: one pass over the row, one rescaling per 32 logits of a thread.
+//
+// Alternatives: among the first logits held, the top-th largest of a wave's 64 thread maxima is a lower bound of the top-th largest of
+// them all, and hardly more than `top` reach it.  They are put into shared memory, and wave 0 sorts them (64 at a time, merged into the
+// best so far).  From then on a thread looks at its logits again only if its maximum beats the last of the best: a row of random
+// logits costs a sort at its start and hardly anything later.  Where more qualify than there is room for (equal logits, rising rows), the
+// rest is looked at again after each merge, against the new last of the best: every turn settles LP_ROOM of them at least.
+constexpr int LP_HOLD = 32;
+
+template <int NW>
+struct LpShared {
+  static constexpr int ROOM = NW == 4 ? 1024 : 256;
+  uint64_t cand[ROOM];
+  uint64_t last_key;
+  float last;
+  int count, any;
+  float red[2][NW];
+};
+
+template <int NW>
+__device__ __forceinline__ void lp_sync() {
+  if (NW == 1) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+template <int NW>
+__device__ __forceinline__ bool lp_any(bool v) {
+  if (NW == 1) return __builtin_amdgcn_ballot_w64(v) != 0;
+  return __syncthreads_or(v) != 0;
+}
+
+// The class of the e-th logit that a thread holds.
+template <int T, int NT>
+__device__ __forceinline__ int lp_class(int c0, int tid, int e) {
+  constexpr int V = LpVec<T>::N;
+  return c0 + ((e / V) * NT + tid) * V + e % V;
+}
+
+template <int T, int NW, bool TOP>
+__global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
+                                                              const int64_t* __restrict__ target, int64_t rows, int C,
+                                                              int64_t ignore, int top, int parts, int part_tiles,
+                                                              float* __restrict__ logprob, float* __restrict__ entropy,
+                                                              float2* __restrict__ stats, float* __restrict__ top_logprob,
+                                                              int64_t* __restrict__ top_index, float4* __restrict__ part_stats,
+                                                              uint64_t* __restrict__ part_keys) {
+  constexpr int NT = NW * 64, V = LpVec<T>::N, NJ = LP_HOLD / V, TILE = NT * LP_HOLD;
+  __shared__ LpShared<NW> shared[4 / NW];
+  LpShared<NW>& sh = shared[NW == 4 ? 0 : threadIdx.x >> 6];
+  const int tid = NW == 4 ? threadIdx.x : threadIdx.x & 63, lane = threadIdx.x & 63, wave = NW == 4 ? threadIdx.x >> 6 : 0;
+  const int64_t unit = NW == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = NW == 4 ? blockIdx.x / (unsigned)parts : unit;
+  const int part = NW == 4 ? (int)(blockIdx.x % (unsigned)parts) : 0;
+  if (NW == 1 && row >= rows) return;                // (a whole wave, and no barrier of the workgroup below)
+  const int64_t at = row * ld;
+  const int beg = part * part_tiles * TILE, end = (int)min((int64_t)C, (int64_t)beg + (int64_t)part_tiles * TILE);
+  // the given class's logit, early: its latency passes beside the row
+  const int64_t t = target[row];
+  float given = 0.f;
+  if (parts == 1 && t >= 0 && t < C) given = ld_el<T>(x, at + t);
+
+  float m = -INFINITY, s = 0.f, w = 0.f;
+  uint64_t best = 0;                                 // (wave 0's list)
+  if (TOP) {
+    if (tid == 0) sh.count = 0;
+    lp_sync<NW>();
+  }
+  for (int c0 = beg; c0 < end; c0 += TILE) {
+    const int n = end - c0;
+    lp_u32x4 raw[NJ];
+    if (n >= TILE) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) raw[j] = lp_load<T>(x, at + c0 + (j * NT + tid) * V);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, at + c0 + (j * NT + tid) * V, n - (j * NT + tid) * V);
+    }
+    float tm = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (j * NT * V < n) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) tm = lp_max(lp_max(tm, lp_el<T>(raw[j], i)), lp_el<T>(raw[j], i + 1));
+      }
+    const float mn = lp_max(m, tm), dm = lp_diff(m, mn), f = lp_exp(dm);
+    w = f * (w + dm * s);
+    s *= f;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (j * NT * V < n) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = lp_diff(lp_el<T>(raw[j], i), mn), e = lp_exp(d);
+          s += e;
+          w = __builtin_fmaf(e, d, w);
+        }
+      }
+    if (TOP) {
+      const bool first = c0 == beg;
+      float limit;
+      if (first) {
+        limit = lp_kth_lane(tm, top);
+        if (NW > 1) {
+          if (lane == 0) sh.red[0][wave] = limit;
+          lp_sync<NW>();
+#pragma unroll
+          for (int k = 0; k < NW; ++k) limit = lp_max(limit, sh.red[0][k]);
+        }
+      } else {
+        limit = sh.last;
+      }
+      // (not below the limit; later ones have to beat it: an equal logit of a higher class comes behind.  A NaN passes.)
+      bool more = first ? !(tm < limit) : !(tm <= limit);
+      if (lp_any<NW>(more)) {
+        lp_forget(raw);
+        uint32_t pending = 0;
+        if (more) {
+#pragma unroll
+          for (int e = 0; e < LP_HOLD; ++e) {
+            const float v = lp_el<T>(raw[e / V], e % V);
+            const int c = ((e / V) * NT + tid) * V + e % V;
+            if ((first ? !(v < limit) : !(v <= limit)) && c < n) pending |= 1u << e;
+          }
+        }
+        do {
+          if (pending) {                               // (few: read again, from a cache, rather than picked out of registers)
+            const int want = __builtin_popcount(pending), to = atomicAdd(&sh.count, want);
+            for (int k = to; k < min(to + want, LpShared<NW>::ROOM); ++k) {
+              const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(pending));
+              sh.cand[k] = lp_key(ld_el<T>(x, at + c), (uint32_t)c);
+              pending &= pending - 1;
+            }
+          }
+          lp_sync<NW>();
+          if (wave == 0) {
+            const int got = min(sh.count, LpShared<NW>::ROOM);
+            for (int b = 0; b < got; b += 64) best = lp_merge64(best, lp_sort64(b + lane < got ? sh.cand[b + lane] : 0));
+            const uint64_t k = __shfl((unsigned long long)best, top - 1, 64);
+            if (lane == 0) {
+              sh.last_key = k;
+              sh.last = k ? lp_key_value(k) : -INFINITY;
+              sh.count = 0;
+            }
+          }
+          lp_sync<NW>();
+          for (uint32_t left = pending; left; left &= left - 1) {
+            const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(left));
+            if (lp_key(ld_el<T>(x, at + c), (uint32_t)c) < sh.last_key) pending &= ~(left & -left);
+          }
+        } while (lp_any<NW>(pending != 0));
+      }
+    }
+  }
+  // the threads' statistics joined
+  float all = m;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) all = lp_max(all, __shfl_xor(all, d, 64));
+  if (NW > 1) {
+    if (lane == 0) sh.red[0][wave] = all;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NW; ++k) all = lp_max(all, sh.red[0][k]);
+    __syncthreads();
+  }
+  const float dm = lp_diff(m, all), f = lp_exp(dm);
+  w = f * (w + dm * s);
+  s *= f;
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    s += __shfl_xor(s, d, 64);
+    w += __shfl_xor(w, d, 64);
+  }
+  if (NW > 1) {
+    if (lane == 0) {
+      sh.red[0][wave] = s;
+      sh.red[1][wave] = w;
+    }
+    __syncthreads();
+    s = w = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      s += sh.red[0][k];
+      w += sh.red[1][k];
+    }
+  }
+  if (wave != 0) return;
+  if (parts > 1) {
+    if (lane == 0) part_stats[unit] = make_float4(all, s, w, 0.f);
+    if (TOP && lane < top) part_keys[unit * top + lane] = best;
+    return;
+  }
+  const LpRow r = lp_finish(all, s, w);
   if (lane == 0) {
-    red[0][w] = total;
-    red[1][w] = weighted;
-  }
-  __syncthreads();
-  total = weighted = 0.f;
-  for (int k = 0; k < LP_TPB / 64; ++k) {
-    total += red[0][k];
-    weighted += red[1][k];
-  }
-  const LpRow r = lp_finish(m, total, weighted);
-  if (threadIdx.x == 0) {
-    const int64_t t = target[row];
-    float lp = 0.f;
-    if (t != ignore) lp = t >= 0 && t < C ? (ld_el<T>(x, at + t) - r.base) - r.log_total : NAN;
-    logprob[row] = lp;
+    logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
     entropy[row] = r.entropy;
     if (stats) stats[row] = make_float2(r.base, r.log_total);
   }
-  uint64_t last = ~(uint64_t)0;             // (above every key)
-  for (int j = 0; j < top; ++j) {           // the largest key below the last one: keys are distinct
-    uint64_t best = 0;
-    for (int c = threadIdx.x; c < C; c += LP_TPB) {
-      const uint64_t k = lp_key(ld_el<T>(x, at + c), (uint32_t)c);
-      if (k < last && k > best) best = k;
-    }
+  if (TOP && lane < top) {
+    top_logprob[row * top + lane] = (lp_key_value(best) - r.base) - r.log_total;
+    top_index[row * top + lane] = lp_key_class(best);
+  }
+}
+
+// The parts of a row joined: four waves merge the lists of every fourth part each, wave 0 theirs.
+template <int T>
+__global__ __launch_bounds__(LP_TPB) void logprob_join_kernel(const void* __restrict__ x, int64_t ld,
+                                                              const int64_t* __restrict__ target, int C, int64_t ignore, int top,
+                                                              int parts, const float4* __restrict__ part_stats,
+                                                              const uint64_t* __restrict__ part_keys, float* __restrict__ logprob,
+                                                              float* __restrict__ entropy, float2* __restrict__ stats,
+                                                              float* __restrict__ top_logprob, int64_t* __restrict__ top_index) {
+  __shared__ uint64_t lists[4][64];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t best = 0;
+  if (top) {
+    for (int p = wave; p < parts; p += 4)
+      best = lp_merge64(best, lane < top ? part_keys[(row * parts + p) * top + lane] : 0);
+    lists[wave][lane] = best;
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  const int64_t t = target[row];
+  float given = 0.f;
+  if (t >= 0 && t < C) given = ld_el<T>(x, row * ld + t);
+  for (int k = 1; top && k < 4; ++k) best = lp_merge64(best, lists[k][lane]);
+  float all = -INFINITY;
+  for (int p = lane; p < parts; p += 64) all = lp_max(all, part_stats[row * parts + p].x);
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      const uint64_t o = __shfl_xor((unsigned long long)best, d, 64);
-      best = o > best ? o : best;
+  for (int d = 32; d >= 1; d >>= 1) all = lp_max(all, __shfl_xor(all, d, 64));
+  float s = 0.f, w = 0.f;
+  for (int p = lane; p < parts; p += 64) {
+    const float4 q = part_stats[row * parts + p];
+    const float d = lp_diff(q.x, all), f = lp_exp(d);
+    s += f * q.y;
+    w += f * (q.z + d * q.y);
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    s += __shfl_xor(s, d, 64);
+    w += __shfl_xor(w, d, 64);
+  }
+  const LpRow r = lp_finish(all, s, w);
+  if (lane == 0) {
+    logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
+    entropy[row] = r.entropy;
+    if (stats) stats[row] = make_float2(r.base, r.log_total);
+  }
+  if (lane < top) {
+    top_logprob[row * top + lane] = (lp_key_value(best) - r.base) - r.log_total;
+    top_index[row * top + lane] = lp_key_class(best);
+  }
+}
+
+// ---- rows of up to 64 classes: 128 rows go through shared memory (wide loads of one run of memory where the rows are adjacent) and
+// every thread walks its own row there; an odd pitch keeps the walks on different banks.  Alternatives: `top` walks, each of which
+// takes the largest value that is left (strictly larger ones replace: the lowest of equal classes wins).
+constexpr int LP_NARROW = 64;
+constexpr int LP_NARROW_ROWS = 128;
+
+template <int T, bool TOP>
+__global__ __launch_bounds__(LP_NARROW_ROWS) void logprob_narrow_kernel(const void* __restrict__ x, int64_t ld,
+                                                                        const int64_t* __restrict__ target, int64_t rows, int C,
+                                                                        uint32_t magic, int64_t ignore, int top,
+                                                                        float* __restrict__ logprob, float* __restrict__ entropy,
+                                                                        float2* __restrict__ stats,
+                                                                        float* __restrict__ top_logprob,
+                                                                        int64_t* __restrict__ top_index) {
+  extern __shared__ float tile[];
+  constexpr int V = LpVec<T>::N;
+  const int P = C | 1;
+  const int64_t r0 = (int64_t)blockIdx.x * LP_NARROW_ROWS;
+  const int live = (int)min((int64_t)LP_NARROW_ROWS, rows - r0), n = live * C;
+  // (i / C as a product: exact for i < 2^16 and 1 < C <= 64, the error of magic is below 2^-16)
+  auto row_of = [&](int i) { return C == 1 ? i : (int)__umulhi((uint32_t)i, magic); };
+  if (ld == C) {
+    for (int i = threadIdx.x * V; i < n; i += LP_NARROW_ROWS * V) {
+      const lp_u32x4 raw = lp_load_part<T>(x, r0 * C + i, n - i);
+      int r = row_of(i), c = i - r * C;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (i + k < n) tile[r * P + c] = lp_el<T>(raw, k);
+        if (++c == C) {
+          c = 0;
+          ++r;
+        }
+      }
     }
-    if (lane == 0) kred[w] = best;
-    __syncthreads();
-    for (int k = 0; k < LP_TPB / 64; ++k) best = kred[k] > best ? kred[k] : best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      top_logprob[row * top + j] = (lp_key_value(best) - r.base) - r.log_total;
-      top_index[row * top + j] = lp_key_class(best);
+  } else {
+    for (int i = threadIdx.x; i < n; i += LP_NARROW_ROWS) {
+      const int r = row_of(i), c = i - r * C;
+      tile[r * P + c] = ld_el<T>(x, (r0 + r) * ld + c);
     }
-    last = best;
+  }
+  __syncthreads();
+  if (threadIdx.x >= live) return;
+  float* const mine = tile + threadIdx.x * P;
+  const int64_t row = r0 + threadIdx.x, t = target[row];
+  float m = -INFINITY;
+  for (int c = 0; c < C; ++c) m = lp_max(m, mine[c]);
+  float s = 0.f, w = 0.f;
+  const float given = t >= 0 && t < C ? mine[t] : 0.f;
+  for (int c = 0; c < C; ++c) {
+    const float v = mine[c], d = lp_diff(v, m), e = lp_exp(d);
+    s += e;
+    w = __builtin_fmaf(e, d, w);
+    if (TOP) {                                       // as a whole number in the order of the alternatives
+      int o = __float_as_int(v + 0.0f);
+      if (v != v) o = 0x7f800001;
+      mine[c] = __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+    }
+  }
+  const LpRow r = lp_finish(m, s, w);
+  logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
+  entropy[row] = r.entropy;
+  if (stats) stats[row] = make_float2(r.base, r.log_total);
+  if (TOP) {
+    int* const order = reinterpret_cast<int*>(mine);
+    for (int j = 0; j < top; ++j) {
+      int v = INT_MIN, at = 0;                       // (below every value; taken ones become it)
+      for (int c = 0; c < C; ++c) {
+        const int o = order[c];
+        at = o > v ? c : at;
+        v = max(v, o);
+      }
+      order[at] = INT_MIN;
+      const float f = __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
+      top_logprob[row * top + j] = (f - r.base) - r.log_total;
+      top_index[row * top + j] = at;
+    }
   }
 }
 
@@ -144,8 +521,8 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_kernel(const void* __restr
   for (int j = 0; j < top; ++j) all += g_top[row * top + j];
   const float base = stats[row].x, log_total = stats[row].y, h = entropy[row], gh = g_entropy ? g_entropy[row * g_entropy_stride] : 0.f;
   for (int c = threadIdx.x; c < C; c += LP_TPB) {
-    const float lp = (ld_el<T>(x, at + c) - base) - log_total, p = lp_exp(lp);
-    float d = p == 0.f ? 0.f : -p * (all + gh * (lp + h));
+    const float lp = fmaxf((ld_el<T>(x, at + c) - base) - log_total, LP_FAR);
+    float d = log_total != log_total ? NAN : -lp_exp(lp) * (all + gh * (lp + h));
     if (c == t && scored) d += g;
     for (int j = 0; j < top; ++j)
       if (top_index[row * top + j] == c) d += g_top[row * top + j];
@@ -153,11 +530,29 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_kernel(const void* __restr
   }
 }
 
+// How the rows are cut: parts of part_tiles tiles each where there are too few rows to fill the card (a workgroup takes a row, or a
+// part of one).
+struct LpPlan {
+  int nw, parts, part_tiles;
+};
+LpPlan lp_plan(int64_t rows, int64_t C) {
+  LpPlan p = {C <= 64 * LP_HOLD ? 1 : 4, 1, 1};
+  const int64_t tile = (int64_t)p.nw * 64 * LP_HOLD, tiles = (C + tile - 1) / tile;
+  int64_t parts = (1024 + rows - 1) / rows;
+  if (parts > tiles) parts = tiles;
+  if (parts > 64) parts = 64;
+  p.part_tiles = (int)((tiles + parts - 1) / parts);
+  p.parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
+  return p;
+}
+
 }  // namespace
 
 extern "C" size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top) {
-  (void)rows; (void)C; (void)top;
-  return 0;
+  if (rows <= 0 || C <= LP_NARROW || top < 0) return 0;
+  const LpPlan p = lp_plan(rows, C);
+  if (p.parts == 1) return 0;
+  return ccn_align256((size_t)rows * p.parts * sizeof(float4)) + ccn_align256((size_t)rows * p.parts * top * sizeof(uint64_t));
 }
 
 extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C,
@@ -165,19 +560,61 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
                                int64_t* top_index, void* ws, size_t ws_bytes, void* stream) {
   CCN_REQUIRE(logits && target && logprob && entropy, "logprob_fwd: null pointer");
   CCN_REQUIRE(dtype >= 0 && dtype <= 2, "logprob_fwd: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
-  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 31) && (ld >= C || rows == 1),
+  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 30) && (ld >= C || rows == 1),
               "logprob_fwd: rows=%lld C=%lld ld=%lld", (long long)rows, (long long)C, (long long)ld);
   CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_fwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
   CCN_REQUIRE(top == 0 || (top_logprob && top_index), "logprob_fwd: top > 0 without its outputs");
-  (void)ws; (void)ws_bytes;
-  const dim3 grid((unsigned)rows), block(LP_TPB);
+  hipStream_t s = (hipStream_t)stream;
+  if (C <= LP_NARROW) {
+    const dim3 grid((unsigned)((rows + LP_NARROW_ROWS - 1) / LP_NARROW_ROWS)), block(LP_NARROW_ROWS);
+    const size_t lds = (size_t)LP_NARROW_ROWS * (C | 1) * sizeof(float);
+    const uint32_t magic = C == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + C - 1) / C);
+#define CCN_LP_NARROW(T, TOP)                                                                                                     \
+  hipLaunchKernelGGL((logprob_narrow_kernel<T, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, magic, ignore_index,  \
+                     top, logprob, entropy, (float2*)stats, top_logprob, top_index)
+    if (top) {
+      if (dtype == 0) CCN_LP_NARROW(0, true);
+      else if (dtype == 1) CCN_LP_NARROW(1, true);
+      else CCN_LP_NARROW(2, true);
+    } else {
+      if (dtype == 0) CCN_LP_NARROW(0, false);
+      else if (dtype == 1) CCN_LP_NARROW(1, false);
+      else CCN_LP_NARROW(2, false);
+    }
+#undef CCN_LP_NARROW
+    CCN_LAUNCH_OK("logprob_fwd");
+    return CCN_OK;
+  }
+  const LpPlan p = lp_plan(rows, C);
+  const size_t need = ccn_logprob_workspace_bytes(rows, C, top);
+  if (need && (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < need)) {
+    ccn_set_error("logprob_fwd: workspace of %zu bytes, %zu are needed (16-byte aligned)", ws ? ws_bytes : (size_t)0, need);
+    return CCN_ERR_WORKSPACE;
+  }
+  float4* const part_stats = (float4*)ws;
+  uint64_t* const part_keys = need ? (uint64_t*)((char*)ws + ccn_align256((size_t)rows * p.parts * sizeof(float4))) : nullptr;
+  const int64_t blocks = p.nw == 1 ? (rows + 3) / 4 : rows * p.parts;
+  CCN_REQUIRE(blocks < ((int64_t)1 << 31), "logprob_fwd: rows=%lld", (long long)rows);
+#define CCN_LP_WIDE(T, NW, TOP)                                                                                                   \
+  hipLaunchKernelGGL((logprob_wide_kernel<T, NW, TOP>), dim3((unsigned)blocks), dim3(LP_TPB), 0, s, logits, ld, target, rows,      \
+                     (int)C, ignore_index, top, p.parts, p.part_tiles, logprob, entropy, (float2*)stats, top_logprob, top_index,   \
+                     part_stats, part_keys)
 #define CCN_LP_FWD(T)                                                                                                             \
-  hipLaunchKernelGGL(logprob_fwd_kernel<T>, grid, block, 0, (hipStream_t)stream, logits, ld, target, (int)C, ignore_index, top,    \
-                     logprob, entropy, (float2*)stats, top_logprob, top_index)
+  do {                                                                                                                            \
+    if (p.nw == 1 && top) CCN_LP_WIDE(T, 1, true);                                                                                \
+    else if (p.nw == 1) CCN_LP_WIDE(T, 1, false);                                                                                 \
+    else if (top) CCN_LP_WIDE(T, 4, true);                                                                                        \
+    else CCN_LP_WIDE(T, 4, false);                                                                                                \
+    if (p.parts > 1)                                                                                                              \
+      hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)rows), dim3(LP_TPB), 0, s, logits, ld, target, (int)C,             \
+                         ignore_index, top, p.parts, part_stats, part_keys, logprob, entropy, (float2*)stats, top_logprob,        \
+                         top_index);                                                                                              \
+  } while (0)
   if (dtype == 0) CCN_LP_FWD(0);
   else if (dtype == 1) CCN_LP_FWD(1);
   else CCN_LP_FWD(2);
 #undef CCN_LP_FWD
+#undef CCN_LP_WIDE
   CCN_LAUNCH_OK("logprob_fwd");
   return CCN_OK;
 }
@@ -188,7 +625,7 @@ extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const 
                                const float* g_top, void* dlogits, int64_t ldd, void* stream) {
   CCN_REQUIRE(logits && target && stats && entropy && dlogits, "logprob_bwd: null pointer");
   CCN_REQUIRE(dtype >= 0 && dtype <= 2, "logprob_bwd: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
-  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 31) && (ld >= C || rows == 1) &&
+  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 30) && (ld >= C || rows == 1) &&
               (ldd >= C || rows == 1), "logprob_bwd: rows=%lld C=%lld ld=%lld ldd=%lld", (long long)rows, (long long)C,
               (long long)ld, (long long)ldd);
   CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_bwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);

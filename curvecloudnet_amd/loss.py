@@ -63,7 +63,7 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
         raise TypeError("token_logprobs: target is %s; int64 or int32 is wanted" % target.dtype)
     if target.is_cuda and logits.is_cuda and target.device != logits.device:
         raise ValueError("token_logprobs: logits on %s, target on %s" % (logits.device, target.device))
-    if logits.dim() == 0 or logits.size(-1) == 0 or logits.size(-1) >= 1 << 31:
+    if logits.dim() == 0 or logits.size(-1) == 0 or logits.size(-1) >= 1 << 30:
         raise ValueError("token_logprobs: logits of shape %s have no classes, or too many" % (tuple(logits.shape),))
     shape, c = logits.shape[:-1], logits.size(-1)
     if target.shape != shape:

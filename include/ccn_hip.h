@@ -704,6 +704,7 @@ int ccn_adam_step(float* param, const float* grad, float* exp_avg, float* exp_av
 
 /* Log-probabilities of given classes, the entropy of every row, its best alternatives, and their gradient.
  * logits: rows x C of `dtype` (0 = fp32, 1 = bf16, 2 = fp16), row stride ld elements (any alignment of the type).  Outputs fp32.
+ * C < 2^30, rows < 2^31.
  * fwd: logprob (rows) of target (0 where target == ignore_index, NaN for another target outside [0, C)), entropy (rows), stats
  * (2 x rows, nullable: what bwd needs), top_logprob / top_index (rows x top, the `top` largest logits, equal ones by ascending
  * class; top <= 64, top <= C).  A row of -inf only: logprob -inf, entropy 0.

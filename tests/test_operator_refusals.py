@@ -95,7 +95,7 @@ def test_c_entries_of_the_scores_refuse():
     for call, word in ((lambda: fwd(x=null), "null"), (lambda: fwd(t=null), "null"), (lambda: fwd(lp=null), "null"),
                        (lambda: fwd(h=null), "null"), (lambda: fwd(dtype=3), "dtype"), (lambda: fwd(dtype=-1), "dtype"),
                        (lambda: fwd(rows=0), "rows"), (lambda: fwd(rows=1 << 31), "rows"), (lambda: fwd(c=0), "rows"),
-                       (lambda: fwd(c=1 << 31, ld=1 << 31), "rows"), (lambda: fwd(ld=7), "ld"), (lambda: fwd(ld=-8), "ld"),
+                       (lambda: fwd(c=1 << 30, ld=1 << 30), "rows"), (lambda: fwd(ld=7), "ld"), (lambda: fwd(ld=-8), "ld"),
                        (lambda: fwd(top=-1), "top"), (lambda: fwd(top=9), "top"), (lambda: fwd(top=65, c=100, ld=100), "top"),
                        (lambda: fwd(top=2, best=null), "top"), (lambda: fwd(top=2, index=null), "top"),
                        (lambda: bwd(x=null), "null"), (lambda: bwd(stats=null), "null"), (lambda: bwd(d=null), "null"),
@@ -103,7 +103,7 @@ def test_c_entries_of_the_scores_refuse():
                        (lambda: bwd(top=2, gt=null), "top"), (lambda: bwd(top=2, index=null), "top"), (lambda: bwd(top=9), "top"),
                        (lambda: bwd(s1=-1), "stride"), (lambda: bwd(s2=-1), "stride")):
         assert call() < 0 and word in err(), (word, err())
-    sizes = [(r, c, k) for r in (1, 96, 1 << 20) for c in (1, 64, 65, 50021, 262144, (1 << 31) - 1) for k in (0, 64)]
+    sizes = [(r, c, k) for r in (1, 96, 1 << 20) for c in (1, 64, 65, 50021, 262144, (1 << 30) - 1) for k in (0, 64)]
     assert all(0 <= lib.ccn_logprob_workspace_bytes(*s) < 1 << 42 for s in sizes)
     assert lib.ccn_logprob_workspace_bytes(-1, 5, 0) == lib.ccn_logprob_workspace_bytes(5, -1, 0) == 0
     # where a workspace is needed, one that is missing or too small is refused
