@@ -504,29 +504,152 @@ __global__ __launch_bounds__(LP_NARROW_ROWS) void logprob_narrow_kernel(const vo
   }
 }
 
-template <int T>
-__global__ __launch_bounds__(LP_TPB) void logprob_bwd_kernel(const void* __restrict__ x, int64_t ld,
-                                                             const int64_t* __restrict__ target, int C, int64_t ignore, int top,
-                                                             const int64_t* __restrict__ top_index, const float2* __restrict__ stats,
-                                                             const float* __restrict__ entropy, const float* __restrict__ g_logprob,
-                                                             int64_t g_logprob_stride, const float* __restrict__ g_entropy,
-                                                             int64_t g_entropy_stride, const float* __restrict__ g_top,
-                                                             void* __restrict__ dx, int64_t ldd) {
-  const int64_t row = blockIdx.x, at = row * ld, to = row * ldd;
+// ---- the gradient: dx = -p (G + g_entropy (l + entropy)) + one-hot terms, 16 bytes of a row at a time.  What belongs to the row alone:
+struct LpGrad {
+  float base, log_total, flat, slope;       // dx = p (flat + slope l)
+  int t;                                    // the given class, -1 where it is not scored
+  float g;
+};
+__device__ __forceinline__ LpGrad lp_grad(int64_t row, const int64_t* __restrict__ target, int C, int64_t ignore, int top,
+                                          const float2* __restrict__ stats, const float* __restrict__ entropy,
+                                          const float* __restrict__ g_logprob, int64_t g_logprob_stride,
+                                          const float* __restrict__ g_entropy, int64_t g_entropy_stride,
+                                          const float* __restrict__ g_top) {
+  LpGrad q;
   const int64_t t = target[row];
-  const bool scored = t != ignore, inside = t >= 0 && t < C;
-  float g = 0.f;
-  if (scored && g_logprob) g = inside ? g_logprob[row * g_logprob_stride] : NAN;
-  float all = g;
+  const float2 st = stats[row];
+  const float gh = g_entropy ? g_entropy[row * g_entropy_stride] : 0.f;
+  q.t = -1;
+  q.g = 0.f;
+  if (t != ignore && g_logprob) {
+    if (t >= 0 && t < C) q.t = (int)t;
+    q.g = q.t >= 0 ? g_logprob[row * g_logprob_stride] : NAN;
+  }
+  float all = q.g;
   for (int j = 0; j < top; ++j) all += g_top[row * top + j];
-  const float base = stats[row].x, log_total = stats[row].y, h = entropy[row], gh = g_entropy ? g_entropy[row * g_entropy_stride] : 0.f;
-  for (int c = threadIdx.x; c < C; c += LP_TPB) {
-    const float lp = fmaxf((ld_el<T>(x, at + c) - base) - log_total, LP_FAR);
-    float d = log_total != log_total ? NAN : -lp_exp(lp) * (all + gh * (lp + h));
-    if (c == t && scored) d += g;
-    for (int j = 0; j < top; ++j)
-      if (top_index[row * top + j] == c) d += g_top[row * top + j];
-    st_el<T>(dx, to + c, d);
+  q.base = st.x;
+  q.log_total = st.y;
+  q.slope = -gh;
+  // (a row with a NaN or an infinity in it: NaN, though every p below is taken as 0)
+  q.flat = st.y != st.y ? NAN : -(all + gh * entropy[row]);
+  return q;
+}
+__device__ __forceinline__ float lp_smooth(const LpGrad& q, float v) {
+  const float l = fmaxf((v - q.base) - q.log_total, LP_FAR);
+  return lp_exp(l) * __builtin_fmaf(q.slope, l, q.flat);
+}
+template <int T>
+__device__ __forceinline__ void lp_put(lp_u32x4& r, int i, float v) {
+  if (T == 0) {
+    r[i] = __float_as_uint(v);
+  } else {
+    uint32_t b;
+    if (T == 1) b = __builtin_bit_cast(uint16_t, (__bf16)v);
+    else b = __builtin_bit_cast(uint16_t, (_Float16)v);
+    r[i >> 1] = (i & 1) ? (r[i >> 1] | (b << 16)) : b;
+  }
+}
+template <int T>
+__device__ __forceinline__ void lp_store_part(void* __restrict__ x, int64_t at, int n, const lp_u32x4& r) {
+  constexpr int V = LpVec<T>::N, B = T == 0 ? 4 : 2;
+  if (n >= V) {
+    *reinterpret_cast<typename LpVec<T>::mem*>(reinterpret_cast<char*>(x) + at * B) = r;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) {
+      if (T == 0) reinterpret_cast<uint32_t*>(x)[at + i] = r[i];
+      else reinterpret_cast<uint16_t*>(x)[at + i] = (uint16_t)(r[i >> 1] >> (16 * (i & 1)));
+    }
+}
+// 16 bytes of the gradient from 16 bytes of the row, c the class of the first.
+template <int T>
+__device__ __forceinline__ lp_u32x4 lp_grad16(const LpGrad& q, const lp_u32x4& raw, int c) {
+  constexpr int V = LpVec<T>::N;
+  lp_u32x4 out;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float d = lp_smooth(q, lp_el<T>(raw, i));
+    if (c + i == q.t) d += q.g;
+    lp_put<T>(out, i, d);
+  }
+  return out;
+}
+// The value of an alternative: written again, with every one-hot term it takes part in (the same class twice gives the same value twice).
+template <int T>
+__device__ __forceinline__ void lp_grad_top(const LpGrad& q, const void* __restrict__ x, int64_t at, void* __restrict__ dx,
+                                            int64_t to, int64_t c, int top, const int64_t* __restrict__ top_index,
+                                            const float* __restrict__ g_top) {
+  float d = lp_smooth(q, ld_el<T>(x, at + c));
+  if (c == q.t) d += q.g;
+  for (int j = 0; j < top; ++j)
+    if (top_index[j] == c) d += g_top[j];
+  st_el<T>(dx, to + c, d);
+}
+
+// A workgroup takes `group` rows of up to LP_GROUP_MAX classes, whose own values it computes once into shared memory; `vecs`: 16-byte
+// pieces of a row.
+constexpr int LP_GROUP = 4096;              // logits of a group of rows, about
+constexpr int LP_GROUP_MAX = 4096;
+
+template <int T>
+__global__ __launch_bounds__(LP_TPB) void logprob_bwd_rows_kernel(
+    const void* __restrict__ x, int64_t ld, const int64_t* __restrict__ target, int64_t rows, int C, int64_t ignore, int top, int group,
+    int vecs, uint32_t magic, const int64_t* __restrict__ top_index, const float2* __restrict__ stats,
+    const float* __restrict__ entropy, const float* __restrict__ g_logprob, int64_t g_logprob_stride,
+    const float* __restrict__ g_entropy, int64_t g_entropy_stride, const float* __restrict__ g_top, void* __restrict__ dx, int64_t ldd) {
+  constexpr int V = LpVec<T>::N;
+  __shared__ LpGrad mine[LP_TPB];
+  const int64_t r0 = (int64_t)blockIdx.x * group;
+  const int live = (int)min((int64_t)group, rows - r0), n = live * vecs;
+  if ((int)threadIdx.x < live)
+    mine[threadIdx.x] = lp_grad(r0 + threadIdx.x, target, C, ignore, top, stats, entropy, g_logprob, g_logprob_stride, g_entropy,
+                                g_entropy_stride, g_top);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += LP_TPB) {
+    const int r = vecs == 1 ? i : (int)__umulhi((uint32_t)i, magic), c = (i - r * vecs) * V;
+    const lp_u32x4 raw = lp_load_part<T>(x, (r0 + r) * ld + c, C - c);
+    lp_store_part<T>(dx, (r0 + r) * ldd + c, C - c, lp_grad16<T>(mine[r], raw, c));
+  }
+  if (top == 0) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < live * top; i += LP_TPB) {
+    const int r = i / top;
+    const int64_t row = r0 + r, c = top_index[r0 * top + i];
+    if (c >= 0 && c < C) lp_grad_top<T>(mine[r], x, row * ld, dx, row * ldd, c, top, top_index + row * top, g_top + row * top);
+  }
+}
+
+// Longer rows: a workgroup takes LP_TPB * LP_HOLD logits of one, all loads in flight before the first is used.
+template <int T>
+__global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
+    const void* __restrict__ x, int64_t ld, const int64_t* __restrict__ target, int C, int64_t ignore, int top, int tiles,
+    const int64_t* __restrict__ top_index, const float2* __restrict__ stats, const float* __restrict__ entropy,
+    const float* __restrict__ g_logprob, int64_t g_logprob_stride, const float* __restrict__ g_entropy, int64_t g_entropy_stride,
+    const float* __restrict__ g_top, void* __restrict__ dx, int64_t ldd) {
+  constexpr int V = LpVec<T>::N, NJ = LP_HOLD / V, TILE = LP_TPB * LP_HOLD;
+  const int64_t row = blockIdx.x / (unsigned)tiles, at = row * ld, to = row * ldd;
+  const int c0 = (int)(blockIdx.x % (unsigned)tiles) * TILE, n = min(C - c0, TILE), tid = threadIdx.x;
+  lp_u32x4 raw[NJ];
+  if (n == TILE) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) raw[j] = lp_load<T>(x, at + c0 + (j * LP_TPB + tid) * V);
+  } else {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, at + c0 + (j * LP_TPB + tid) * V, n - (j * LP_TPB + tid) * V);
+  }
+  const LpGrad q = lp_grad(row, target, C, ignore, top, stats, entropy, g_logprob, g_logprob_stride, g_entropy, g_entropy_stride, g_top);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int c = (j * LP_TPB + tid) * V;
+    if (j * LP_TPB * V < n) lp_store_part<T>(dx, to + c0 + c, n - c, lp_grad16<T>(q, raw[j], c0 + c));
+  }
+  if (top == 0) return;
+  __syncthreads();
+  if (tid < top) {
+    const int64_t c = top_index[row * top + tid];
+    if (c >= c0 && c < c0 + n) lp_grad_top<T>(q, x, at, dx, to, c, top, top_index + row * top, g_top + row * top);
   }
 }
 
@@ -631,14 +754,34 @@ extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const 
   CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_bwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
   CCN_REQUIRE(top == 0 || (g_top && top_index), "logprob_bwd: top > 0 without its gradient and classes");
   CCN_REQUIRE(g_logprob_stride >= 0 && g_entropy_stride >= 0, "logprob_bwd: negative gradient stride");
-  const dim3 grid((unsigned)rows), block(LP_TPB);
+  hipStream_t s = (hipStream_t)stream;
+  if (C <= LP_GROUP_MAX) {
+    const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
+    const int group = (int)(LP_GROUP / C < 1 ? 1 : LP_GROUP / C > LP_TPB ? LP_TPB : LP_GROUP / C);
+    const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
+    const dim3 grid((unsigned)((rows + group - 1) / group)), block(LP_TPB);
 #define CCN_LP_BWD(T)                                                                                                             \
-  hipLaunchKernelGGL(logprob_bwd_kernel<T>, grid, block, 0, (hipStream_t)stream, logits, ld, target, (int)C, ignore_index, top,    \
-                     top_index, (const float2*)stats, entropy, g_logprob, g_logprob_stride, g_entropy, g_entropy_stride, g_top, dlogits, ldd)
-  if (dtype == 0) CCN_LP_BWD(0);
-  else if (dtype == 1) CCN_LP_BWD(1);
-  else CCN_LP_BWD(2);
+  hipLaunchKernelGGL(logprob_bwd_rows_kernel<T>, grid, block, 0, s, logits, ld, target, rows, (int)C, ignore_index, top, group,    \
+                     vecs, magic, top_index, (const float2*)stats, entropy, g_logprob, g_logprob_stride, g_entropy,               \
+                     g_entropy_stride, g_top, dlogits, ldd)
+    if (dtype == 0) CCN_LP_BWD(0);
+    else if (dtype == 1) CCN_LP_BWD(1);
+    else CCN_LP_BWD(2);
 #undef CCN_LP_BWD
+  } else {
+    const int64_t tiles = (C + LP_TPB * LP_HOLD - 1) / (LP_TPB * LP_HOLD);
+    CCN_REQUIRE(rows * tiles < ((int64_t)1 << 31), "logprob_bwd: rows=%lld C=%lld: too many for one launch", (long long)rows,
+                (long long)C);
+    const dim3 grid((unsigned)(rows * tiles)), block(LP_TPB);
+#define CCN_LP_BWD(T)                                                                                                             \
+  hipLaunchKernelGGL(logprob_bwd_wide_kernel<T>, grid, block, 0, s, logits, ld, target, (int)C, ignore_index, top, (int)tiles,     \
+                     top_index, (const float2*)stats, entropy, g_logprob, g_logprob_stride, g_entropy, g_entropy_stride, g_top,   \
+                     dlogits, ldd)
+    if (dtype == 0) CCN_LP_BWD(0);
+    else if (dtype == 1) CCN_LP_BWD(1);
+    else CCN_LP_BWD(2);
+#undef CCN_LP_BWD
+  }
   CCN_LAUNCH_OK("logprob_bwd");
   return CCN_OK;
 }
