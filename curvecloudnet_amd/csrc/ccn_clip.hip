@@ -15,24 +15,51 @@
 namespace {
 
 constexpr int CLIP_TPB = 256;
-constexpr int CLIP_MAX = 160;                      // tensors of one launch: 20 bytes of arguments each
+constexpr int CLIP_MAX = 320;                      // tensors of one launch: 12 bytes of arguments each
 constexpr int CLIP_PART_MAX = 1024;                // workgroups of one launch of the norm, each with a partial result
-constexpr int64_t CLIP_CHUNK = 16384;              // values that a workgroup takes at a time
+constexpr int CLIP_CHUNK = 16384;                  // values that a workgroup takes at a time
 
+// Tensor i is chunks first[i] ... first[i + 1] - 1.  at[i]: its address (bits 0-47), the length of its last chunk less one (48-61),
+// its type (62-63).
 struct ClipTable {
-  void* ptr[CLIP_MAX];
-  int64_t size[CLIP_MAX];
-  uint8_t dtype[CLIP_MAX];
-  int first[CLIP_MAX + 1];                         // chunks in front of tensor i
+  uint64_t at[CLIP_MAX];
+  int first[CLIP_MAX + 1];
   int n;
 };
-static_assert(sizeof(ClipTable) < 3584, "kernel arguments");
+static_assert(sizeof(ClipTable) + 64 < 4096, "kernel arguments");
+static_assert(CLIP_CHUNK <= 1 << 14 && CLIP_MAX % 64 == 0, "fields of ClipTable");
 
 enum { NORM_SUM = 1, NORM_TWO = 2, NORM_MAX = 3 };
 
+// The entry of `first` (ascending, n of them in use) whose run holds chunk c: all lanes look at once, the entries sit in memory that
+// is slow to reach for the first time.
+template <int N>
+__device__ __forceinline__ int clip_find(const int (&first)[N], int n, int c) {
+  const int lane = threadIdx.x & 63;
+  int found = 0;
+#pragma unroll
+  for (int k = 0; k < N / 64; ++k) {
+    const int i = k * 64 + lane;
+    found += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < n && first[i] <= c));
+  }
+  return __builtin_amdgcn_readfirstlane(found - 1);
+}
+
+// ---- a thread's share of the norm: sums in 64 bits; the maximum as the largest pattern of bits without the sign (a NaN's is above
+// every number's, so it stays)
+template <int KIND> struct ClipAcc { double v = 0.0; };
+template <> struct ClipAcc<NORM_MAX> { uint32_t v = 0; };
+
+template <int KIND, int T>
+__device__ __forceinline__ void clip_add(ClipAcc<KIND>& a, float x) {
+  if constexpr (KIND == NORM_MAX) a.v = max(a.v, __float_as_uint(x) & 0x7fffffffu);
+  else if constexpr (KIND == NORM_TWO) a.v = __builtin_fma((double)x, (double)x, a.v);
+  else a.v += (double)fabsf(x);
+}
 template <int KIND>
-__device__ __forceinline__ double clip_term(float v) {
-  return KIND == NORM_TWO ? (double)v * (double)v : fabs((double)v);
+__device__ __forceinline__ double clip_value(const ClipAcc<KIND>& a) {
+  if constexpr (KIND == NORM_MAX) return (double)__uint_as_float(a.v);
+  else return a.v;
 }
 // (a NaN stays: fmax would drop it)
 template <int KIND>
@@ -40,12 +67,11 @@ __device__ __forceinline__ double clip_join(double a, double b) {
   if (KIND != NORM_MAX) return a + b;
   return a != a ? a : (b > a || b != b ? b : a);
 }
-__device__ __forceinline__ double clip_shfl_xor(double v, int d) { return __shfl_xor(v, d, 64); }
 
 template <int KIND>
 __device__ __forceinline__ double clip_block(double v, double* red) {
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = clip_join<KIND>(v, clip_shfl_xor(v, d));
+  for (int d = 32; d >= 1; d >>= 1) v = clip_join<KIND>(v, __shfl_xor(v, d, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = red[0];
@@ -54,36 +80,53 @@ __device__ __forceinline__ double clip_block(double v, double* red) {
   return v;
 }
 
-// The tensor that chunk c belongs to.
-__device__ __forceinline__ int clip_find(const ClipTable& t, int c) {
-  int lo = 0, hi = t.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.first[mid] <= c) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
+// n <= CLIP_CHUNK values at p: eight 16-byte loads of a thread in flight
 template <int KIND, int T>
-__device__ __forceinline__ double clip_sum(const void* p, int64_t beg, int64_t end) {
-  double v = 0.0;
-  for (int64_t i = beg + threadIdx.x; i < end; i += CLIP_TPB) v = clip_join<KIND>(v, clip_term<KIND>(ld_el<T>(p, i)));
-  return v;
+__device__ __forceinline__ void clip_sum(ClipAcc<KIND>& a, const char* p, int n) {
+  constexpr int V = CcnVec16<T>::N, STEP = CLIP_TPB * V, U = 8;
+  int i = threadIdx.x * V;
+  for (; i - (int)threadIdx.x * V + U * STEP <= n; i += U * STEP) {
+    ccn_u32x4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = ld16<T>(p, i + u * STEP);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < V; ++k) clip_add<KIND, T>(a, get16<T>(r[u], k));
+  }
+  ccn_u32x4 r[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    r[u] = ccn_u32x4{0, 0, 0, 0};
+    if (i + u * STEP + V <= n) r[u] = ld16<T>(p, i + u * STEP);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (i + u * STEP + V <= n)
+#pragma unroll
+      for (int k = 0; k < V; ++k) clip_add<KIND, T>(a, get16<T>(r[u], k));
+  const int whole = n / V * V;
+  if ((int)threadIdx.x < n - whole) clip_add<KIND, T>(a, ld_el<T>(p, whole + threadIdx.x));
 }
 
 template <int KIND>
 __global__ __launch_bounds__(CLIP_TPB) void grad_norm_kernel(const ClipTable t, double* __restrict__ partial) {
   __shared__ double red[CLIP_TPB / 64];
-  double v = 0.0;
-  for (int c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
-    const int i = clip_find(t, c);
-    const int64_t beg = (int64_t)(c - t.first[i]) * CLIP_CHUNK, end = min(beg + CLIP_CHUNK, t.size[i]);
-    const double u = t.dtype[i] == 0 ? clip_sum<KIND, 0>(t.ptr[i], beg, end)
-                     : t.dtype[i] == 1 ? clip_sum<KIND, 1>(t.ptr[i], beg, end) : clip_sum<KIND, 2>(t.ptr[i], beg, end);
-    v = clip_join<KIND>(v, u);
+  const int chunks = t.first[t.n];
+  // (a workgroup's chunks lie next to one another)
+  const int beg = (int)((int64_t)blockIdx.x * chunks / gridDim.x), end = (int)(((int64_t)blockIdx.x + 1) * chunks / gridDim.x);
+  ClipAcc<KIND> a;
+  int i = clip_find(t.first, t.n, beg);
+  for (int c = beg; c < end; ++c) {
+    if (c == t.first[i + 1]) ++i;
+    const uint64_t at = t.at[i];
+    const int n = c + 1 == t.first[i + 1] ? (int)((at >> 48) & 0x3fff) + 1 : CLIP_CHUNK, type = (int)(at >> 62);
+    const char* const p = reinterpret_cast<const char*>(at & 0xffffffffffffull) + (int64_t)(c - t.first[i]) * CLIP_CHUNK * (type ? 2 : 4);
+    if (type == 0) clip_sum<KIND, 0>(a, p, n);
+    else if (type == 1) clip_sum<KIND, 1>(a, p, n);
+    else clip_sum<KIND, 2>(a, p, n);
   }
-  v = clip_block<KIND>(v, red);
+  const double v = clip_block<KIND>(clip_value<KIND>(a), red);
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
@@ -109,24 +152,47 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double*
 }
 
 template <int T>
-__device__ __forceinline__ void clip_apply(void* p, int64_t beg, int64_t end, float scale) {
-  for (int64_t i = beg + threadIdx.x; i < end; i += CLIP_TPB) st_el<T>(p, i, ld_el<T>(p, i) * scale);
+__device__ __forceinline__ void clip_apply(char* p, int n, float scale) {
+  constexpr int V = CcnVec16<T>::N, STEP = CLIP_TPB * V, U = 4;
+  for (int i = threadIdx.x * V; i - (int)threadIdx.x * V < n; i += U * STEP) {
+    ccn_u32x4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = ccn_u32x4{0, 0, 0, 0};
+      if (i + u * STEP + V <= n) r[u] = ld16<T>(p, i + u * STEP);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ccn_u32x4 o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) put16<T>(o, k, get16<T>(r[u], k) * scale);
+      if (i + u * STEP + V <= n) st16<T>(p, i + u * STEP, o);
+    }
+  }
+  const int whole = n / V * V;
+  if ((int)threadIdx.x < n - whole) st_el<T>(p, whole + threadIdx.x, ld_el<T>(p, whole + threadIdx.x) * scale);
 }
 
 template <int KIND>
-__global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, const double* __restrict__ partial, int n,
+__global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, const double* __restrict__ partial, int count,
                                                              double max_norm, float* __restrict__ norm) {
   __shared__ double red[CLIP_TPB / 64];
-  const double v = clip_total<KIND>(partial, n, red);
+  const double v = clip_total<KIND>(partial, count, red);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
   const float scale = clip_scale(v, max_norm);
   if (scale == 1.f) return;
-  for (int c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
-    const int i = clip_find(t, c);
-    const int64_t beg = (int64_t)(c - t.first[i]) * CLIP_CHUNK, end = min(beg + CLIP_CHUNK, t.size[i]);
-    if (t.dtype[i] == 0) clip_apply<0>(t.ptr[i], beg, end, scale);
-    else if (t.dtype[i] == 1) clip_apply<1>(t.ptr[i], beg, end, scale);
-    else clip_apply<2>(t.ptr[i], beg, end, scale);
+  const int chunks = t.first[t.n];
+  const int beg = (int)((int64_t)blockIdx.x * chunks / gridDim.x), end = (int)(((int64_t)blockIdx.x + 1) * chunks / gridDim.x);
+  // (from the last to the first: what the norm read last is the likeliest to sit in a cache still)
+  int i = clip_find(t.first, t.n, end - 1);
+  for (int c = end - 1; c >= beg; --c) {
+    if (c < t.first[i]) --i;
+    const uint64_t at = t.at[i];
+    const int n = c + 1 == t.first[i + 1] ? (int)((at >> 48) & 0x3fff) + 1 : CLIP_CHUNK, type = (int)(at >> 62);
+    char* const p = reinterpret_cast<char*>(at & 0xffffffffffffull) + (int64_t)(c - t.first[i]) * CLIP_CHUNK * (type ? 2 : 4);
+    if (type == 0) clip_apply<0>(p, n, scale);
+    else if (type == 1) clip_apply<1>(p, n, scale);
+    else clip_apply<2>(p, n, scale);
   }
 }
 
@@ -142,27 +208,54 @@ struct AdamTable {
   int first[ADAM_MAX + 1];
   int n;
 };
-static_assert(sizeof(AdamTable) < 3584, "kernel arguments");
+static_assert(sizeof(AdamTable) + 96 < 4096, "kernel arguments");
 
-__global__ __launch_bounds__(CLIP_TPB) void adam_clip_kernel(const AdamTable t, const double* __restrict__ partial, int n,
-                                                             double max_norm, float* __restrict__ norm, float beta1_rest,
-                                                             float beta2, float beta2_rest, float step_size, float inv_bc2_sqrt,
-                                                             float eps, float weight_decay) {
+struct AdamCoef {
+  float scale, beta1_rest, beta2, beta2_rest, step_size, inv_bc2_sqrt, eps, decay;
+};
+__device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, const AdamCoef& k) {
+  const float grad = g * k.scale + k.decay * p;
+  m = m + (grad - m) * k.beta1_rest;
+  v = v * k.beta2 + k.beta2_rest * grad * grad;
+  p = p - k.step_size * (m / (sqrtf(v) * k.inv_bc2_sqrt + k.eps));
+}
+
+__global__ __launch_bounds__(CLIP_TPB) void adam_clip_kernel(const AdamTable t, const double* __restrict__ partial, int count,
+                                                             double max_norm, float* __restrict__ norm, AdamCoef k) {
   __shared__ double red[CLIP_TPB / 64];
-  const double total = clip_total<NORM_TWO>(partial, n, red);
+  const double total = clip_total<NORM_TWO>(partial, count, red);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
-  const float scale = clip_scale(total, max_norm);
-  for (int c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
-    int i = 0;
-    while (t.first[i + 1] <= c) ++i;
-    const int64_t beg = (int64_t)(c - t.first[i]) * CLIP_CHUNK, end = min(beg + CLIP_CHUNK, t.size[i]);
-    for (int64_t k = beg + threadIdx.x; k < end; k += CLIP_TPB) {
-      const float pk = t.p[i][k], grad = t.g[i][k] * scale + weight_decay * pk;
-      const float mk = t.m[i][k] + (grad - t.m[i][k]) * beta1_rest;
-      const float vk = t.v[i][k] * beta2 + beta2_rest * grad * grad;
-      t.m[i][k] = mk;
-      t.v[i][k] = vk;
-      t.p[i][k] = pk - step_size * (mk / (sqrtf(vk) * inv_bc2_sqrt + eps));
+  k.scale = clip_scale(total, max_norm);
+  const int chunks = t.first[t.n];
+  const int beg = (int)((int64_t)blockIdx.x * chunks / gridDim.x), end = (int)(((int64_t)blockIdx.x + 1) * chunks / gridDim.x);
+  int i = __builtin_amdgcn_readfirstlane(__builtin_popcountll(
+              __builtin_amdgcn_ballot_w64((int)(threadIdx.x & 63) < t.n && t.first[threadIdx.x & 63] <= end - 1))) - 1;
+  for (int c = end - 1; c >= beg; --c) {             // (from the last to the first, as in grad_clip_kernel)
+    if (c < t.first[i]) --i;
+    const int64_t from = (int64_t)(c - t.first[i]) * CLIP_CHUNK;
+    const int n = (int)min((int64_t)CLIP_CHUNK, t.size[i] - from);
+    float* const p = t.p[i] + from;
+    const float* const g = t.g[i] + from;
+    float* const m = t.m[i] + from;
+    float* const v = t.v[i] + from;
+    for (int e = threadIdx.x * 4; e + 4 <= n; e += CLIP_TPB * 4) {
+      float4 pp = *(const float4*)(p + e), mm = *(const float4*)(m + e), vv = *(const float4*)(v + e);
+      const float4 gg = *(const float4*)(g + e);
+      adam_one(pp.x, gg.x, mm.x, vv.x, k);
+      adam_one(pp.y, gg.y, mm.y, vv.y, k);
+      adam_one(pp.z, gg.z, mm.z, vv.z, k);
+      adam_one(pp.w, gg.w, mm.w, vv.w, k);
+      *(float4*)(p + e) = pp;
+      *(float4*)(m + e) = mm;
+      *(float4*)(v + e) = vv;
+    }
+    const int e = n / 4 * 4 + threadIdx.x;
+    if (e < n) {
+      float pp = p[e], mm = m[e], vv = v[e];
+      adam_one(pp, g[e], mm, vv, k);
+      p[e] = pp;
+      m[e] = mm;
+      v[e] = vv;
     }
   }
 }
@@ -174,8 +267,8 @@ int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype
     CCN_REQUIRE(!dtype || (dtype[i] >= 0 && dtype[i] <= 2), "%s: tensor %lld: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", who,
                 (long long)i, dtype ? dtype[i] : 0);
     CCN_REQUIRE(size[i] >= 0 && size[i] < ((int64_t)1 << 36), "%s: tensor %lld has %lld values", who, (long long)i, (long long)size[i]);
-    CCN_REQUIRE(size[i] == 0 || (ptr[i] && (uintptr_t)ptr[i] % el == 0), "%s: tensor %lld: null or not aligned to its type", who,
-                (long long)i);
+    CCN_REQUIRE(size[i] == 0 || (ptr[i] && (uintptr_t)ptr[i] % el == 0 && (uintptr_t)ptr[i] < (uintptr_t)1 << 48),
+                "%s: tensor %lld: null or not aligned to its type", who, (long long)i);
   }
   if (!writes) return CCN_OK;
   bool ordered = true;                               // tensors of one buffer come in order, or in reverse: looked at before sorting
@@ -208,9 +301,7 @@ int clip_tables(const void* const* ptr, const int64_t* size, const int32_t* dtyp
   t.first[0] = 0;
   for (int64_t i = 0; i < n; ++i) {
     if (size[i] == 0) continue;
-    t.ptr[t.n] = const_cast<void*>(ptr[i]);
-    t.size[t.n] = size[i];
-    t.dtype[t.n] = (uint8_t)(dtype ? dtype[i] : 0);
+    t.at[t.n] = (uint64_t)(uintptr_t)ptr[i] | ((uint64_t)((size[i] - 1) % CLIP_CHUNK) << 48) | ((uint64_t)(dtype ? dtype[i] : 0) << 62);
     t.first[t.n + 1] = t.first[t.n] + clip_chunks(size[i]);
     if (++t.n == CLIP_MAX) {
       if (int rc = f(t)) return rc;
@@ -284,7 +375,7 @@ extern "C" int ccn_grad_clip(void* const* grads, const int64_t* sizes, const int
   }
   float* out = norm;
   const int rc = clip_tables(grads, sizes, dtypes, n, [&](const ClipTable& t) {
-    const int chunks = t.first[t.n], grid = chunks < 4 * CLIP_PART_MAX ? chunks : 4 * CLIP_PART_MAX;
+    const int chunks = t.first[t.n], grid = chunks < CLIP_PART_MAX ? chunks : CLIP_PART_MAX;
     if (kind == NORM_TWO)
       hipLaunchKernelGGL(grad_clip_kernel<NORM_TWO>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
     else if (kind == NORM_SUM)
@@ -337,7 +428,8 @@ extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, fl
   }
   // bias corrections and 1 - beta in double on the host (1 - 0.999 from a beta in 32 bits is off by 1.3e-5 of itself)
   const double bc1 = 1.0 - pow(beta1, (double)step), bc2 = 1.0 - pow(beta2, (double)step);
-  const float step_size = (float)(lr / bc1), inv_bc2_sqrt = (float)(1.0 / sqrt(bc2));
+  const AdamCoef coef = {1.f, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)(lr / bc1), (float)(1.0 / sqrt(bc2)),
+                         (float)eps, (float)weight_decay};
   float* out = norm;
   AdamTable t;
   t.n = 0;
@@ -353,10 +445,8 @@ extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, fl
       ++t.n;
     }
     if (t.n == ADAM_MAX || (i == n - 1 && t.n > 0)) {
-      const int chunks = t.first[t.n], grid = chunks < 4 * CLIP_PART_MAX ? chunks : 4 * CLIP_PART_MAX;
-      hipLaunchKernelGGL(adam_clip_kernel, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out,
-                         (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), step_size, inv_bc2_sqrt, (float)eps,
-                         (float)weight_decay);
+      const int chunks = t.first[t.n], grid = chunks < 2 * CLIP_PART_MAX ? chunks : 2 * CLIP_PART_MAX;
+      hipLaunchKernelGGL(adam_clip_kernel, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out, coef);
       out = nullptr;
       t.n = 0;
     }

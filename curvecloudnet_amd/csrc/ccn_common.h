@@ -130,3 +130,40 @@ __device__ __forceinline__ void st_el(void* __restrict__ p, int64_t i, float v) 
     reinterpret_cast<uint16_t*>(p)[i] = __builtin_bit_cast(uint16_t, x);
   }
 }
+
+// ---- 16 bytes of fp32 / bf16 / fp16 values (T as above) at any alignment of the type
+typedef uint32_t ccn_u32x4 __attribute__((ext_vector_type(4)));
+template <int T> struct CcnVec16 {
+  static constexpr int N = 8;
+  typedef ccn_u32x4 mem __attribute__((aligned(2)));
+};
+template <> struct CcnVec16<0> {
+  static constexpr int N = 4;
+  typedef ccn_u32x4 mem __attribute__((aligned(4)));
+};
+template <int T>
+__device__ __forceinline__ float get16(const ccn_u32x4& r, int i) {
+  if (T == 0) return __builtin_bit_cast(float, (uint32_t)r[i]);
+  if (T == 1) return __builtin_bit_cast(float, (uint32_t)((i & 1) ? (r[i >> 1] & 0xffff0000u) : (r[i >> 1] << 16)));
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i >> 1] >> (16 * (i & 1))));
+}
+// (values are put in ascending order: an even one clears its neighbour)
+template <int T>
+__device__ __forceinline__ void put16(ccn_u32x4& r, int i, float v) {
+  if (T == 0) {
+    r[i] = __builtin_bit_cast(uint32_t, v);
+  } else {
+    uint32_t b;
+    if (T == 1) b = __builtin_bit_cast(uint16_t, (__bf16)v);
+    else b = __builtin_bit_cast(uint16_t, (_Float16)v);
+    r[i >> 1] = (i & 1) ? (r[i >> 1] | (b << 16)) : b;
+  }
+}
+template <int T>
+__device__ __forceinline__ ccn_u32x4 ld16(const void* p, int64_t i) {
+  return *reinterpret_cast<const typename CcnVec16<T>::mem*>(reinterpret_cast<const char*>(p) + i * (T == 0 ? 4 : 2));
+}
+template <int T>
+__device__ __forceinline__ void st16(void* p, int64_t i, const ccn_u32x4& r) {
+  *reinterpret_cast<typename CcnVec16<T>::mem*>(reinterpret_cast<char*>(p) + i * (T == 0 ? 4 : 2)) = r;
+}

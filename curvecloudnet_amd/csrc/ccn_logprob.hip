@@ -64,41 +64,16 @@ __device__ __forceinline__ LpRow lp_finish(float m, float total, float weighted)
   return r;
 }
 
-// 16 bytes of a row, at any alignment of the type.
-typedef uint32_t lp_u32x4 __attribute__((ext_vector_type(4)));
-template <int T> struct LpVec;
-template <> struct LpVec<0> {
-  static constexpr int N = 4;
-  static constexpr uint32_t FILL = 0xff800000u;      // -inf
-  typedef lp_u32x4 mem __attribute__((aligned(4)));
-};
-template <> struct LpVec<1> {
-  static constexpr int N = 8;
-  static constexpr uint32_t FILL = 0xff80ff80u;
-  typedef lp_u32x4 mem __attribute__((aligned(2)));
-};
-template <> struct LpVec<2> {
-  static constexpr int N = 8;
-  static constexpr uint32_t FILL = 0xfc00fc00u;
-  typedef lp_u32x4 mem __attribute__((aligned(2)));
-};
+// -inf throughout, in 32 bits of the type
 template <int T>
-__device__ __forceinline__ float lp_el(const lp_u32x4& r, int i) {
-  if (T == 0) return __uint_as_float(r[i]);
-  if (T == 1) return __uint_as_float((i & 1) ? (r[i >> 1] & 0xffff0000u) : (r[i >> 1] << 16));
-  return (float)__builtin_bit_cast(_Float16, (uint16_t)(r[i >> 1] >> (16 * (i & 1))));
-}
+constexpr uint32_t LP_FILL = T == 0 ? 0xff800000u : T == 1 ? 0xff80ff80u : 0xfc00fc00u;
+
+// 16 bytes of which only the first n values are the row's: the others are -inf and not read.
 template <int T>
-__device__ __forceinline__ lp_u32x4 lp_load(const void* __restrict__ x, int64_t at) {
-  constexpr int B = T == 0 ? 4 : 2;
-  return *reinterpret_cast<const typename LpVec<T>::mem*>(reinterpret_cast<const char*>(x) + at * B);
-}
-// ... of which only the first n values are the row's: the others are -inf and not read.
-template <int T>
-__device__ __forceinline__ lp_u32x4 lp_load_part(const void* __restrict__ x, int64_t at, int n) {
-  constexpr int V = LpVec<T>::N;
-  lp_u32x4 r = {LpVec<T>::FILL, LpVec<T>::FILL, LpVec<T>::FILL, LpVec<T>::FILL};
-  if (n >= V) return lp_load<T>(x, at);
+__device__ __forceinline__ ccn_u32x4 lp_load_part(const void* __restrict__ x, int64_t at, int n) {
+  constexpr int V = CcnVec16<T>::N;
+  ccn_u32x4 r = {LP_FILL<T>, LP_FILL<T>, LP_FILL<T>, LP_FILL<T>};
+  if (n >= V) return ld16<T>(x, at);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (i < n) {
@@ -114,7 +89,7 @@ __device__ __forceinline__ lp_u32x4 lp_load_part(const void* __restrict__ x, int
 
 // (what was computed from the values is computed again where it is rarely needed, and not kept in registers until then)
 template <int N>
-__device__ __forceinline__ void lp_forget(lp_u32x4 (&raw)[N]) {
+__device__ __forceinline__ void lp_forget(ccn_u32x4 (&raw)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j) asm volatile("" : "+v"(raw[j]));
 }
@@ -204,7 +179,7 @@ __device__ __forceinline__ bool lp_any(bool v) {
 // The class of the e-th logit that a thread holds.
 template <int T, int NT>
 __device__ __forceinline__ int lp_class(int c0, int tid, int e) {
-  constexpr int V = LpVec<T>::N;
+  constexpr int V = CcnVec16<T>::N;
   return c0 + ((e / V) * NT + tid) * V + e % V;
 }
 
@@ -216,7 +191,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
                                                               float2* __restrict__ stats, float* __restrict__ top_logprob,
                                                               int64_t* __restrict__ top_index, float4* __restrict__ part_stats,
                                                               uint64_t* __restrict__ part_keys) {
-  constexpr int NT = NW * 64, V = LpVec<T>::N, NJ = LP_HOLD / V, TILE = NT * LP_HOLD;
+  constexpr int NT = NW * 64, V = CcnVec16<T>::N, NJ = LP_HOLD / V, TILE = NT * LP_HOLD;
   __shared__ LpShared<NW> shared[4 / NW];
   LpShared<NW>& sh = shared[NW == 4 ? 0 : threadIdx.x >> 6];
   const int tid = NW == 4 ? threadIdx.x : threadIdx.x & 63, lane = threadIdx.x & 63, wave = NW == 4 ? threadIdx.x >> 6 : 0;
@@ -239,10 +214,10 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
   }
   for (int c0 = beg; c0 < end; c0 += TILE) {
     const int n = end - c0;
-    lp_u32x4 raw[NJ];
+    ccn_u32x4 raw[NJ];
     if (n >= TILE) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) raw[j] = lp_load<T>(x, at + c0 + (j * NT + tid) * V);
+      for (int j = 0; j < NJ; ++j) raw[j] = ld16<T>(x, at + c0 + (j * NT + tid) * V);
     } else {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, at + c0 + (j * NT + tid) * V, n - (j * NT + tid) * V);
@@ -252,7 +227,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
     for (int j = 0; j < NJ; ++j)
       if (j * NT * V < n) {
 #pragma unroll
-        for (int i = 0; i < V; i += 2) tm = lp_max(lp_max(tm, lp_el<T>(raw[j], i)), lp_el<T>(raw[j], i + 1));
+        for (int i = 0; i < V; i += 2) tm = lp_max(lp_max(tm, get16<T>(raw[j], i)), get16<T>(raw[j], i + 1));
       }
     const float mn = lp_max(m, tm), dm = lp_diff(m, mn), f = lp_exp(dm);
     w = f * (w + dm * s);
@@ -263,7 +238,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
       if (j * NT * V < n) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = lp_diff(lp_el<T>(raw[j], i), mn), e = lp_exp(d);
+          const float d = lp_diff(get16<T>(raw[j], i), mn), e = lp_exp(d);
           s += e;
           w = __builtin_fmaf(e, d, w);
         }
@@ -290,7 +265,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
         if (more) {
 #pragma unroll
           for (int e = 0; e < LP_HOLD; ++e) {
-            const float v = lp_el<T>(raw[e / V], e % V);
+            const float v = get16<T>(raw[e / V], e % V);
             const int c = ((e / V) * NT + tid) * V + e % V;
             if ((first ? !(v < limit) : !(v <= limit)) && c < n) pending |= 1u << e;
           }
@@ -440,7 +415,7 @@ __global__ __launch_bounds__(LP_NARROW_ROWS) void logprob_narrow_kernel(const vo
                                                                         float* __restrict__ top_logprob,
                                                                         int64_t* __restrict__ top_index) {
   extern __shared__ float tile[];
-  constexpr int V = LpVec<T>::N;
+  constexpr int V = CcnVec16<T>::N;
   const int P = C | 1;
   const int64_t r0 = (int64_t)blockIdx.x * LP_NARROW_ROWS;
   const int live = (int)min((int64_t)LP_NARROW_ROWS, rows - r0), n = live * C;
@@ -448,11 +423,11 @@ __global__ __launch_bounds__(LP_NARROW_ROWS) void logprob_narrow_kernel(const vo
   auto row_of = [&](int i) { return C == 1 ? i : (int)__umulhi((uint32_t)i, magic); };
   if (ld == C) {
     for (int i = threadIdx.x * V; i < n; i += LP_NARROW_ROWS * V) {
-      const lp_u32x4 raw = lp_load_part<T>(x, r0 * C + i, n - i);
+      const ccn_u32x4 raw = lp_load_part<T>(x, r0 * C + i, n - i);
       int r = row_of(i), c = i - r * C;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        if (i + k < n) tile[r * P + c] = lp_el<T>(raw, k);
+        if (i + k < n) tile[r * P + c] = get16<T>(raw, k);
         if (++c == C) {
           c = 0;
           ++r;
@@ -539,21 +514,10 @@ __device__ __forceinline__ float lp_smooth(const LpGrad& q, float v) {
   return lp_exp(l) * __builtin_fmaf(q.slope, l, q.flat);
 }
 template <int T>
-__device__ __forceinline__ void lp_put(lp_u32x4& r, int i, float v) {
-  if (T == 0) {
-    r[i] = __float_as_uint(v);
-  } else {
-    uint32_t b;
-    if (T == 1) b = __builtin_bit_cast(uint16_t, (__bf16)v);
-    else b = __builtin_bit_cast(uint16_t, (_Float16)v);
-    r[i >> 1] = (i & 1) ? (r[i >> 1] | (b << 16)) : b;
-  }
-}
-template <int T>
-__device__ __forceinline__ void lp_store_part(void* __restrict__ x, int64_t at, int n, const lp_u32x4& r) {
-  constexpr int V = LpVec<T>::N, B = T == 0 ? 4 : 2;
+__device__ __forceinline__ void lp_store_part(void* __restrict__ x, int64_t at, int n, const ccn_u32x4& r) {
+  constexpr int V = CcnVec16<T>::N;
   if (n >= V) {
-    *reinterpret_cast<typename LpVec<T>::mem*>(reinterpret_cast<char*>(x) + at * B) = r;
+    st16<T>(x, at, r);
     return;
   }
 #pragma unroll
@@ -565,14 +529,14 @@ __device__ __forceinline__ void lp_store_part(void* __restrict__ x, int64_t at, 
 }
 // 16 bytes of the gradient from 16 bytes of the row, c the class of the first.
 template <int T>
-__device__ __forceinline__ lp_u32x4 lp_grad16(const LpGrad& q, const lp_u32x4& raw, int c) {
-  constexpr int V = LpVec<T>::N;
-  lp_u32x4 out;
+__device__ __forceinline__ ccn_u32x4 lp_grad16(const LpGrad& q, const ccn_u32x4& raw, int c) {
+  constexpr int V = CcnVec16<T>::N;
+  ccn_u32x4 out;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    float d = lp_smooth(q, lp_el<T>(raw, i));
+    float d = lp_smooth(q, get16<T>(raw, i));
     if (c + i == q.t) d += q.g;
-    lp_put<T>(out, i, d);
+    put16<T>(out, i, d);
   }
   return out;
 }
@@ -599,7 +563,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_rows_kernel(
     int vecs, uint32_t magic, const int64_t* __restrict__ top_index, const float2* __restrict__ stats,
     const float* __restrict__ entropy, const float* __restrict__ g_logprob, int64_t g_logprob_stride,
     const float* __restrict__ g_entropy, int64_t g_entropy_stride, const float* __restrict__ g_top, void* __restrict__ dx, int64_t ldd) {
-  constexpr int V = LpVec<T>::N;
+  constexpr int V = CcnVec16<T>::N;
   __shared__ LpGrad mine[LP_TPB];
   const int64_t r0 = (int64_t)blockIdx.x * group;
   const int live = (int)min((int64_t)group, rows - r0), n = live * vecs;
@@ -609,7 +573,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_rows_kernel(
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += LP_TPB) {
     const int r = vecs == 1 ? i : (int)__umulhi((uint32_t)i, magic), c = (i - r * vecs) * V;
-    const lp_u32x4 raw = lp_load_part<T>(x, (r0 + r) * ld + c, C - c);
+    const ccn_u32x4 raw = lp_load_part<T>(x, (r0 + r) * ld + c, C - c);
     lp_store_part<T>(dx, (r0 + r) * ldd + c, C - c, lp_grad16<T>(mine[r], raw, c));
   }
   if (top == 0) return;
@@ -628,13 +592,13 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
     const int64_t* __restrict__ top_index, const float2* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ g_logprob, int64_t g_logprob_stride, const float* __restrict__ g_entropy, int64_t g_entropy_stride,
     const float* __restrict__ g_top, void* __restrict__ dx, int64_t ldd) {
-  constexpr int V = LpVec<T>::N, NJ = LP_HOLD / V, TILE = LP_TPB * LP_HOLD;
+  constexpr int V = CcnVec16<T>::N, NJ = LP_HOLD / V, TILE = LP_TPB * LP_HOLD;
   const int64_t row = blockIdx.x / (unsigned)tiles, at = row * ld, to = row * ldd;
   const int c0 = (int)(blockIdx.x % (unsigned)tiles) * TILE, n = min(C - c0, TILE), tid = threadIdx.x;
-  lp_u32x4 raw[NJ];
+  ccn_u32x4 raw[NJ];
   if (n == TILE) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) raw[j] = lp_load<T>(x, at + c0 + (j * LP_TPB + tid) * V);
+    for (int j = 0; j < NJ; ++j) raw[j] = ld16<T>(x, at + c0 + (j * LP_TPB + tid) * V);
   } else {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, at + c0 + (j * LP_TPB + tid) * V, n - (j * LP_TPB + tid) * V);

@@ -92,7 +92,7 @@ def test_many_tensors_of_mixed_types(flat, shift, kind):
         _check_clip(_params(sizes, [d] * len(sizes), flat=flat, shift=shift), 1.0, kind)
 
 
-@pytest.mark.parametrize("n", [1, 63, 64, 65, 159, 160, 161, 319, 320, 321, 1000])
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 159, 160, 161, 319, 320, 321, 640, 641, 1000])
 def test_more_tensors_than_a_launch_holds(n):
     _check_clip(_params([(1 + i % 37,) for i in range(n)], [DTYPES[i % 3] for i in range(n)]), 0.5)
 

@@ -147,5 +147,5 @@ def test_c_entries_of_the_norm_refuse():
                        (lambda: adam(m=(0x1000,)), "share"), (lambda: adam(v=(0x2000,)), "share"), (lambda: adam(g=(0x1000,)), "share"),
                        (lambda: adam(p=(0,)), "null"), (lambda: adam(wn=8), "workspace"), (lambda: adam(out=null), "null")):
         assert call() < 0 and word in err(), (word, err())
-    sizes = [lib.ccn_grad_norm_workspace_bytes(n) for n in (0, 1, 160, 161, 1000, 1 << 20)]
+    sizes = [lib.ccn_grad_norm_workspace_bytes(n) for n in (0, 1, 160, 161, 320, 321, 1000, 1 << 20)]
     assert sizes == sorted(sizes) and 0 < sizes[0] and sizes[-1] < 1 << 30 and lib.ccn_grad_norm_workspace_bytes(-1) == 0
