@@ -18,6 +18,14 @@ constexpr int CLIP_TPB = 256;
 constexpr int CLIP_MAX = 320;                      // tensors of one launch: 12 bytes of arguments each
 constexpr int CLIP_PART_MAX = 1024;                // workgroups of one launch of the norm, each with a partial result
 constexpr int CLIP_CHUNK = 16384;                  // values that a workgroup takes at a time
+#ifndef CG
+#define CG 64
+#endif
+#ifndef AG
+#define AG 64
+#endif
+constexpr int CLIP_GRID = CG * 1024;               // workgroups of one launch of the clipping
+constexpr int ADAM_GRID = AG * 1024;               // ... and of the update
 
 // Tensor i is chunks first[i] ... first[i + 1] - 1.  at[i]: its address (bits 0-47), the length of its last chunk less one (48-61),
 // its type (62-63).
@@ -113,12 +121,9 @@ template <int KIND>
 __global__ __launch_bounds__(CLIP_TPB) void grad_norm_kernel(const ClipTable t, double* __restrict__ partial) {
   __shared__ double red[CLIP_TPB / 64];
   const int chunks = t.first[t.n];
-  // (a workgroup's chunks lie next to one another)
-  const int beg = (int)((int64_t)blockIdx.x * chunks / gridDim.x), end = (int)(((int64_t)blockIdx.x + 1) * chunks / gridDim.x);
   ClipAcc<KIND> a;
-  int i = clip_find(t.first, t.n, beg);
-  for (int c = beg; c < end; ++c) {
-    if (c == t.first[i + 1]) ++i;
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int i = clip_find(t.first, t.n, c);
     const uint64_t at = t.at[i];
     const int n = c + 1 == t.first[i + 1] ? (int)((at >> 48) & 0x3fff) + 1 : CLIP_CHUNK, type = (int)(at >> 62);
     const char* const p = reinterpret_cast<const char*>(at & 0xffffffffffffull) + (int64_t)(c - t.first[i]) * CLIP_CHUNK * (type ? 2 : 4);
@@ -143,12 +148,16 @@ __device__ __forceinline__ float clip_scale(double norm, double max_norm) {
   return s != s ? NAN : s < 1.0 ? (float)s : 1.f;       // (a NaN norm makes every gradient NaN; an infinite one makes them 0)
 }
 
+// The norm, and the factor of the kernels that follow where there are many of their workgroups.
 template <int KIND>
-__global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double* __restrict__ partial, int n,
-                                                                   float* __restrict__ norm) {
+__global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double* __restrict__ partial, int n, double max_norm,
+                                                                   float* __restrict__ norm, float* __restrict__ scale) {
   __shared__ double red[CLIP_TPB / 64];
   const double v = clip_total<KIND>(partial, n, red);
-  if (threadIdx.x == 0) *norm = (float)v;
+  if (threadIdx.x == 0) {
+    *norm = (float)v;
+    if (scale) *scale = clip_scale(v, max_norm);
+  }
 }
 
 template <int T>
@@ -175,18 +184,21 @@ __device__ __forceinline__ void clip_apply(char* p, int n, float scale) {
 
 template <int KIND>
 __global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, const double* __restrict__ partial, int count,
-                                                             double max_norm, float* __restrict__ norm) {
+                                                             double max_norm, float* __restrict__ norm,
+                                                             const float* __restrict__ ready) {
   __shared__ double red[CLIP_TPB / 64];
-  const double v = clip_total<KIND>(partial, count, red);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-  const float scale = clip_scale(v, max_norm);
+  float scale;
+  if (ready) {
+    scale = *ready;
+  } else {
+    const double v = clip_total<KIND>(partial, count, red);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
+    scale = clip_scale(v, max_norm);
+  }
   if (scale == 1.f) return;
-  const int chunks = t.first[t.n];
-  const int beg = (int)((int64_t)blockIdx.x * chunks / gridDim.x), end = (int)(((int64_t)blockIdx.x + 1) * chunks / gridDim.x);
-  // (from the last to the first: what the norm read last is the likeliest to sit in a cache still)
-  int i = clip_find(t.first, t.n, end - 1);
-  for (int c = end - 1; c >= beg; --c) {
-    if (c < t.first[i]) --i;
+  // (from the last chunk to the first: what the norm read last is the likeliest to sit in a cache still)
+  for (int c = t.first[t.n] - 1 - (int)blockIdx.x; c >= 0; c -= (int)gridDim.x) {
+    const int i = clip_find(t.first, t.n, c);
     const uint64_t at = t.at[i];
     const int n = c + 1 == t.first[i + 1] ? (int)((at >> 48) & 0x3fff) + 1 : CLIP_CHUNK, type = (int)(at >> 62);
     char* const p = reinterpret_cast<char*>(at & 0xffffffffffffull) + (int64_t)(c - t.first[i]) * CLIP_CHUNK * (type ? 2 : 4);
@@ -198,6 +210,10 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, 
 
 // ---- Adam over several runs of parameters with the gradients scaled on the way
 constexpr int ADAM_MAX = 64;
+#ifndef ACHK
+#define ACHK 4096
+#endif
+constexpr int ADAM_CHUNK = ACHK;
 
 struct AdamTable {
   float* p[ADAM_MAX];
@@ -221,19 +237,21 @@ __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, 
 }
 
 __global__ __launch_bounds__(CLIP_TPB) void adam_clip_kernel(const AdamTable t, const double* __restrict__ partial, int count,
-                                                             double max_norm, float* __restrict__ norm, AdamCoef k) {
+                                                             double max_norm, float* __restrict__ norm,
+                                                             const float* __restrict__ ready, AdamCoef k) {
   __shared__ double red[CLIP_TPB / 64];
-  const double total = clip_total<NORM_TWO>(partial, count, red);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
-  k.scale = clip_scale(total, max_norm);
-  const int chunks = t.first[t.n];
-  const int beg = (int)((int64_t)blockIdx.x * chunks / gridDim.x), end = (int)(((int64_t)blockIdx.x + 1) * chunks / gridDim.x);
-  int i = __builtin_amdgcn_readfirstlane(__builtin_popcountll(
-              __builtin_amdgcn_ballot_w64((int)(threadIdx.x & 63) < t.n && t.first[threadIdx.x & 63] <= end - 1))) - 1;
-  for (int c = end - 1; c >= beg; --c) {             // (from the last to the first, as in grad_clip_kernel)
-    if (c < t.first[i]) --i;
-    const int64_t from = (int64_t)(c - t.first[i]) * CLIP_CHUNK;
-    const int n = (int)min((int64_t)CLIP_CHUNK, t.size[i] - from);
+  if (ready) {
+    k.scale = *ready;
+  } else {
+    const double total = clip_total<NORM_TWO>(partial, count, red);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+    k.scale = clip_scale(total, max_norm);
+  }
+  for (int c = t.first[t.n] - 1 - (int)blockIdx.x; c >= 0; c -= (int)gridDim.x) {     // (as in grad_clip_kernel)
+    const int lane = threadIdx.x & 63;
+    const int i = __builtin_amdgcn_readfirstlane(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < t.n && t.first[lane] <= c))) - 1;
+    const int64_t from = (int64_t)(c - t.first[i]) * ADAM_CHUNK;
+    const int n = (int)min((int64_t)ADAM_CHUNK, t.size[i] - from);
     float* const p = t.p[i] + from;
     const float* const g = t.g[i] + from;
     float* const m = t.m[i] + from;
@@ -291,7 +309,7 @@ int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype
   return CCN_OK;
 }
 
-int clip_chunks(int64_t size) { return (int)((size + CLIP_CHUNK - 1) / CLIP_CHUNK); }
+int clip_chunks(int64_t size, int chunk) { return (int)((size + chunk - 1) / chunk); }
 
 // The tables of the launches that a list of tensors takes: f(table) for each.
 template <typename F>
@@ -302,7 +320,7 @@ int clip_tables(const void* const* ptr, const int64_t* size, const int32_t* dtyp
   for (int64_t i = 0; i < n; ++i) {
     if (size[i] == 0) continue;
     t.at[t.n] = (uint64_t)(uintptr_t)ptr[i] | ((uint64_t)((size[i] - 1) % CLIP_CHUNK) << 48) | ((uint64_t)(dtype ? dtype[i] : 0) << 62);
-    t.first[t.n + 1] = t.first[t.n] + clip_chunks(size[i]);
+    t.first[t.n + 1] = t.first[t.n] + clip_chunks(size[i], CLIP_CHUNK);
     if (++t.n == CLIP_MAX) {
       if (int rc = f(t)) return rc;
       t.n = 0;
@@ -311,45 +329,64 @@ int clip_tables(const void* const* ptr, const int64_t* size, const int32_t* dtyp
   return t.n ? f(t) : CCN_OK;
 }
 
+#define CLIP_KINDS(kind, KERNEL, ...)                                                              \
+  do {                                                                                             \
+    if ((kind) == NORM_TWO) hipLaunchKernelGGL(KERNEL<NORM_TWO>, __VA_ARGS__);                     \
+    else if ((kind) == NORM_SUM) hipLaunchKernelGGL(KERNEL<NORM_SUM>, __VA_ARGS__);                \
+    else hipLaunchKernelGGL(KERNEL<NORM_MAX>, __VA_ARGS__);                                        \
+  } while (0)
+
+int clip_grid(int chunks, int most) { return chunks < most ? chunks : most; }
+
 // The partial results of the norm: *count of them, at `partial`.
 int clip_norm_launches(const void* const* ptr, const int64_t* size, const int32_t* dtype, int64_t n, int kind, double* partial,
                        int* count, hipStream_t s) {
   *count = 0;
   return clip_tables(ptr, size, dtype, n, [&](const ClipTable& t) {
-    const int chunks = t.first[t.n], grid = chunks < CLIP_PART_MAX ? chunks : CLIP_PART_MAX;
-    double* const to = partial + *count;
-    if (kind == NORM_TWO) hipLaunchKernelGGL(grad_norm_kernel<NORM_TWO>, dim3(grid), dim3(CLIP_TPB), 0, s, t, to);
-    else if (kind == NORM_SUM) hipLaunchKernelGGL(grad_norm_kernel<NORM_SUM>, dim3(grid), dim3(CLIP_TPB), 0, s, t, to);
-    else hipLaunchKernelGGL(grad_norm_kernel<NORM_MAX>, dim3(grid), dim3(CLIP_TPB), 0, s, t, to);
+    const int grid = clip_grid(t.first[t.n], CLIP_PART_MAX);
+    CLIP_KINDS(kind, grad_norm_kernel, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial + *count);
     *count += grid;
     return CCN_OK;
   });
 }
 
+int clip_outputs(const void* norm, const void* ws, size_t ws_bytes, int64_t n, const char* who) {
+  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "%s: null norm or workspace", who);
+  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
+    ccn_set_error("%s: workspace %zu < %zu bytes", who, ws_bytes, ccn_grad_norm_workspace_bytes(n));
+    return CCN_ERR_WORKSPACE;
+  }
+  return CCN_OK;
+}
+
+// Where the kernels that apply the factor have more workgroups than CLIP_PART_MAX, each of them adding up the partial results costs
+// more than a launch that does it once.
+float* clip_factor(int kind, const double* partial, int count, double max_norm, float* norm, int64_t chunks, hipStream_t s) {
+  if (count > 0 && chunks <= CLIP_PART_MAX) return nullptr;
+  float* const factor = (float*)const_cast<double*>(partial + count);
+  CLIP_KINDS(kind, grad_norm_final_kernel, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, max_norm, norm, factor);
+  return factor;
+}
+
 }  // namespace
 
+// (a partial result for every workgroup, and the factor behind them)
 extern "C" size_t ccn_grad_norm_workspace_bytes(int64_t n) {
   if (n < 0) return 0;
   const int64_t launches = (n + CLIP_MAX - 1) / CLIP_MAX;
-  return ccn_align256((size_t)(launches < 1 ? 1 : launches) * CLIP_PART_MAX * sizeof(double));
+  return ccn_align256(((size_t)(launches < 1 ? 1 : launches) * CLIP_PART_MAX + 1) * sizeof(double));
 }
 
 extern "C" int ccn_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, void* ws,
                              size_t ws_bytes, float* norm, void* stream) {
   if (int rc = clip_check(grads, sizes, dtypes, n, false, "grad_norm")) return rc;
   CCN_REQUIRE(kind >= NORM_SUM && kind <= NORM_MAX, "grad_norm: kind %d is not 1 (sum), 2 (two) or 3 (max)", kind);
-  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "grad_norm: null norm or workspace");
-  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
-    ccn_set_error("grad_norm: workspace %zu < %zu bytes", ws_bytes, ccn_grad_norm_workspace_bytes(n));
-    return CCN_ERR_WORKSPACE;
-  }
+  if (int rc = clip_outputs(norm, ws, ws_bytes, n, "grad_norm")) return rc;
   double* const partial = (double*)ws;
   int count = 0;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = clip_norm_launches(grads, sizes, dtypes, n, kind, partial, &count, s)) return rc;
-  if (kind == NORM_TWO) hipLaunchKernelGGL(grad_norm_final_kernel<NORM_TWO>, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, norm);
-  else if (kind == NORM_SUM) hipLaunchKernelGGL(grad_norm_final_kernel<NORM_SUM>, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, norm);
-  else hipLaunchKernelGGL(grad_norm_final_kernel<NORM_MAX>, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, norm);
+  CLIP_KINDS(kind, grad_norm_final_kernel, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, 0.0, norm, nullptr);
   CCN_LAUNCH_OK("grad_norm");
   return CCN_OK;
 }
@@ -359,29 +396,18 @@ extern "C" int ccn_grad_clip(void* const* grads, const int64_t* sizes, const int
   if (int rc = clip_check(grads, sizes, dtypes, n, true, "grad_clip")) return rc;
   CCN_REQUIRE(kind >= NORM_SUM && kind <= NORM_MAX, "grad_clip: kind %d is not 1 (sum), 2 (two) or 3 (max)", kind);
   CCN_REQUIRE(max_norm >= 0.0, "grad_clip: max_norm %g", max_norm);
-  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "grad_clip: null norm or workspace");
-  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
-    ccn_set_error("grad_clip: workspace %zu < %zu bytes", ws_bytes, ccn_grad_norm_workspace_bytes(n));
-    return CCN_ERR_WORKSPACE;
-  }
+  if (int rc = clip_outputs(norm, ws, ws_bytes, n, "grad_clip")) return rc;
   double* const partial = (double*)ws;
   int count = 0;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < n; ++i) chunks += clip_chunks(sizes[i], CLIP_CHUNK);
   hipStream_t s = (hipStream_t)stream;
   if (int rc = clip_norm_launches(grads, sizes, dtypes, n, kind, partial, &count, s)) return rc;
-  if (count == 0) {
-    hipLaunchKernelGGL(grad_norm_final_kernel<NORM_SUM>, dim3(1), dim3(CLIP_TPB), 0, s, partial, 0, norm);
-    CCN_LAUNCH_OK("grad_clip");
-    return CCN_OK;
-  }
-  float* out = norm;
+  const float* const factor = clip_factor(kind, partial, count, max_norm, norm, chunks, s);
+  float* out = factor ? nullptr : norm;
   const int rc = clip_tables(grads, sizes, dtypes, n, [&](const ClipTable& t) {
-    const int chunks = t.first[t.n], grid = chunks < CLIP_PART_MAX ? chunks : CLIP_PART_MAX;
-    if (kind == NORM_TWO)
-      hipLaunchKernelGGL(grad_clip_kernel<NORM_TWO>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
-    else if (kind == NORM_SUM)
-      hipLaunchKernelGGL(grad_clip_kernel<NORM_SUM>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
-    else
-      hipLaunchKernelGGL(grad_clip_kernel<NORM_MAX>, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out);
+    CLIP_KINDS(kind, grad_clip_kernel, dim3(clip_grid(t.first[t.n], CLIP_GRID)), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm,
+               out, factor);
     out = nullptr;
     return CCN_OK;
   });
@@ -400,37 +426,32 @@ extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, fl
   if (int rc = clip_check((const void* const*)grads, sizes, nullptr, n, false, "adam_clip")) return rc;
   std::vector<const void*> all;
   std::vector<int64_t> every;
+  int64_t chunks = 0;
   try {                                              // nothing that is written may share memory with anything else that is used
-    for (int64_t i = 0; i < n; ++i)
+    for (int64_t i = 0; i < n; ++i) {
+      chunks += clip_chunks(sizes[i], ADAM_CHUNK);
       for (const void* p : {(const void*)params[i], (const void*)grads[i], (const void*)exp_avgs[i], (const void*)exp_avg_sqs[i]}) {
-        CCN_REQUIRE(size_t(p) % 16 == 0, "adam_clip: buffers must be 16-byte aligned");
+        CCN_REQUIRE((uintptr_t)p % 16 == 0, "adam_clip: buffers must be 16-byte aligned");
         all.push_back(p);
         every.push_back(sizes[i]);
       }
+    }
   } catch (...) {
     ccn_set_error("adam_clip: out of host memory");
     return CCN_ERR_ARG;
   }
   if (int rc = clip_check(all.data(), every.data(), nullptr, 4 * n, true, "adam_clip")) return rc;
-  CCN_REQUIRE(norm && ws && (uintptr_t)ws % 8 == 0, "adam_clip: null norm or workspace");
-  if (ws_bytes < ccn_grad_norm_workspace_bytes(n)) {
-    ccn_set_error("adam_clip: workspace %zu < %zu bytes", ws_bytes, ccn_grad_norm_workspace_bytes(n));
-    return CCN_ERR_WORKSPACE;
-  }
+  if (int rc = clip_outputs(norm, ws, ws_bytes, n, "adam_clip")) return rc;
   double* const partial = (double*)ws;
   int count = 0;
   hipStream_t s = (hipStream_t)stream;
   if (int rc = clip_norm_launches((const void* const*)grads, sizes, nullptr, n, NORM_TWO, partial, &count, s)) return rc;
-  if (count == 0) {
-    hipLaunchKernelGGL(grad_norm_final_kernel<NORM_TWO>, dim3(1), dim3(CLIP_TPB), 0, s, partial, 0, norm);
-    CCN_LAUNCH_OK("adam_clip");
-    return CCN_OK;
-  }
+  const float* const factor = clip_factor(NORM_TWO, partial, count, max_norm, norm, chunks, s);
+  float* out = factor ? nullptr : norm;
   // bias corrections and 1 - beta in double on the host (1 - 0.999 from a beta in 32 bits is off by 1.3e-5 of itself)
   const double bc1 = 1.0 - pow(beta1, (double)step), bc2 = 1.0 - pow(beta2, (double)step);
   const AdamCoef coef = {1.f, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)(lr / bc1), (float)(1.0 / sqrt(bc2)),
                          (float)eps, (float)weight_decay};
-  float* out = norm;
   AdamTable t;
   t.n = 0;
   t.first[0] = 0;
@@ -441,12 +462,12 @@ extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, fl
       t.m[t.n] = exp_avgs[i];
       t.v[t.n] = exp_avg_sqs[i];
       t.size[t.n] = sizes[i];
-      t.first[t.n + 1] = t.first[t.n] + clip_chunks(sizes[i]);
+      t.first[t.n + 1] = t.first[t.n] + clip_chunks(sizes[i], ADAM_CHUNK);
       ++t.n;
     }
     if (t.n == ADAM_MAX || (i == n - 1 && t.n > 0)) {
-      const int chunks = t.first[t.n], grid = chunks < 2 * CLIP_PART_MAX ? chunks : 2 * CLIP_PART_MAX;
-      hipLaunchKernelGGL(adam_clip_kernel, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm, out, coef);
+      hipLaunchKernelGGL(adam_clip_kernel, dim3(clip_grid(t.first[t.n], ADAM_GRID)), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm,
+                         out, factor, coef);
       out = nullptr;
       t.n = 0;
     }
