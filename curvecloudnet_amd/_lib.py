@@ -4,6 +4,7 @@ The prototypes are read from the header itself, so the header is the single sour
 the boundary.  There is NO fallback: if the shared library is missing, or an op is called without
 a GPU tensor, this raises.
 """
+import contextlib
 import ctypes
 import os
 import re
@@ -98,7 +99,16 @@ def ptr(t):
 
 
 def stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current torch stream of the current device, as the C ABI takes it."""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+def on_device(index):
+    """``with on_device(t.get_device()):`` launches beside ``t``, at no cost where that device is the current one already."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def check(rc, what):

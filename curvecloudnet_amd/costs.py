@@ -180,10 +180,10 @@ _TABLE = {
     # (dtype, ld, rows, C, ignore, top, …): logits, target; logprob and entropy, alternatives / + the gradient's read and write
     "logprob_fwd": ("loss_optim", lambda i, r: (F32, 2.0, 2.0)[i[0]] * _rc(i, 2, 3) + (16.0 + 12.0 * i[5]) * i[2]),
     "logprob_bwd": ("loss_optim", lambda i, r: 2 * (F32, 2.0, 2.0)[i[0]] * _rc(i, 2, 3) + (28.0 + 12.0 * i[5]) * i[2]),
-    # (work_rows: BYTES of the gradients, whose sizes travel in tables)
-    "grad_norm": ("loss_optim", lambda i, r: float(r)),
-    "grad_clip": ("loss_optim", lambda i, r: 2.0 * r),
-    "adam_clip": ("loss_optim", lambda i, r: 7.0 * r),
+    # (work_rows: the gradients' values, whose sizes travel in tables; priced as the fp32 of the flat buckets)
+    "grad_norm": ("loss_optim", lambda i, r: F32 * r),
+    "grad_clip": ("loss_optim", lambda i, r: 2 * F32 * r),
+    "adam_clip": ("loss_optim", lambda i, r: 7 * F32 * r),
 }
 
 _GEOMETRY_PREFIXES = ("frnn_", "fps", "curve_fps", "curve_group", "curve_topology", "curve_split", "segment_ptr", "knn_",

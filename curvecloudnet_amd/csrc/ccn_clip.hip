@@ -18,14 +18,7 @@ constexpr int CLIP_TPB = 256;
 constexpr int CLIP_MAX = 320;                      // tensors of one launch: 12 bytes of arguments each
 constexpr int CLIP_PART_MAX = 1024;                // workgroups of one launch of the norm, each with a partial result
 constexpr int CLIP_CHUNK = 16384;                  // values that a workgroup takes at a time
-#ifndef CG
-#define CG 64
-#endif
-#ifndef AG
-#define AG 64
-#endif
-constexpr int CLIP_GRID = CG * 1024;               // workgroups of one launch of the clipping
-constexpr int ADAM_GRID = AG * 1024;               // ... and of the update
+constexpr int CLIP_GRID = 64 * 1024;               // workgroups of one launch of the clipping, and of the update
 
 // Tensor i is chunks first[i] ... first[i + 1] - 1.  at[i]: its address (bits 0-47), the length of its last chunk less one (48-61),
 // its type (62-63).
@@ -210,10 +203,7 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, 
 
 // ---- Adam over several runs of parameters with the gradients scaled on the way
 constexpr int ADAM_MAX = 64;
-#ifndef ACHK
-#define ACHK 4096
-#endif
-constexpr int ADAM_CHUNK = ACHK;
+constexpr int ADAM_CHUNK = 4096;
 
 struct AdamTable {
   float* p[ADAM_MAX];
@@ -466,7 +456,7 @@ extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, fl
       ++t.n;
     }
     if (t.n == ADAM_MAX || (i == n - 1 && t.n > 0)) {
-      hipLaunchKernelGGL(adam_clip_kernel, dim3(clip_grid(t.first[t.n], ADAM_GRID)), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm,
+      hipLaunchKernelGGL(adam_clip_kernel, dim3(clip_grid(t.first[t.n], CLIP_GRID)), dim3(CLIP_TPB), 0, s, t, partial, count, max_norm,
                          out, factor, coef);
       out = nullptr;
       t.n = 0;

@@ -59,34 +59,33 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
     The gradient has the logits' type, its rows 16-byte aligned (their stride padded where C is odd)."""
     if logits.dtype not in ops.LOGIT_DTYPES:
         raise TypeError("token_logprobs: logits are %s; fp32, bf16 or fp16 is wanted" % logits.dtype)
-    if target.dtype not in (torch.int64, torch.int32):
+    if target.dtype is not torch.int64 and target.dtype is not torch.int32:
         raise TypeError("token_logprobs: target is %s; int64 or int32 is wanted" % target.dtype)
-    if target.is_cuda and logits.is_cuda and target.device != logits.device:
-        raise ValueError("token_logprobs: logits on %s, target on %s" % (logits.device, target.device))
-    if logits.dim() == 0 or logits.size(-1) == 0 or logits.size(-1) >= 1 << 30:
+    if logits.dim() == 0 or not 0 < logits.size(-1) < 1 << 30:
         raise ValueError("token_logprobs: logits of shape %s have no classes, or too many" % (tuple(logits.shape),))
-    shape, c = logits.shape[:-1], logits.size(-1)
+    shape, c, rows = logits.shape[:-1], logits.size(-1), target.numel()
     if target.shape != shape:
         raise ValueError("token_logprobs: logits of shape %s want a target of shape %s, got %s"
                          % (tuple(logits.shape), tuple(shape), tuple(target.shape)))
-    top = int(top)
-    if top < 0 or top > min(ops.TOP_MAX, c):
-        raise ValueError("token_logprobs: top=%d; 0 to %d is wanted" % (top, min(ops.TOP_MAX, c)))
-    rows = target.numel()
+    if not 0 <= top <= min(ops.TOP_MAX, c):
+        raise ValueError("token_logprobs: top=%r; 0 to %d is wanted" % (top, min(ops.TOP_MAX, c)))
     if rows >= 1 << 31:
         raise ValueError("token_logprobs: %d rows" % rows)
     require_gpu(logits, target)
-    x = logits if logits.dim() == 2 else logits.reshape(-1, c) if rows else logits.reshape(0, c)
+    if target.get_device() != logits.get_device():
+        raise ValueError("token_logprobs: logits on %s, target on %s" % (logits.device, target.device))
+    flat = logits.dim() == 2
+    x = logits if flat else logits.reshape(rows, c)
     # (one row: its stride is never used, and torch may report any)
     if (x.stride(1) != 1 and c > 1) or (rows > 1 and x.stride(0) < c):
         x = x.contiguous()
-    target = target.reshape(-1).to(torch.int64).contiguous()
-    with torch.cuda.device(logits.device):
-        if torch.is_grad_enabled() and logits.requires_grad:
-            out = ops.TokenLogProbs.apply(x, target, top, int(ignore_index))
-        else:
-            out = ops.logprob_forward(x.detach(), target, top, int(ignore_index), stats=False)[:4]
-    if len(shape) == 1:
+    if not flat or target.dtype is not torch.int64 or not target.is_contiguous():
+        target = target.reshape(-1).to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = ops.TokenLogProbs.apply(x, target, int(top), int(ignore_index))
+    else:
+        out = ops.logprob_forward(x, target, int(top), int(ignore_index), stats=False)[:4]
+    if flat:
         return Scores(*out)
     logprob, entropy, best, index = out
     return Scores(logprob.view(shape), entropy.view(shape), best.view(*shape, top) if top else None,

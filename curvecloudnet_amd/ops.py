@@ -9,7 +9,7 @@ import threading
 
 import torch
 
-from ._lib import call, lib, ptr, require_gpu, workspace
+from ._lib import call, lib, on_device, ptr, require_gpu, workspace
 
 ACT = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2}
 LEAKY_SLOPE = 0.01  # torch.nn.LeakyReLU default, the only slope the reference uses
@@ -1537,8 +1537,9 @@ def logprob_forward(logits, target, top, ignore_index, stats=True):
     if rows:
         nbytes = lib().ccn_logprob_workspace_bytes(rows, c, top)
         ws = workspace(nbytes, dev) if nbytes else None
-        call("logprob_fwd", ptr(logits), LOGIT_DTYPES[logits.dtype], logits.stride(0), ptr(target), rows, c, ignore_index, top,
-             ptr(logprob), ptr(entropy), ptr(stats), ptr(best), ptr(index), ptr(ws), nbytes)
+        with on_device(logits.get_device()):
+            call("logprob_fwd", ptr(logits), LOGIT_DTYPES[logits.dtype], logits.stride(0), ptr(target), rows, c, ignore_index, top,
+                 ptr(logprob), ptr(entropy), ptr(stats), ptr(best), ptr(index), ptr(ws), nbytes)
     return logprob, entropy, best, index, stats
 
 
@@ -1557,20 +1558,27 @@ class TokenLogProbs(torch.autograd.Function):
         return logprob, entropy, best, index
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_top, _):
-        logits, target, index, stats, entropy = ctx.saved_tensors
-        rows, c = logits.shape
-        d = _rows(rows, c, logits.device) if logits.dtype == torch.float32 else _rows16(rows, c, logits.device, logits.dtype)
-        if rows:
-            top = 0 if g_top is None else g_top.size(1)
-            g_top = g_top.contiguous() if top else None
-            with torch.cuda.device(logits.device):
-                call("logprob_bwd", ptr(logits), LOGIT_DTYPES[logits.dtype], logits.stride(0), ptr(target), rows, c, ctx.ignore, top,
-                     ptr(index) if top else None, ptr(stats), ptr(entropy), ptr(g_logprob),
-                     0 if g_logprob is None else g_logprob.stride(0), ptr(g_entropy),
-                     0 if g_entropy is None else g_entropy.stride(0), ptr(g_top), ptr(d), d.stride(0))
-        return d, None, None, None
+    def backward(ctx, *grads):
+        # (with create_graph: a graph behind the gradient that refuses to be differentiated; its bookkeeping costs 5 us)
+        return (_logprob_backward_once if torch.is_grad_enabled() else _logprob_backward)(ctx, *grads)
+
+
+def _logprob_backward(ctx, g_logprob, g_entropy, g_top, _):
+    logits, target, index, stats, entropy = ctx.saved_tensors
+    rows, c = logits.shape
+    d = _rows(rows, c, logits.device) if logits.dtype == torch.float32 else _rows16(rows, c, logits.device, logits.dtype)
+    if rows:
+        top = 0
+        if g_top is not None:
+            top, g_top = g_top.size(1), g_top.contiguous()
+        with on_device(logits.get_device()):
+            call("logprob_bwd", ptr(logits), LOGIT_DTYPES[logits.dtype], logits.stride(0), ptr(target), rows, c, ctx.ignore, top,
+                 ptr(index) if top else None, ptr(stats), ptr(entropy), ptr(g_logprob), 0 if g_logprob is None else g_logprob.stride(0),
+                 ptr(g_entropy), 0 if g_entropy is None else g_entropy.stride(0), ptr(g_top), ptr(d), d.stride(0))
+    return d, None, None, None
+
+
+_logprob_backward_once = torch.autograd.function.once_differentiable(_logprob_backward)
 
 
 # --------------------------------------------------------------------------------------

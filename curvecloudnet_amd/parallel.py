@@ -267,39 +267,54 @@ def _dense(t):
     return True
 
 
+_POINTER, _NUMEL, _PLACE, _PLAIN = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+_DTYPE, _GRAD = torch.Tensor.dtype.__get__, torch.Tensor.grad.__get__
+
+
 class _Tensors:
-    """The tables that the norm's entry points read on the host: addresses, sizes and types of tensors of one device."""
+    """The tables that the norm's entry points read on the host: addresses, sizes and types of tensors of one device.  (map over
+    unbound methods: half of what a comprehension costs, and a network has hundreds of tensors.)"""
 
     def __init__(self, tensors, who):
-        if any(t.layout is not torch.strided for t in tensors):
-            raise TypeError("%s: sparse tensors are not built" % who)
         try:
-            codes = [_GRAD_DTYPES[t.dtype] for t in tensors]
+            plain = all(map(_PLAIN, tensors))
+            pointers = array.array("q", list(map(_POINTER, tensors)))
+        except RuntimeError:
+            raise TypeError("%s: sparse tensors are not built" % who) from None
+        types = list(map(_DTYPE, tensors))
+        try:
+            codes = [_GRAD_DTYPES[t] for t in set(types)]
         except KeyError as e:
             raise TypeError("%s: %s; fp32, bf16 or fp16 is wanted" % (who, e.args[0])) from None
-        for t in tensors:
-            if not t.is_contiguous() and not _dense(t):
-                raise ValueError("%s: a tensor of strides %s does not fill its memory" % (who, tuple(t.stride())))
-        places = set(map(torch.Tensor.get_device, tensors))
+        if len(codes) > 1 or codes[0]:
+            codes = [_GRAD_DTYPES[t] for t in types]
+        else:
+            codes = None                        # (all fp32: no table)
+        if not plain:
+            for t in tensors:
+                if not t.is_contiguous() and not _dense(t):
+                    raise ValueError("%s: a tensor of strides %s does not fill its memory" % (who, tuple(t.stride())))
+        places = set(map(_PLACE, tensors))
         if -1 in places:
             raise RuntimeError("curvecloudnet_amd ops run on the GPU only (got a cpu tensor); there is no CPU path")
         if len(places) != 1:
             raise ValueError("%s: tensors on %d devices; one is wanted" % (who, len(places)))
         self.place = places.pop()
-        sizes = [t.numel() for t in tensors]
         self.n = len(tensors)
-        self.nbytes = sum(n * (4, 2, 2)[k] for n, k in zip(sizes, codes))
-        self.keep = [array.array("q", (t.data_ptr() for t in tensors)), array.array("q", sizes), array.array("i", codes)]
-        self.ptrs, self.sizes, self.codes = (ctypes.c_void_p(a.buffer_info()[0]) for a in self.keep)
+        sizes = list(map(_NUMEL, tensors))
+        self.total = sum(sizes)
+        self.pointers, self.lengths = pointers, array.array("q", sizes)
+        self.keep = None if codes is None else array.array("i", codes)
+        self.ptrs, self.sizes = ctypes.c_void_p(pointers.buffer_info()[0]), ctypes.c_void_p(self.lengths.buffer_info()[0])
+        self.codes = None if codes is None else ctypes.c_void_p(self.keep.buffer_info()[0])
 
 
 def _norm_call(entry, tables, *args):
-    from ._lib import call, lib, ptr, workspace
-    with torch.cuda.device(tables.place):
-        dev = torch.device("cuda", tables.place)
+    from ._lib import call, lib, on_device, ptr
+    with on_device(tables.place):
         nbytes = lib().ccn_grad_norm_workspace_bytes(tables.n)
-        ws, norm = workspace(nbytes, dev), torch.empty((), dtype=torch.float32, device=dev)
-        call(entry, *args, ptr(ws), nbytes, ptr(norm), work_rows=tables.nbytes)
+        ws, norm = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), torch.empty((), dtype=torch.float32, device="cuda")
+        call(entry, *args, ptr(ws), nbytes, ptr(norm), work_rows=tables.total)
     return norm
 
 
@@ -322,7 +337,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     32 bits and rounded once to the gradient's type.  A norm that is not finite gives what the formula gives (0 or NaN), or raises with
     ``error_if_nonfinite`` (which waits for the GPU) before anything is scaled.  Gradients that share memory are refused."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    grads = [g for g in map(_GRAD, parameters) if g is not None]
     kind, max_norm = _norm_kind(norm_type, "clip_grad_norm_"), _bound(max_norm, "clip_grad_norm_")
     if not grads:
         return torch.zeros(())
@@ -359,7 +374,7 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     for t in tables:
         if t.place != tables[0].place:
             raise ValueError("adam_step_: the tensors of a parameter are on one device")
-        if any(p % 16 for p in t.keep[0]):
+        if any(p % 16 for p in t.pointers):
             raise ValueError("adam_step_: a tensor does not start at a multiple of 16 bytes")
     return _adam(tables, step, lr, betas, eps, weight_decay, max_norm)
 
@@ -370,9 +385,9 @@ def _adam(tables, step, lr, betas, eps, weight_decay, max_norm):
     _join_wgrad()
     if max_norm is not None:
         return _norm_call("adam_clip", g, p.ptrs, g.ptrs, m.ptrs, v.ptrs, g.sizes, g.n, *rest, max_norm)
-    from ._lib import call
-    with torch.cuda.device(g.place):
-        for at in zip(*(t.keep[0] for t in tables), g.keep[1]):
+    from ._lib import call, on_device
+    with on_device(g.place):
+        for at in zip(*(t.pointers for t in tables), g.lengths):
             call("adam_step", *map(ctypes.c_void_p, at[:4]), at[4], *rest)
 
 
