@@ -4,7 +4,6 @@ The prototypes are read from the header itself, so the header is the single sour
 the boundary.  There is NO fallback: if the shared library is missing, or an op is called without
 a GPU tensor, this raises.
 """
-import contextlib
 import ctypes
 import os
 import re
@@ -103,14 +102,6 @@ def stream():
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
-def on_device(index):
-    """``with on_device(t.get_device()):`` launches beside ``t``, at no cost where that device is the current one already."""
-    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
-
-
-_HERE = contextlib.nullcontext()
-
-
 def check(rc, what):
     if rc != 0:
         raise RuntimeError("libccn_hip %s failed (%d): %s" % (what, rc, lib().ccn_last_error().decode()))
@@ -136,6 +127,19 @@ def call(name, *args, work_rows=None):
     the edge-sized operand where the prototype does not carry it (CSR aggregations) -- recorded for bench.py's step
     roofline (curvecloudnet_amd.costs), never passed to the library."""
     fn = getattr(lib(), "ccn_" + name)
+    if not _watched():
+        check(fn(*args, stream()), name)
+        return
+    # (a product with scratch is recorded as the product: its name, its arguments without the trailing scratch pair)
+    pname, pargs = (PROFILE_ALIAS[name], args[:-2]) if name in PROFILE_ALIAS else (name, args)
+    _observe(name, args, pname, pargs, work_rows, lambda: check(fn(*args, stream()), name))
+
+
+def _watched():
+    return PROFILE is not None or DEBUG_SYNC is not None or EXTRA_LAUNCH is not None
+
+
+def _observe(name, args, pname, pargs, work_rows, run):
     if EXTRA_LAUNCH is not None:
         EXTRA_LAUNCH()
     if DEBUG_SYNC is not None:
@@ -143,26 +147,43 @@ def call(name, *args, work_rows=None):
         # AFTER it -- the last line of the file is the launch that faulted
         with open(DEBUG_SYNC, "a") as f:
             f.write("%s %s\n" % (name, [a for a in args if isinstance(a, int)]))
-        check(fn(*args, stream()), name)
+        run()
         torch.cuda.synchronize()
         return
-    if PROFILE is None:
-        check(fn(*args, stream()), name)
-        return
-    # (a product with scratch is recorded as the product: its name, its arguments without the trailing scratch pair)
-    pname, pargs = (PROFILE_ALIAS[name], args[:-2]) if name in PROFILE_ALIAS else (name, args)
-    if ((PROFILE_ONLY is not None and not pname.startswith(PROFILE_ONLY))
+    if (PROFILE is None or (PROFILE_ONLY is not None and not pname.startswith(PROFILE_ONLY))
             or (PROFILE_FILTER is not None and not PROFILE_FILTER(pname, pargs))):
-        check(fn(*args, stream()), name)
+        run()
         return
     # torch.cuda.Event records on torch's current stream, which is exactly the stream passed to the kernel
     beg, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     beg.record()
-    check(fn(*args, stream()), name)
+    run()
     end.record()
     # integer arguments (sizes / leading dimensions) and the positions of NULL pointers identify the kernel variant
     PROFILE.append((pname, tuple(a for a in pargs if isinstance(a, int)), beg, end,
                     tuple(i for i, a in enumerate(pargs) if a is None), work_rows))
+
+
+_binding, _observing = None, False
+
+
+def binding():
+    """The operators bound to torch in C++ (csrc/ccn_torch.cpp), over the library of ``lib()``.  There is no fallback."""
+    global _binding, _observing
+    if _binding is None:
+        handle = lib()
+        try:
+            from . import _ccn_torch as module
+        except ImportError as e:
+            raise RuntimeError("curvecloudnet_amd: _ccn_torch.so is missing or does not fit this torch (%s) -- build it with "
+                               "`make -C curvecloudnet_amd/csrc`" % e) from e
+        module.bind({name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in parse_header(HEADER_PATH)
+                     if hasattr(handle, name)})
+        _binding = module
+    if _observing != _watched():
+        _observing = not _observing
+        _binding.observe((lambda name, ints, work, run: _observe(name, ints, name, ints, work, run)) if _observing else None)
+    return _binding
 
 
 def require_gpu(*tensors):

@@ -10,8 +10,7 @@ from typing import NamedTuple, Optional
 import torch
 import torch.nn.functional as F
 
-from . import ops
-from ._lib import require_gpu
+from ._lib import binding
 
 
 def lovasz_softmax_flat(probas, labels, classes="present"):
@@ -57,39 +56,7 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
     target outside [0, C): NaN, in logprob and (where logprob takes part in the loss) in the row's gradient.  Logits of -inf are
     classes without probability; a row of nothing else has logprob -inf, entropy 0 and gradient 0 but for the given class's own.
     The gradient has the logits' type, its rows 16-byte aligned (their stride padded where C is odd)."""
-    if logits.dtype not in ops.LOGIT_DTYPES:
-        raise TypeError("token_logprobs: logits are %s; fp32, bf16 or fp16 is wanted" % logits.dtype)
-    if target.dtype is not torch.int64 and target.dtype is not torch.int32:
-        raise TypeError("token_logprobs: target is %s; int64 or int32 is wanted" % target.dtype)
-    if logits.dim() == 0 or not 0 < logits.size(-1) < 1 << 30:
-        raise ValueError("token_logprobs: logits of shape %s have no classes, or too many" % (tuple(logits.shape),))
-    shape, c, rows = logits.shape[:-1], logits.size(-1), target.numel()
-    if target.shape != shape:
-        raise ValueError("token_logprobs: logits of shape %s want a target of shape %s, got %s"
-                         % (tuple(logits.shape), tuple(shape), tuple(target.shape)))
-    if not 0 <= top <= min(ops.TOP_MAX, c):
-        raise ValueError("token_logprobs: top=%r; 0 to %d is wanted" % (top, min(ops.TOP_MAX, c)))
-    if rows >= 1 << 31:
-        raise ValueError("token_logprobs: %d rows" % rows)
-    require_gpu(logits, target)
-    if target.get_device() != logits.get_device():
-        raise ValueError("token_logprobs: logits on %s, target on %s" % (logits.device, target.device))
-    flat = logits.dim() == 2
-    x = logits if flat else logits.reshape(rows, c)
-    # (one row: its stride is never used, and torch may report any)
-    if (x.stride(1) != 1 and c > 1) or (rows > 1 and x.stride(0) < c):
-        x = x.contiguous()
-    if not flat or target.dtype is not torch.int64 or not target.is_contiguous():
-        target = target.reshape(-1).to(torch.int64).contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        out = ops.TokenLogProbs.apply(x, target, int(top), int(ignore_index))
-    else:
-        out = ops.logprob_forward(x, target, int(top), int(ignore_index), stats=False)[:4]
-    if flat:
-        return Scores(*out)
-    logprob, entropy, best, index = out
-    return Scores(logprob.view(shape), entropy.view(shape), best.view(*shape, top) if top else None,
-                  index.view(*shape, top) if top else None)
+    return Scores(*binding().token_logprobs(logits, target, top, ignore_index))
 
 
 def seg_loss_kitti(pred, gt, ignore=0, use_lovasz=False, class_weights=None):

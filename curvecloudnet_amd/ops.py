@@ -9,7 +9,7 @@ import threading
 
 import torch
 
-from ._lib import call, lib, on_device, ptr, require_gpu, workspace
+from ._lib import call, lib, ptr, require_gpu, workspace
 
 ACT = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2}
 LEAKY_SLOPE = 0.01  # torch.nn.LeakyReLU default, the only slope the reference uses
@@ -1518,67 +1518,6 @@ class NLLLoss(torch.autograd.Function):
         call("nll_loss_bwd", ptr(logits), _ld(logits), ptr(target), ptr(lse), rows, c, ctx.ignore, ptr(g),
              ptr(totals), ptr(d), _ld(d))
         return d, None, None, None
-
-
-LOGIT_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-TOP_MAX = 64            # alternatives of a row that ccn_logprob_fwd gives at most
-
-
-def logprob_forward(logits, target, top, ignore_index, stats=True):
-    """ccn_logprob_fwd on a (rows, C) matrix whose columns are adjacent: logprob, entropy, top_logprob, top_index (None where
-    ``top`` is 0) and, for the backward pass, the rows' statistics."""
-    rows, c = logits.shape
-    dev = logits.device
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if stats else None
-    best = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
-    index = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
-    if rows:
-        nbytes = lib().ccn_logprob_workspace_bytes(rows, c, top)
-        ws = workspace(nbytes, dev) if nbytes else None
-        with on_device(logits.get_device()):
-            call("logprob_fwd", ptr(logits), LOGIT_DTYPES[logits.dtype], logits.stride(0), ptr(target), rows, c, ignore_index, top,
-                 ptr(logprob), ptr(entropy), ptr(stats), ptr(best), ptr(index), ptr(ws), nbytes)
-    return logprob, entropy, best, index, stats
-
-
-class TokenLogProbs(torch.autograd.Function):
-    """log_softmax(logits)[target], the rows' entropies and the log-probabilities of their best alternatives, with the gradient of
-    all three in one pass over the logits (ccn_logprob_fwd / _bwd; loss.token_logprobs checks the arguments)."""
-
-    @staticmethod
-    def forward(ctx, logits, target, top, ignore_index):
-        ctx.set_materialize_grads(False)
-        logprob, entropy, best, index, stats = logprob_forward(logits, target, top, ignore_index)
-        ctx.save_for_backward(logits, target, index, stats, entropy)
-        ctx.ignore = ignore_index
-        if index is not None:
-            ctx.mark_non_differentiable(index)
-        return logprob, entropy, best, index
-
-    @staticmethod
-    def backward(ctx, *grads):
-        # (with create_graph: a graph behind the gradient that refuses to be differentiated; its bookkeeping costs 5 us)
-        return (_logprob_backward_once if torch.is_grad_enabled() else _logprob_backward)(ctx, *grads)
-
-
-def _logprob_backward(ctx, g_logprob, g_entropy, g_top, _):
-    logits, target, index, stats, entropy = ctx.saved_tensors
-    rows, c = logits.shape
-    d = _rows(rows, c, logits.device) if logits.dtype == torch.float32 else _rows16(rows, c, logits.device, logits.dtype)
-    if rows:
-        top = 0
-        if g_top is not None:
-            top, g_top = g_top.size(1), g_top.contiguous()
-        with on_device(logits.get_device()):
-            call("logprob_bwd", ptr(logits), LOGIT_DTYPES[logits.dtype], logits.stride(0), ptr(target), rows, c, ctx.ignore, top,
-                 ptr(index) if top else None, ptr(stats), ptr(entropy), ptr(g_logprob), 0 if g_logprob is None else g_logprob.stride(0),
-                 ptr(g_entropy), 0 if g_entropy is None else g_entropy.stride(0), ptr(g_top), ptr(d), d.stride(0))
-    return d, None, None, None
-
-
-_logprob_backward_once = torch.autograd.function.once_differentiable(_logprob_backward)
 
 
 # --------------------------------------------------------------------------------------

@@ -6,14 +6,14 @@ The reference has no distributed code at all; this is th
 section 8(e).  BatchNorm statistics stay per rank (a rank's result equals the reference run on
 that rank's sub-batch).  Works with the gloo backend on CPU tensors too (used by the tests).
 """
-import array
 import contextlib
-import ctypes
 import math
 import os
 
 import torch
 import torch.distributed as dist
+
+from ._lib import binding
 
 SLOT_ALIGN = 4          # floats: every parameter's slot in a bucket starts 16-byte aligned (vector / LDS-DMA loads)
 
@@ -239,7 +239,6 @@ class GradientAllReduce:
         return sum(f.numel() * f.element_size() for f, _, _ in self.buckets)
 
 
-_GRAD_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NORM_KINDS = {1.0: 1, 2.0: 2, math.inf: 3}
 
 
@@ -257,67 +256,6 @@ def _bound(max_norm, who):
     return max_norm
 
 
-def _dense(t):
-    """Whether the values of ``t`` fill one run of memory, in whatever order of the dimensions."""
-    want = 1
-    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.size()) if n != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-_POINTER, _NUMEL, _PLACE, _PLAIN = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
-_DTYPE, _GRAD = torch.Tensor.dtype.__get__, torch.Tensor.grad.__get__
-
-
-class _Tensors:
-    """The tables that the norm's entry points read on the host: addresses, sizes and types of tensors of one device.  (map over
-    unbound methods: half of what a comprehension costs, and a network has hundreds of tensors.)"""
-
-    def __init__(self, tensors, who):
-        try:
-            plain = all(map(_PLAIN, tensors))
-            pointers = array.array("q", list(map(_POINTER, tensors)))
-        except RuntimeError:
-            raise TypeError("%s: sparse tensors are not built" % who) from None
-        types = list(map(_DTYPE, tensors))
-        try:
-            codes = [_GRAD_DTYPES[t] for t in set(types)]
-        except KeyError as e:
-            raise TypeError("%s: %s; fp32, bf16 or fp16 is wanted" % (who, e.args[0])) from None
-        if len(codes) > 1 or codes[0]:
-            codes = [_GRAD_DTYPES[t] for t in types]
-        else:
-            codes = None                        # (all fp32: no table)
-        if not plain:
-            for t in tensors:
-                if not t.is_contiguous() and not _dense(t):
-                    raise ValueError("%s: a tensor of strides %s does not fill its memory" % (who, tuple(t.stride())))
-        places = set(map(_PLACE, tensors))
-        if -1 in places:
-            raise RuntimeError("curvecloudnet_amd ops run on the GPU only (got a cpu tensor); there is no CPU path")
-        if len(places) != 1:
-            raise ValueError("%s: tensors on %d devices; one is wanted" % (who, len(places)))
-        self.place = places.pop()
-        self.n = len(tensors)
-        sizes = list(map(_NUMEL, tensors))
-        self.total = sum(sizes)
-        self.pointers, self.lengths = pointers, array.array("q", sizes)
-        self.keep = None if codes is None else array.array("i", codes)
-        self.ptrs, self.sizes = ctypes.c_void_p(pointers.buffer_info()[0]), ctypes.c_void_p(self.lengths.buffer_info()[0])
-        self.codes = None if codes is None else ctypes.c_void_p(self.keep.buffer_info()[0])
-
-
-def _norm_call(entry, tables, *args):
-    from ._lib import call, lib, on_device, ptr
-    with on_device(tables.place):
-        nbytes = lib().ccn_grad_norm_workspace_bytes(tables.n)
-        ws, norm = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), torch.empty((), dtype=torch.float32, device="cuda")
-        call(entry, *args, ptr(ws), nbytes, ptr(norm), work_rows=tables.total)
-    return norm
-
-
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all values of all ``tensors`` (fp32, bf16 or fp16, of one GPU) as ONE vector: an fp32 scalar on the device, summed
     in 64 bits in a fixed order (ccn_grad_norm).  norm_type: 1, 2 or inf.  The gradients of a GradientAllReduce are already reduced
@@ -327,8 +265,7 @@ def grad_norm(tensors, norm_type=2.0):
     if not tensors:
         return torch.zeros(())
     _join_wgrad()
-    t = _Tensors(tensors, "grad_norm")
-    return _norm_call("grad_norm", t, t.ptrs, t.sizes, t.codes, t.n, kind)
+    return binding().grad_norm(tensors, kind)
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -336,20 +273,16 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     in place by min(1, max_norm / (norm + 1e-6)); returns the norm before clipping, an fp32 scalar on the device.  The product is taken in
     32 bits and rounded once to the gradient's type.  A norm that is not finite gives what the formula gives (0 or NaN), or raises with
     ``error_if_nonfinite`` (which waits for the GPU) before anything is scaled.  Gradients that share memory are refused."""
-    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    grads = [g for g in map(_GRAD, parameters) if g is not None]
     kind, max_norm = _norm_kind(norm_type, "clip_grad_norm_"), _bound(max_norm, "clip_grad_norm_")
+    grads = binding().grads_of([parameters] if isinstance(parameters, torch.Tensor) else list(parameters))
     if not grads:
         return torch.zeros(())
     _join_wgrad()
-    t = _Tensors(grads, "clip_grad_norm_")
     if error_if_nonfinite:
-        norm = _norm_call("grad_norm", t, t.ptrs, t.sizes, t.codes, t.n, kind)
-        if not math.isfinite(float(norm)):
-            raise RuntimeError("clip_grad_norm_: the norm of the gradients is %r" % float(norm))
-    norm = _norm_call("grad_clip", t, t.ptrs, t.sizes, t.codes, t.n, kind, max_norm)
-    torch.autograd.graph.increment_version(grads)
-    return norm
+        norm = float(binding().grad_norm(grads, kind))
+        if not math.isfinite(norm):
+            raise RuntimeError("clip_grad_norm_: the norm of the gradients is %r" % norm)
+    return binding().clip_grad_norm(grads, kind, max_norm)
 
 
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, max_norm=None):
@@ -357,38 +290,14 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     ``max_norm``: the gradients' global norm is bounded as by clip_grad_norm_, but each is scaled as it is read (ccn_adam_clip): they keep
     their values, and the read and write of a separate clipping pass are saved.  Returns the norm before clipping (an fp32 scalar on the
     device), or None without ``max_norm``.  ``step``: the 1-based count of this update."""
-    lists = [list(v) for v in (params, grads, exp_avgs, exp_avg_sqs)]
     step, max_norm = int(step), None if max_norm is None else _bound(max_norm, "adam_step_")
     if step < 1:
         raise ValueError("adam_step_: step %d; the first update is step 1" % step)
-    if len(set(map(len, lists))) != 1:
-        raise ValueError("adam_step_: %d parameters, %d gradients, %d and %d moments" % tuple(map(len, lists)))
-    if not lists[0]:
+    lists = [list(v) for v in (params, grads, exp_avgs, exp_avg_sqs)]
+    if not any(lists):
         return None if max_norm is None else torch.zeros(())
-    for v in lists:
-        if any(t.dtype != torch.float32 for t in v):
-            raise TypeError("adam_step_: fp32 tensors are wanted")
-        if [t.numel() for t in v] != [t.numel() for t in lists[0]] or not all(map(torch.Tensor.is_contiguous, v)):
-            raise ValueError("adam_step_: the tensors of a parameter are contiguous and of one size")
-    tables = [_Tensors(v, "adam_step_") for v in lists]
-    for t in tables:
-        if t.place != tables[0].place:
-            raise ValueError("adam_step_: the tensors of a parameter are on one device")
-        if any(p % 16 for p in t.pointers):
-            raise ValueError("adam_step_: a tensor does not start at a multiple of 16 bytes")
-    return _adam(tables, step, lr, betas, eps, weight_decay, max_norm)
-
-
-def _adam(tables, step, lr, betas, eps, weight_decay, max_norm):
-    p, g, m, v = tables
-    rest = (float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay), step)         # (as both entries take them)
     _join_wgrad()
-    if max_norm is not None:
-        return _norm_call("adam_clip", g, p.ptrs, g.ptrs, m.ptrs, v.ptrs, g.sizes, g.n, *rest, max_norm)
-    from ._lib import call, on_device
-    with on_device(g.place):
-        for at in zip(*(t.pointers for t in tables), g.lengths):
-            call("adam_step", *map(ctypes.c_void_p, at[:4]), at[4], *rest)
+    return binding().adam_step(*lists, step, lr, *betas, eps, weight_decay, max_norm)
 
 
 class FlatAdam(torch.optim.Optimizer):

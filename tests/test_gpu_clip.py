@@ -389,12 +389,12 @@ def test_a_run_of_all_of_them():
         ref = (-(logp.gather(1, y[:, None]).squeeze(1) * (y != 0)).sum() / (y != 0).sum() + 0.01 * (logp.exp() * logp).sum(1).mean()
                + 0.001 * logp.gather(1, r.top_index).mean())
         (d,) = torch.autograd.grad(ref, z)
-        assert abs(float(ref) - float(loss)) <= 400 * U * 4
+        assert abs(float(ref.detach()) - float(loss.detach())) <= 400 * U * 4
         bias = mlp.lins[-1].bias.grad.double()
         assert float((bias - d.sum(0)).abs().max()) <= 3000 * U * float(d.abs().sum(0).max())
         opt.step()
         assert abs(float(opt.grad_norm) - want) <= 2 * U * want
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
     assert all(math.isfinite(v) for v in losses)
     sync.zero_grad()
     token_logprobs(mlp(x), y).logprob.mean().backward()

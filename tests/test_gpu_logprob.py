@@ -448,3 +448,62 @@ def test_rows_beside_the_outputs_stay():
              None, 0, None, ptr(d[1:]), d.stride(0))
         assert bool((d[0] == 7).all()) and bool((d[-1] == 7).all()) and bool((d[:, c:] == 7).all())
         assert bool((d[1:-1, :c] != 7).all())
+
+
+def test_launches_are_observed(monkeypatch):
+    """The timing of launches (bench.py's) sees these operators, the backward pass on autograd's thread among them; results stay."""
+    from curvecloudnet_amd import _lib, costs
+    from curvecloudnet_amd.parallel import grad_norm
+    x, t = _logits(40, 5000, torch.float32).requires_grad_(True), _target(40, 5000)
+
+    def step():
+        r = _score(x, t, top=3)
+        (d,) = torch.autograd.grad([r.logprob, r.top_logprob], x, [torch.ones_like(r.logprob), torch.ones_like(r.top_logprob)])
+        return [v.detach() for v in (*r, d, grad_norm([d]))]
+
+    want = step()
+    monkeypatch.setattr(_lib, "PROFILE", [])
+    got = step()
+    torch.cuda.synchronize()
+    records = _lib.PROFILE
+    monkeypatch.setattr(_lib, "PROFILE", None)
+    assert [r[0] for r in records] == ["logprob_fwd", "logprob_bwd", "grad_norm"]
+    assert all(r[2].elapsed_time(r[3]) > 0 for r in records)
+    for name, ints, _, _, _, work in records:
+        family, _, nbytes, modelled = costs.entry_cost(name, ints, work)
+        assert family == "loss_optim" and modelled and nbytes >= 40 * 5000 * 4
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def test_gradient_is_not_differentiated_again():
+    x, t = _logits(4, 30, torch.float32).requires_grad_(True), _target(4, 30)
+    w = torch.ones((), device=DEV, requires_grad=True)
+    (d,) = torch.autograd.grad((_score(x, t).logprob * w).sum(), x, create_graph=True)
+    (ref,) = torch.autograd.grad(_score(x, t).logprob.sum(), x)
+    assert torch.equal(d.detach(), ref)
+    with pytest.raises(RuntimeError):                                  # (no way from the gradient back to the logits)
+        torch.autograd.grad(d.sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        d.sum().backward()
+
+
+def test_other_kinds_of_tensors():
+    x, t = _logits(6, 40, torch.float32), _target(6, 40)
+    want = _score(x, t, top=2)
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(_score(x.clone(), t.clone(), top=2), want))
+    z = torch.complex(torch.zeros_like(x), -x)
+    assert z.conj().imag.is_neg() and all(torch.equal(a, b) for a, b in zip(_score(z.conj().imag, t, top=2), want))
+    leaf = x.clone().requires_grad_(True)
+    r = _score(leaf, t)
+    r.entropy.sum().backward()
+    a = leaf.grad.clone()
+    r = _score(leaf, t)
+    r.entropy.sum().backward()
+    assert torch.equal(leaf.grad, 2 * a)                                # (accumulated as any gradient is)
+    r = _score(leaf, t)
+    with torch.no_grad():
+        leaf.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.logprob.sum().backward()
