@@ -71,8 +71,7 @@ __device__ __forceinline__ double clip_join(double a, double b) {
 
 template <int KIND>
 __device__ __forceinline__ double clip_block(double v, double* red) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = clip_join<KIND>(v, __shfl_xor(v, d, 64));
+  v = ccn_wave_join(v, [](double a, double b) { return clip_join<KIND>(a, b); });
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = red[0];

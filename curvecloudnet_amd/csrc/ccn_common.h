@@ -167,3 +167,48 @@ template <int T>
 __device__ __forceinline__ void st16(void* p, int64_t i, const ccn_u32x4& r) {
   *reinterpret_cast<typename CcnVec16<T>::mem*>(reinterpret_cast<char*>(p) + i * (T == 0 ? 4 : 2)) = r;
 }
+
+// ---- the value of lane (lane ^ D), by data-parallel moves instead of the LDS crossbar (4 to 16 cycles instead of about 100); every lane
+// of the wave has to be active
+template <int D>
+__device__ __forceinline__ uint32_t ccn_lane_xor(uint32_t v) {
+  static_assert(D == 1 || D == 2 || D == 4 || D == 8 || D == 16 || D == 32, "a power of two below 64");
+  if constexpr (D == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);         // quad_perm [1,0,3,2]
+  else if constexpr (D == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);    // quad_perm [2,3,0,1]
+  else if constexpr (D == 4)                                                                    // ^ 7 by row_half_mirror, then ^ 3
+    return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true), 0x1B, 0xf, 0xf, true);
+  else if constexpr (D == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, true);   // row_ror:8
+  else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return (threadIdx.x & 16) ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (threadIdx.x & 32) ? r[0] : r[1];
+  }
+}
+template <int D>
+__device__ __forceinline__ float ccn_lane_xor(float v) {
+  return __builtin_bit_cast(float, ccn_lane_xor<D>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int D>
+__device__ __forceinline__ uint64_t ccn_lane_xor(uint64_t v) {
+  return ((uint64_t)ccn_lane_xor<D>((uint32_t)(v >> 32)) << 32) | ccn_lane_xor<D>((uint32_t)v);
+}
+template <int D>
+__device__ __forceinline__ double ccn_lane_xor(double v) {
+  return __builtin_bit_cast(double, ccn_lane_xor<D>(__builtin_bit_cast(uint64_t, v)));
+}
+// v of all 64 lanes joined by f, in the same order in every lane's tree
+template <typename V, typename F>
+__device__ __forceinline__ V ccn_wave_join(V v, F f) {
+  v = f(v, ccn_lane_xor<1>(v));
+  v = f(v, ccn_lane_xor<2>(v));
+  v = f(v, ccn_lane_xor<4>(v));
+  v = f(v, ccn_lane_xor<8>(v));
+  v = f(v, ccn_lane_xor<16>(v));
+  return f(v, ccn_lane_xor<32>(v));
+}
+template <typename V>
+__device__ __forceinline__ V ccn_wave_sum(V v) {
+  return ccn_wave_join(v, [](V a, V b) { return a + b; });
+}

@@ -96,49 +96,42 @@ __device__ __forceinline__ void lp_forget(ccn_u32x4 (&raw)[N]) {
 
 // ---- sorted lists of 64 keys, one to a lane, descending
 
-__device__ __forceinline__ uint64_t lp_shfl_xor(uint64_t v, int d) { return __shfl_xor((unsigned long long)v, d, 64); }
-
-__device__ __forceinline__ uint64_t lp_sort64(uint64_t v) {
+// One step of a bitonic sort: lanes D apart, in runs of SIZE of alternating direction (SIZE 64: descending throughout).
+template <int SIZE, int D, typename K>
+__device__ __forceinline__ K lp_step(K v) {
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int d = size >> 1; d >= 1; d >>= 1) {
-      const uint64_t o = lp_shfl_xor(v, d);
-      const bool larger = ((lane & size) == 0) == ((lane & d) == 0);
-      v = (o > v) == larger ? o : v;
-    }
-  return v;
+  const K o = ccn_lane_xor<D>(v);
+  const bool larger = ((lane & SIZE) == 0) == ((lane & D) == 0);
+  return (o > v) == larger ? o : v;
+}
+template <int SIZE, typename K>
+__device__ __forceinline__ K lp_steps(K v) {
+  if constexpr (SIZE >= 64) v = lp_step<SIZE, 32>(v);
+  if constexpr (SIZE >= 32) v = lp_step<SIZE, 16>(v);
+  if constexpr (SIZE >= 16) v = lp_step<SIZE, 8>(v);
+  if constexpr (SIZE >= 8) v = lp_step<SIZE, 4>(v);
+  if constexpr (SIZE >= 4) v = lp_step<SIZE, 2>(v);
+  return lp_step<SIZE, 1>(v);
+}
+template <typename K>
+__device__ __forceinline__ K lp_sort64(K v) {
+  v = lp_steps<2>(v);
+  v = lp_steps<4>(v);
+  v = lp_steps<8>(v);
+  v = lp_steps<16>(v);
+  v = lp_steps<32>(v);
+  return lp_steps<64>(v);
 }
 // The 64 largest of two lists: the larger of each pair (i, 63 - i) are they, and fall and rise; six steps put them in order.
 __device__ __forceinline__ uint64_t lp_merge64(uint64_t a, uint64_t b) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t o = __shfl((unsigned long long)b, 63 - lane, 64);
-  uint64_t v = a > o ? a : o;
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    const uint64_t p = lp_shfl_xor(v, d);
-    v = (p > v) == ((lane & d) == 0) ? p : v;
-  }
-  return v;
+  const uint64_t o = __shfl((unsigned long long)b, 63 - (int)(threadIdx.x & 63), 64);
+  return lp_steps<64>(a > o ? a : o);
 }
 // Lane k - 1 of the lane values in descending order (NaN first), as a value.
 __device__ __forceinline__ float lp_kth_lane(float m, int k) {
-  const int lane = threadIdx.x & 63;
-  int v = __float_as_int(m + 0.0f);
-  if (m != m) v = 0x7f800001;
-  v ^= (v >> 31) & 0x7fffffff;
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int d = size >> 1; d >= 1; d >>= 1) {
-      const int o = __shfl_xor(v, d, 64);
-      const bool larger = ((lane & size) == 0) == ((lane & d) == 0);
-      v = larger ? max(v, o) : min(v, o);
-    }
-  v = __shfl(v, k - 1, 64);
-  v ^= (v >> 31) & 0x7fffffff;
-  return __int_as_float(v);
+  uint32_t v = (uint32_t)(lp_key(m, 0) >> 32);
+  v = lp_sort64(v);
+  return lp_key_value((uint64_t)(uint32_t)__builtin_amdgcn_readlane(v, k - 1) << 32);
 }
 
 // ---- rows of more than 64 classes: NW waves hold NW * 2048 logits of a row at a time in registers (32 a thread), take their maximum,
@@ -208,6 +201,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
 
   float m = -INFINITY, s = 0.f, w = 0.f;
   uint64_t best = 0;                                 // (wave 0's list)
+  bool fresh = true;
   if (TOP) {
     if (tid == 0) sh.count = 0;
     lp_sync<NW>();
@@ -282,7 +276,11 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
           lp_sync<NW>();
           if (wave == 0) {
             const int got = min(sh.count, LpShared<NW>::ROOM);
-            for (int b = 0; b < got; b += 64) best = lp_merge64(best, lp_sort64(b + lane < got ? sh.cand[b + lane] : 0));
+            for (int b = 0; b < got; b += 64) {
+              const uint64_t k = lp_sort64(b + lane < got ? sh.cand[b + lane] : 0);
+              best = fresh ? k : lp_merge64(best, k);
+              fresh = false;
+            }
             const uint64_t k = __shfl((unsigned long long)best, top - 1, 64);
             if (lane == 0) {
               sh.last_key = k;
@@ -301,8 +299,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
   }
   // the threads' statistics joined
   float all = m;
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) all = lp_max(all, __shfl_xor(all, d, 64));
+  all = ccn_wave_join(all, lp_max);
   if (NW > 1) {
     if (lane == 0) sh.red[0][wave] = all;
     __syncthreads();
@@ -313,11 +310,8 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
   const float dm = lp_diff(m, all), f = lp_exp(dm);
   w = f * (w + dm * s);
   s *= f;
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    s += __shfl_xor(s, d, 64);
-    w += __shfl_xor(w, d, 64);
-  }
+  s = ccn_wave_sum(s);
+  w = ccn_wave_sum(w);
   if (NW > 1) {
     if (lane == 0) {
       sh.red[0][wave] = s;
@@ -374,8 +368,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_join_kernel(const void* __rest
   for (int k = 1; top && k < 4; ++k) best = lp_merge64(best, lists[k][lane]);
   float all = -INFINITY;
   for (int p = lane; p < parts; p += 64) all = lp_max(all, part_stats[row * parts + p].x);
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) all = lp_max(all, __shfl_xor(all, d, 64));
+  all = ccn_wave_join(all, lp_max);
   float s = 0.f, w = 0.f;
   for (int p = lane; p < parts; p += 64) {
     const float4 q = part_stats[row * parts + p];
@@ -383,11 +376,8 @@ __global__ __launch_bounds__(LP_TPB) void logprob_join_kernel(const void* __rest
     s += f * q.y;
     w += f * (q.z + d * q.y);
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    s += __shfl_xor(s, d, 64);
-    w += __shfl_xor(w, d, 64);
-  }
+  s = ccn_wave_sum(s);
+  w = ccn_wave_sum(w);
   const LpRow r = lp_finish(all, s, w);
   if (lane == 0) {
     logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
