@@ -390,82 +390,112 @@ __global__ __launch_bounds__(LP_TPB) void logprob_join_kernel(const void* __rest
   }
 }
 
-// ---- rows of up to 64 classes: 128 rows go through shared memory (wide loads of one run of memory where the rows are adjacent) and
-// every thread walks its own row there; an odd pitch keeps the walks on different banks.  Alternatives: `top` walks, each of which
-// takes the largest value that is left (strictly larger ones replace: the lowest of equal classes wins).
+// ---- rows of up to 64 classes: 128 / TEAM rows go through shared memory (16-byte loads) and TEAM threads walk each of them there,
+// every TEAM-th class one, their results joined by lane moves.  The pitch puts the lanes of a wave on different banks.  More than one
+// thread to a long row, or shared memory has room for too few waves (us with one / two / four: 400070 x 20 10.7 / 12.0 / 13.7,
+// 300000 x 32 14.8 / 12.9 / 12.6, 300000 x 40 20.2 / 15.7 / 15.8, 220011 x 55 28.4 / 19.1 / 15.8).
+// Alternatives: `top` walks, each of which takes the largest value that is left (of equal ones the lowest class); 16 values in
+// registers instead of shared memory take as long.  Many of them leave through shared memory: a thread's own are `top` values wide,
+// 64 such stores side by side cost more than the walks (400070 x 20: 3 of them 17.6 us without the detour and 20.1 with it, 5 23.2
+// and 23.5, 8 36.6 and 29.6; 500000 x 8: 5 of them 20.4 and 14.3).
 constexpr int LP_NARROW = 64;
-constexpr int LP_NARROW_ROWS = 128;
+constexpr int LP_NARROW_TPB = 128;
+constexpr int LP_TEAM1 = 24, LP_TEAM2 = 40;          // classes up to which one, two threads walk a row
+constexpr int LP_DIRECT_TOP = 4;                     // alternatives that are stored as they are found
 
-template <int T, bool TOP>
-__global__ __launch_bounds__(LP_NARROW_ROWS) void logprob_narrow_kernel(const void* __restrict__ x, int64_t ld,
-                                                                        const int64_t* __restrict__ target, int64_t rows, int C,
-                                                                        uint32_t magic, int64_t ignore, int top,
-                                                                        float* __restrict__ logprob, float* __restrict__ entropy,
-                                                                        float2* __restrict__ stats,
-                                                                        float* __restrict__ top_logprob,
-                                                                        int64_t* __restrict__ top_index) {
+template <int TEAM, typename V, typename F>
+__device__ __forceinline__ V lp_team(V v, F f) {
+  if constexpr (TEAM >= 2) v = f(v, ccn_lane_xor<1>(v));
+  if constexpr (TEAM >= 4) v = f(v, ccn_lane_xor<2>(v));
+  return v;
+}
+
+template <int T, int TEAM, bool TOP>
+__global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const void* __restrict__ x, int64_t ld,
+                                                                       const int64_t* __restrict__ target, int64_t rows, int C,
+                                                                       int pitch, int vecs, uint32_t magic, int64_t ignore, int top,
+                                                                       float* __restrict__ logprob, float* __restrict__ entropy,
+                                                                       float2* __restrict__ stats,
+                                                                       float* __restrict__ top_logprob,
+                                                                       int64_t* __restrict__ top_index) {
   extern __shared__ float tile[];
-  constexpr int V = CcnVec16<T>::N;
-  const int P = C | 1;
-  const int64_t r0 = (int64_t)blockIdx.x * LP_NARROW_ROWS;
-  const int live = (int)min((int64_t)LP_NARROW_ROWS, rows - r0), n = live * C;
-  // (i / C as a product: exact for i < 2^16 and 1 < C <= 64, the error of magic is below 2^-16)
-  auto row_of = [&](int i) { return C == 1 ? i : (int)__umulhi((uint32_t)i, magic); };
-  if (ld == C) {
-    for (int i = threadIdx.x * V; i < n; i += LP_NARROW_ROWS * V) {
-      const ccn_u32x4 raw = lp_load_part<T>(x, r0 * C + i, n - i);
-      int r = row_of(i), c = i - r * C;
+  constexpr int V = CcnVec16<T>::N, ROWS = LP_NARROW_TPB / TEAM;
+  const int64_t r0 = (int64_t)blockIdx.x * ROWS;
+  const int live = (int)min((int64_t)ROWS, rows - r0);
+  // 16-byte pieces, `vecs` to a row (i / vecs as a product: exact for i < 2^16, the error of magic is below 2^-16)
+  const int n = live * vecs;
+  for (int i = threadIdx.x; i < n; i += LP_NARROW_TPB) {
+    const int q = vecs == 1 ? i : (int)__umulhi((uint32_t)i, magic), c = (i - q * vecs) * V;
+    const ccn_u32x4 raw = lp_load_part<T>(x, (r0 + q) * ld + c, C - c);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (i + k < n) tile[r * P + c] = get16<T>(raw, k);
-        if (++c == C) {
-          c = 0;
-          ++r;
-        }
-      }
-    }
-  } else {
-    for (int i = threadIdx.x; i < n; i += LP_NARROW_ROWS) {
-      const int r = row_of(i), c = i - r * C;
-      tile[r * P + c] = ld_el<T>(x, (r0 + r) * ld + c);
-    }
+    for (int k = 0; k < V; ++k)
+      if (c + k < C) tile[q * pitch + c + k] = get16<T>(raw, k);
   }
   __syncthreads();
-  if (threadIdx.x >= live) return;
-  float* const mine = tile + threadIdx.x * P;
-  const int64_t row = r0 + threadIdx.x, t = target[row];
+  const int lane = threadIdx.x % TEAM, mine_row = min((int)threadIdx.x / TEAM, live - 1);       // (all lanes stay for the joins)
+  const bool writes = (int)threadIdx.x / TEAM < live && lane == 0;
+  float* const mine = tile + mine_row * pitch;
+  const int64_t row = r0 + mine_row, t = target[row];
   float m = -INFINITY;
-  for (int c = 0; c < C; ++c) m = lp_max(m, mine[c]);
-  float s = 0.f, w = 0.f;
+#pragma unroll 4
+  for (int c = lane; c < C; c += TEAM) m = lp_max(m, mine[c]);
+  m = lp_team<TEAM>(m, lp_max);
   const float given = t >= 0 && t < C ? mine[t] : 0.f;
-  for (int c = 0; c < C; ++c) {
+  float s = 0.f, w = 0.f;
+#pragma unroll 4
+  for (int c = lane; c < C; c += TEAM) {
     const float v = mine[c], d = lp_diff(v, m), e = lp_exp(d);
     s += e;
     w = __builtin_fmaf(e, d, w);
-    if (TOP) {                                       // as a whole number in the order of the alternatives
-      int o = __float_as_int(v + 0.0f);
-      if (v != v) o = 0x7f800001;
-      mine[c] = __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
-    }
   }
+  s = lp_team<TEAM>(s, [](float a, float b) { return a + b; });
+  w = lp_team<TEAM>(w, [](float a, float b) { return a + b; });
   const LpRow r = lp_finish(m, s, w);
-  logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
-  entropy[row] = r.entropy;
-  if (stats) stats[row] = make_float2(r.base, r.log_total);
-  if (TOP) {
-    int* const order = reinterpret_cast<int*>(mine);
-    for (int j = 0; j < top; ++j) {
-      int v = INT_MIN, at = 0;                       // (below every value; taken ones become it)
-      for (int c = 0; c < C; ++c) {
-        const int o = order[c];
-        at = o > v ? c : at;
-        v = max(v, o);
-      }
-      order[at] = INT_MIN;
-      const float f = __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
+  if (writes) {
+    logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
+    entropy[row] = r.entropy;
+    if (stats) stats[row] = make_float2(r.base, r.log_total);
+  }
+  if (!TOP) return;
+  // (the given class's logit has been read by every thread of its wave, and a row's threads are of one wave)
+  int* const order = reinterpret_cast<int*>(mine);
+  float* const out = tile + ROWS * pitch;
+  int* const out_class = reinterpret_cast<int*>(out + ROWS * top);
+  const bool own = (int)threadIdx.x / TEAM < live;
+  for (int c = lane; c < C && own; c += TEAM) {      // as whole numbers in the order of the alternatives
+    const float v = mine[c];
+    int o = __float_as_int(v + 0.0f);
+    if (v != v) o = 0x7f800001;
+    order[c] = o ^ ((o >> 31) & 0x7fffffff);
+  }
+  for (int j = 0; j < top; ++j) {
+    int v = INT_MIN, at = 0;                         // (below every value; taken ones become it)
+#pragma unroll 4
+    for (int c = lane; c < C; c += TEAM) {
+      const int o = order[c];
+      at = o > v ? c : at;
+      v = max(v, o);
+    }
+    // (value, then lower class, as one number)
+    const uint64_t k = lp_team<TEAM>(((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (uint32_t)~at,
+                                     [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    at = (int)(uint32_t)~(uint32_t)k;
+    v = (int)((uint32_t)(k >> 32) ^ 0x80000000u);
+    if (own && at % TEAM == lane) order[at] = INT_MIN;
+    const float f = __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
+    if (writes && top <= LP_DIRECT_TOP) {
       top_logprob[row * top + j] = (f - r.base) - r.log_total;
       top_index[row * top + j] = at;
+    } else if (writes) {
+      out[mine_row * top + j] = (f - r.base) - r.log_total;
+      out_class[mine_row * top + j] = at;
     }
+  }
+  if (top <= LP_DIRECT_TOP) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < live * top; i += LP_NARROW_TPB) {
+    top_logprob[r0 * top + i] = out[i];
+    top_index[r0 * top + i] = out_class[i];
   }
 }
 
@@ -643,21 +673,31 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
   CCN_REQUIRE(top == 0 || (top_logprob && top_index), "logprob_fwd: top > 0 without its outputs");
   hipStream_t s = (hipStream_t)stream;
   if (C <= LP_NARROW) {
-    const dim3 grid((unsigned)((rows + LP_NARROW_ROWS - 1) / LP_NARROW_ROWS)), block(LP_NARROW_ROWS);
-    const size_t lds = (size_t)LP_NARROW_ROWS * (C | 1) * sizeof(float);
-    const uint32_t magic = C == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + C - 1) / C);
-#define CCN_LP_NARROW(T, TOP)                                                                                                     \
-  hipLaunchKernelGGL((logprob_narrow_kernel<T, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, magic, ignore_index,  \
-                     top, logprob, entropy, (float2*)stats, top_logprob, top_index)
+    const int team = C <= LP_TEAM1 ? 1 : C <= LP_TEAM2 ? 2 : 4, per = dtype == 0 ? 4 : 8;
+    const int vecs = (int)((C + per - 1) / per), n = LP_NARROW_TPB / team;
+    const int pitch = team == 1 ? (int)C | 1 : (int)((C + team - 1) / (2 * team) * 2 * team + team);     // team modulo 2 team
+    const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
+    const dim3 grid((unsigned)((rows + n - 1) / n)), block(LP_NARROW_TPB);
+    const size_t lds = (size_t)n * (pitch + (top > LP_DIRECT_TOP ? 2 * top : 0)) * sizeof(float);
+#define CCN_LP_NARROW(T, TEAM, TOP)                                                                                               \
+  hipLaunchKernelGGL((logprob_narrow_kernel<T, TEAM, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, pitch, vecs,    \
+                     magic, ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index)
+#define CCN_LP_TEAM(T, TOP)                                                                                                       \
+  do {                                                                                                                            \
+    if (team == 1) CCN_LP_NARROW(T, 1, TOP);                                                                                      \
+    else if (team == 2) CCN_LP_NARROW(T, 2, TOP);                                                                                 \
+    else CCN_LP_NARROW(T, 4, TOP);                                                                                                \
+  } while (0)
     if (top) {
-      if (dtype == 0) CCN_LP_NARROW(0, true);
-      else if (dtype == 1) CCN_LP_NARROW(1, true);
-      else CCN_LP_NARROW(2, true);
+      if (dtype == 0) CCN_LP_TEAM(0, true);
+      else if (dtype == 1) CCN_LP_TEAM(1, true);
+      else CCN_LP_TEAM(2, true);
     } else {
-      if (dtype == 0) CCN_LP_NARROW(0, false);
-      else if (dtype == 1) CCN_LP_NARROW(1, false);
-      else CCN_LP_NARROW(2, false);
+      if (dtype == 0) CCN_LP_TEAM(0, false);
+      else if (dtype == 1) CCN_LP_TEAM(1, false);
+      else CCN_LP_TEAM(2, false);
     }
+#undef CCN_LP_TEAM
 #undef CCN_LP_NARROW
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
