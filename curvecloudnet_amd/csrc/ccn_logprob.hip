@@ -19,6 +19,7 @@ namespace {
 
 constexpr int LP_TPB = 256;
 constexpr int LP_TOP_MAX = 64;
+
 constexpr float LP_LOG2E = 1.44269504088896340736f;
 constexpr float LP_FAR = -1000.f;           // differences below it weigh nothing; -inf, and -inf - -inf, become it
 
@@ -87,13 +88,6 @@ __device__ __forceinline__ ccn_u32x4 lp_load_part(const void* __restrict__ x, in
   return r;
 }
 
-// (what was computed from the values is computed again where it is rarely needed, and not kept in registers until then)
-template <int N>
-__device__ __forceinline__ void lp_forget(ccn_u32x4 (&raw)[N]) {
-#pragma unroll
-  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(raw[j]));
-}
-
 // ---- sorted lists of 64 keys, one to a lane, descending
 
 // One step of a bitonic sort: lanes D apart, in runs of SIZE of alternating direction (SIZE 64: descending throughout).
@@ -127,30 +121,28 @@ __device__ __forceinline__ uint64_t lp_merge64(uint64_t a, uint64_t b) {
   const uint64_t o = __shfl((unsigned long long)b, 63 - (int)(threadIdx.x & 63), 64);
   return lp_steps<64>(a > o ? a : o);
 }
-// Lane k - 1 of the lane values in descending order (NaN first), as a value.
-__device__ __forceinline__ float lp_kth_lane(float m, int k) {
-  uint32_t v = (uint32_t)(lp_key(m, 0) >> 32);
-  v = lp_sort64(v);
-  return lp_key_value((uint64_t)(uint32_t)__builtin_amdgcn_readlane(v, k - 1) << 32);
-}
+// Lane k - 1 of the lane values in descending order (NaN first).
+__device__ __forceinline__ uint32_t lp_kth_lane(uint32_t sorted, int k) { return (uint32_t)__builtin_amdgcn_readlane(sorted, k - 1); }
 
 // ---- rows of more than 64 classes: NW waves hold NW * 2048 logits of a row at a time in registers (32 a thread), take their maximum,
 // and add weights relative to the maximum so far: one pass over the row, one rescaling per 32 logits of a thread.
 //
-// Alternatives: among the first logits held, the top-th largest of a wave's 64 thread maxima is a lower bound of the top-th largest of
-// them all, and hardly more than `top` reach it.  They are put into shared memory, and wave 0 sorts them (64 at a time, merged into the
-// best so far).  From then on a thread looks at its logits again only if its maximum beats the last of the best: a row of random
-// logits costs a sort at its start and hardly anything later.  Where more qualify than there is room for (equal logits, rising rows), the
-// rest is looked at again after each merge, against the new last of the best: every turn settles LP_ROOM of them at least.
+// Alternatives: the threads' maxima give a lower bound of the top-th largest of the first logits held that few others reach
+// (lp_limit).  Those that do wait in shared memory, and so do later ones that beat the bound, about `top` of 8192 random logits.  Wave 0
+// puts them in order when another `top` would make them more than 64, and at the end; the last of the best is the new bound.  Where
+// more qualify than there is room for (equal logits, rising rows), the rest is looked at again after an ordering, against the new bound;
+// every turn settles LpShared::ROOM of them.
 constexpr int LP_HOLD = 32;
 
 template <int NW>
 struct LpShared {
   static constexpr int ROOM = NW == 4 ? 1024 : 256;
-  uint64_t cand[ROOM];
-  uint64_t last_key;
+  uint64_t cand[ROOM];                      // waiting
+  uint64_t best[64];                        // in order, descending
+  uint64_t last_key;                        // the top-th of them, 0 where there are fewer
   float last;
-  int count, any;
+  int count[3];                             // those that came with this tile, the last one, the one before
+  uint32_t limit[2][NW];
   float red[2][NW];
 };
 
@@ -163,10 +155,84 @@ __device__ __forceinline__ void lp_sync() {
     __syncthreads();
   }
 }
+
+// A value that at least `top` of the logits held reach, from the threads' maxima m.
+//   up to 16: the least of the maxima of 2^g >= top groups of threads (about top log top logits reach it: one ordering of 64)
+//   more: of every wave's 64 maxima in order, the larger of: the top-th of one wave; the (top / NW)-th, the least over the waves
+// (us, 1000 x 10000 fp32: PLACEHOLDER)
 template <int NW>
-__device__ __forceinline__ bool lp_any(bool v) {
-  if (NW == 1) return __builtin_amdgcn_ballot_w64(v) != 0;
-  return __syncthreads_or(v) != 0;
+__device__ __forceinline__ float lp_limit(float m, int top, LpShared<NW>& sh) {
+  const int lane = threadIdx.x & 63, wave = NW == 4 ? threadIdx.x >> 6 : 0;
+  uint32_t v = (uint32_t)(lp_key(m, 0) >> 32);
+  uint32_t bound;
+  if (top <= 16) {
+    const int groups = NW == 4 ? (top + 3) / 4 : top;        // ... of a wave, 1 to 16
+    auto more = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    auto less = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
+    // (groups of lanes that are equal in their last bits: a short row fills the first lanes)
+    v = more(v, ccn_lane_xor<32>(v));
+    v = more(v, ccn_lane_xor<16>(v));
+    const uint32_t v8 = ccn_lane_xor<8>(v);
+    v = groups > 8 ? less(v, v8) : more(v, v8);
+    const uint32_t v4 = ccn_lane_xor<4>(v);
+    v = groups > 4 ? less(v, v4) : more(v, v4);
+    const uint32_t v2 = ccn_lane_xor<2>(v);
+    v = groups > 2 ? less(v, v2) : more(v, v2);
+    const uint32_t v1 = ccn_lane_xor<1>(v);
+    bound = groups > 1 ? less(v, v1) : more(v, v1);
+    if (NW > 1) {
+      if (lane == 0) sh.limit[0][wave] = bound;
+      lp_sync<NW>();
+      bound = sh.limit[0][0];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) bound = top > 1 ? less(bound, sh.limit[0][k]) : more(bound, sh.limit[0][k]);
+    }
+  } else {
+    v = lp_sort64(v);
+    bound = lp_kth_lane(v, top);
+    if (NW > 1) {
+      const uint32_t share = lp_kth_lane(v, (top + NW - 1) / NW);
+      if (lane == 0) {
+        sh.limit[0][wave] = bound;
+        sh.limit[1][wave] = share;
+      }
+      lp_sync<NW>();
+      uint32_t all = sh.limit[1][0];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) all = min(all, sh.limit[1][k]);
+      bound = all;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) bound = max(bound, sh.limit[0][k]);
+    }
+  }
+  return lp_key_value((uint64_t)bound << 32);
+}
+
+// Wave 0: the `got` that wait put among the `have` best.  64 in all: every key counts those above it, which is its place; more: sorted 64
+// at a time and merged.
+template <int NW>
+__device__ __forceinline__ void lp_order(LpShared<NW>& sh, int top, int have, int got) {
+  const int lane = threadIdx.x & 63;
+  if (have + got <= 64) {
+    const uint64_t k = lane < have ? sh.best[lane] : lane < have + got ? sh.cand[lane - have] : 0;
+    int place = 0;
+#pragma unroll 4
+    for (int i = 0; i < have; ++i) place += sh.best[i] > k;
+#pragma unroll 4
+    for (int i = 0; i < got; ++i) place += sh.cand[i] > k;
+    lp_sync<1>();
+    if (lane < have + got && place < top) sh.best[place] = k;
+  } else {
+    uint64_t best = lane < have ? sh.best[lane] : 0;
+    for (int b = 0; b < got; b += 64) best = lp_merge64(best, lp_sort64(b + lane < got ? sh.cand[b + lane] : 0));
+    sh.best[lane] = best;
+  }
+  lp_sync<1>();
+  if (lane == 0) {
+    const uint64_t last = have + got >= top ? sh.best[top - 1] : 0;
+    sh.last_key = last;
+    sh.last = last ? lp_key_value(last) : -INFINITY;
+  }
 }
 
 // The class of the e-th logit that a thread holds.
@@ -177,9 +243,9 @@ __device__ __forceinline__ int lp_class(int c0, int tid, int e) {
 }
 
 template <int T, int NW, bool TOP>
-__global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
+__global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 ? 5 : 6) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
                                                               const int64_t* __restrict__ target, int64_t rows, int C,
-                                                              int64_t ignore, int top, int parts, int part_tiles,
+                                                              int64_t ignore, int top, int parts, int part_len,
                                                               float* __restrict__ logprob, float* __restrict__ entropy,
                                                               float2* __restrict__ stats, float* __restrict__ top_logprob,
                                                               int64_t* __restrict__ top_index, float4* __restrict__ part_stats,
@@ -193,17 +259,17 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
   const int part = NW == 4 ? (int)(blockIdx.x % (unsigned)parts) : 0;
   if (NW == 1 && row >= rows) return;                // (a whole wave, and no barrier of the workgroup below)
   const int64_t at = row * ld;
-  const int beg = part * part_tiles * TILE, end = (int)min((int64_t)C, (int64_t)beg + (int64_t)part_tiles * TILE);
+  const int beg = part * part_len, end = min(C, beg + part_len);
   // the given class's logit, early: its latency passes beside the row
   const int64_t t = target[row];
   float given = 0.f;
   if (parts == 1 && t >= 0 && t < C) given = ld_el<T>(x, at + t);
 
   float m = -INFINITY, s = 0.f, w = 0.f;
-  uint64_t best = 0;                                 // (wave 0's list)
-  bool fresh = true;
+  int turn = 0, have = 0, waiting = 0;               // (the same in every thread)
+  float limit = -INFINITY;
   if (TOP) {
-    if (tid == 0) sh.count = 0;
+    if (tid < 3) sh.count[tid] = 0;
     lp_sync<NW>();
   }
   for (int c0 = beg; c0 < end; c0 += TILE) {
@@ -216,13 +282,16 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
 #pragma unroll
       for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, at + c0 + (j * NT + tid) * V, n - (j * NT + tid) * V);
     }
-    float tm = -INFINITY;
+    float tm = -INFINITY, vm[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NJ; ++j) {
+      vm[j] = -INFINITY;
       if (j * NT * V < n) {
 #pragma unroll
-        for (int i = 0; i < V; i += 2) tm = lp_max(lp_max(tm, get16<T>(raw[j], i)), get16<T>(raw[j], i + 1));
+        for (int i = 0; i < V; i += 2) vm[j] = lp_max(lp_max(vm[j], get16<T>(raw[j], i)), get16<T>(raw[j], i + 1));
       }
+      tm = lp_max(tm, vm[j]);
+    }
     const float mn = lp_max(m, tm), dm = lp_diff(m, mn), f = lp_exp(dm);
     w = f * (w + dm * s);
     s *= f;
@@ -239,63 +308,62 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
       }
     if (TOP) {
       const bool first = c0 == beg;
-      float limit;
-      if (first) {
-        limit = lp_kth_lane(tm, top);
-        if (NW > 1) {
-          if (lane == 0) sh.red[0][wave] = limit;
-          lp_sync<NW>();
+      if (first) limit = lp_limit<NW>(tm, top, sh);
+      // (the first: not below the limit; later ones have to beat it, an equal logit of a higher class comes behind.  A NaN passes.)
+      uint32_t pending = 0;
 #pragma unroll
-          for (int k = 0; k < NW; ++k) limit = lp_max(limit, sh.red[0][k]);
+      for (int j = 0; j < NJ; ++j)
+        if (first ? !(vm[j] < limit) : !(vm[j] <= limit)) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float v = get16<T>(raw[j], i);
+            if (first ? !(v < limit) : !(v <= limit)) pending |= 1u << (j * V + i);
+          }
+          const int left = n - (j * NT + tid) * V;   // (of this row)
+          if (left < V) pending &= ~(~0u << (j * V + max(0, left)));
         }
-      } else {
-        limit = sh.last;
-      }
-      // (not below the limit; later ones have to beat it: an equal logit of a higher class comes behind.  A NaN passes.)
-      bool more = first ? !(tm < limit) : !(tm <= limit);
-      if (lp_any<NW>(more)) {
-        lp_forget(raw);
-        uint32_t pending = 0;
-        if (more) {
-#pragma unroll
-          for (int e = 0; e < LP_HOLD; ++e) {
-            const float v = get16<T>(raw[e / V], e % V);
-            const int c = ((e / V) * NT + tid) * V + e % V;
-            if ((first ? !(v < limit) : !(v <= limit)) && c < n) pending |= 1u << e;
+      auto push = [&]() {                            // (few: read again, from a cache, rather than picked out of registers)
+        if (pending) {
+          const int want = __builtin_popcount(pending), to = waiting + atomicAdd(&sh.count[turn], want);
+          for (int k = to; k < min(to + want, LpShared<NW>::ROOM); ++k) {
+            const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(pending));
+            sh.cand[k] = lp_key(ld_el<T>(x, at + c), (uint32_t)c);
+            pending &= pending - 1;
           }
         }
-        do {
-          if (pending) {                               // (few: read again, from a cache, rather than picked out of registers)
-            const int want = __builtin_popcount(pending), to = atomicAdd(&sh.count, want);
-            for (int k = to; k < min(to + want, LpShared<NW>::ROOM); ++k) {
-              const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(pending));
-              sh.cand[k] = lp_key(ld_el<T>(x, at + c), (uint32_t)c);
-              pending &= pending - 1;
-            }
-          }
+      };
+      push();
+      lp_sync<NW>();
+      waiting += sh.count[turn];
+      if ((have + waiting + top > 64 && c0 + TILE < end) || waiting > LpShared<NW>::ROOM) {
+        for (;;) {
+          const int got = min(waiting, LpShared<NW>::ROOM);
+          if (wave == 0) lp_order<NW>(sh, top, have, got);
+          have = min(top, have + got);
+          if (NW > 1 && waiting > got) lp_sync<NW>();        // (everyone has read the count that is cleared now)
+          if (waiting > got && tid == 0) sh.count[turn] = 0;
           lp_sync<NW>();
-          if (wave == 0) {
-            const int got = min(sh.count, LpShared<NW>::ROOM);
-            for (int b = 0; b < got; b += 64) {
-              const uint64_t k = lp_sort64(b + lane < got ? sh.cand[b + lane] : 0);
-              best = fresh ? k : lp_merge64(best, k);
-              fresh = false;
-            }
-            const uint64_t k = __shfl((unsigned long long)best, top - 1, 64);
-            if (lane == 0) {
-              sh.last_key = k;
-              sh.last = k ? lp_key_value(k) : -INFINITY;
-              sh.count = 0;
-            }
-          }
-          lp_sync<NW>();
+          limit = sh.last;
+          if (waiting == got) break;
           for (uint32_t left = pending; left; left &= left - 1) {
             const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(left));
             if (lp_key(ld_el<T>(x, at + c), (uint32_t)c) < sh.last_key) pending &= ~(left & -left);
           }
-        } while (lp_any<NW>(pending != 0));
+          waiting = 0;
+          push();
+          lp_sync<NW>();
+          waiting = sh.count[turn];
+        }
+        waiting = 0;
       }
+      // (the count after next: read last before this tile's barrier, added to next behind the next one's)
+      turn = turn == 2 ? 0 : turn + 1;
+      if (tid == 0) sh.count[turn == 2 ? 0 : turn + 1] = 0;
     }
+  }
+  if (TOP) {
+    if (waiting && wave == 0) lp_order<NW>(sh, top, have, waiting);
+    have = min(top, have + waiting);
   }
   // the threads' statistics joined
   float all = m;
@@ -328,7 +396,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
   if (wave != 0) return;
   if (parts > 1) {
     if (lane == 0) part_stats[unit] = make_float4(all, s, w, 0.f);
-    if (TOP && lane < top) part_keys[unit * top + lane] = best;
+    if (TOP && lane < top) part_keys[unit * top + lane] = lane < have ? sh.best[lane] : 0;
     return;
   }
   const LpRow r = lp_finish(all, s, w);
@@ -338,6 +406,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_wide_kernel(const void* __rest
     if (stats) stats[row] = make_float2(r.base, r.log_total);
   }
   if (TOP && lane < top) {
+    const uint64_t best = sh.best[lane];
     top_logprob[row * top + lane] = (lp_key_value(best) - r.base) - r.log_total;
     top_index[row * top + lane] = lp_key_class(best);
   }
@@ -354,30 +423,35 @@ __global__ __launch_bounds__(LP_TPB) void logprob_join_kernel(const void* __rest
   __shared__ uint64_t lists[4][64];
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // everything that is read, before anything waits: what depends on one another only
+  const int64_t t = target[row];
+  float4 q = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  if (lane < parts) q = part_stats[row * parts + lane];
   uint64_t best = 0;
   if (top) {
-    for (int p = wave; p < parts; p += 4)
-      best = lp_merge64(best, lane < top ? part_keys[(row * parts + p) * top + lane] : 0);
+    constexpr int U = 4;
+    for (int p0 = wave; p0 < parts; p0 += 4 * U) {
+      uint64_t k[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) k[u] = p0 + 4 * u < parts && lane < top ? part_keys[(row * parts + p0 + 4 * u) * top + lane] : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p0 + 4 * u < parts) best = p0 + 4 * u == wave ? k[u] : lp_merge64(best, k[u]);
+    }
     lists[wave][lane] = best;
+  }
+  float given = 0.f;
+  if (wave == 0 && t >= 0 && t < C) given = ld_el<T>(x, row * ld + t);
+  if (top) {
     __syncthreads();
+    if (wave < 2 && wave + 2 < parts) lists[wave][lane] = best = lp_merge64(best, lists[wave + 2][lane]);
+    __syncthreads();
+    if (wave == 0) best = lp_merge64(best, lists[1][lane]);
   }
   if (wave != 0) return;
-  const int64_t t = target[row];
-  float given = 0.f;
-  if (t >= 0 && t < C) given = ld_el<T>(x, row * ld + t);
-  for (int k = 1; top && k < 4; ++k) best = lp_merge64(best, lists[k][lane]);
-  float all = -INFINITY;
-  for (int p = lane; p < parts; p += 64) all = lp_max(all, part_stats[row * parts + p].x);
-  all = ccn_wave_join(all, lp_max);
-  float s = 0.f, w = 0.f;
-  for (int p = lane; p < parts; p += 64) {
-    const float4 q = part_stats[row * parts + p];
-    const float d = lp_diff(q.x, all), f = lp_exp(d);
-    s += f * q.y;
-    w += f * (q.z + d * q.y);
-  }
-  s = ccn_wave_sum(s);
-  w = ccn_wave_sum(w);
+  const float all = ccn_wave_join(q.x, lp_max);
+  const float d = lp_diff(q.x, all), f = lp_exp(d);
+  const float s = ccn_wave_sum(f * q.y), w = ccn_wave_sum(f * (q.z + d * q.y));
   const LpRow r = lp_finish(all, s, w);
   if (lane == 0) {
     logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
@@ -637,19 +711,22 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
   }
 }
 
-// How the rows are cut: parts of part_tiles tiles each where there are too few rows to fill the card (a workgroup takes a row, or a
-// part of one).
+// How rows are cut into parts of about one length, a workgroup each, where there are too few rows to fill the card: 512 x 131072 bf16
+// with 8 alternatives takes 58 us in one part to a row and 45 in three, 512 x 50000 31 and 27, but 1000 x 50000 38 and 44 in two (each
+// part orders its own); without alternatives 256 x 50000 12.2 and 13.0, 512 x 20000 fp32 11.3 and 13.6 (the joining launch).  Parts of less
+// than LP_PART cost more than they gain (96 x 131072 fp16 with 20: 23.9, with parts of half that 34.6).
+constexpr int64_t LP_FULL = 256, LP_FULL_TOP = 768, LP_WORKGROUPS = 1536, LP_PART = LP_TPB * LP_HOLD, LP_PARTS_MAX = 64;
 struct LpPlan {
-  int nw, parts, part_tiles;
+  int nw, parts, part_len;
 };
-LpPlan lp_plan(int64_t rows, int64_t C) {
-  LpPlan p = {C <= 64 * LP_HOLD ? 1 : 4, 1, 1};
-  const int64_t tile = (int64_t)p.nw * 64 * LP_HOLD, tiles = (C + tile - 1) / tile;
-  int64_t parts = (1024 + rows - 1) / rows;
-  if (parts > tiles) parts = tiles;
-  if (parts > 64) parts = 64;
-  p.part_tiles = (int)((tiles + parts - 1) / parts);
-  p.parts = (int)((tiles + p.part_tiles - 1) / p.part_tiles);
+LpPlan lp_plan(int64_t rows, int64_t C, int top) {
+  LpPlan p = {C <= 64 * LP_HOLD ? 1 : 4, 1, (int)C};
+  if (p.nw == 1 || rows >= (top ? LP_FULL_TOP : LP_FULL)) return p;
+  int64_t parts = (LP_WORKGROUPS + rows - 1) / rows;
+  if (parts > (C + LP_PART - 1) / LP_PART) parts = (C + LP_PART - 1) / LP_PART;
+  if (parts > LP_PARTS_MAX) parts = LP_PARTS_MAX;
+  p.part_len = (int)(((C + parts - 1) / parts + 7) / 8 * 8);
+  p.parts = (int)((C + p.part_len - 1) / p.part_len);
   return p;
 }
 
@@ -657,7 +734,7 @@ LpPlan lp_plan(int64_t rows, int64_t C) {
 
 extern "C" size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top) {
   if (rows <= 0 || C <= LP_NARROW || top < 0) return 0;
-  const LpPlan p = lp_plan(rows, C);
+  const LpPlan p = lp_plan(rows, C, top);
   if (p.parts == 1) return 0;
   return ccn_align256((size_t)rows * p.parts * sizeof(float4)) + ccn_align256((size_t)rows * p.parts * top * sizeof(uint64_t));
 }
@@ -702,7 +779,7 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
-  const LpPlan p = lp_plan(rows, C);
+  const LpPlan p = lp_plan(rows, C, top);
   const size_t need = ccn_logprob_workspace_bytes(rows, C, top);
   if (need && (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < need)) {
     ccn_set_error("logprob_fwd: workspace of %zu bytes, %zu are needed (16-byte aligned)", ws ? ws_bytes : (size_t)0, need);
@@ -714,7 +791,7 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
   CCN_REQUIRE(blocks < ((int64_t)1 << 31), "logprob_fwd: rows=%lld", (long long)rows);
 #define CCN_LP_WIDE(T, NW, TOP)                                                                                                   \
   hipLaunchKernelGGL((logprob_wide_kernel<T, NW, TOP>), dim3((unsigned)blocks), dim3(LP_TPB), 0, s, logits, ld, target, rows,      \
-                     (int)C, ignore_index, top, p.parts, p.part_tiles, logprob, entropy, (float2*)stats, top_logprob, top_index,   \
+                     (int)C, ignore_index, top, p.parts, p.part_len, logprob, entropy, (float2*)stats, top_logprob, top_index,   \
                      part_stats, part_keys)
 #define CCN_LP_FWD(T)                                                                                                             \
   do {                                                                                                                            \
