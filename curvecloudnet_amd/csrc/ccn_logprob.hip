@@ -124,7 +124,7 @@ __device__ __forceinline__ uint64_t lp_merge64(uint64_t a, uint64_t b) {
 // Lane k - 1 of the lane values in descending order (NaN first).
 __device__ __forceinline__ uint32_t lp_kth_lane(uint32_t sorted, int k) { return (uint32_t)__builtin_amdgcn_readlane(sorted, k - 1); }
 
-// ---- rows of more than 64 classes: NW waves hold NW * 2048 logits of a row at a time in registers (32 a thread), take their maximum,
+// ---- rows of more than 512 classes (or many alternatives of fewer): NW waves hold NW * 2048 logits of a row at a time in registers (32 a thread), take their maximum,
 // and add weights relative to the maximum so far: one pass over the row, one rescaling per 32 logits of a thread.
 //
 // Alternatives: the threads' maxima give a lower bound of the top-th largest of the first logits held that few others reach
@@ -464,38 +464,131 @@ __global__ __launch_bounds__(LP_TPB) void logprob_join_kernel(const void* __rest
   }
 }
 
-// ---- rows of up to 64 classes: 128 / TEAM rows go through shared memory (16-byte loads) and TEAM threads walk each of them there,
-// every TEAM-th class one, their results joined by lane moves.  The pitch puts the lanes of a wave on different banks.  More than one
-// thread to a long row, or shared memory has room for too few waves (us with one / two / four: 400070 x 20 10.7 / 12.0 / 13.7,
-// 300000 x 32 14.8 / 12.9 / 12.6, 300000 x 40 20.2 / 15.7 / 15.8, 220011 x 55 28.4 / 19.1 / 15.8).
-// Alternatives: `top` walks, each of which takes the largest value that is left (of equal ones the lowest class); 16 values in
-// registers instead of shared memory take as long.  Many of them leave through shared memory: a thread's own are `top` values wide,
-// 64 such stores side by side cost more than the walks (400070 x 20: 3 of them 17.6 us without the detour and 20.1 with it, 5 23.2
-// and 23.5, 8 36.6 and 29.6; 500000 x 8: 5 of them 20.4 and 14.3).
-constexpr int LP_NARROW = 64;
-constexpr int LP_NARROW_TPB = 128;
-constexpr int LP_TEAM1 = 24, LP_TEAM2 = 40;          // classes up to which one, two threads walk a row
-constexpr int LP_DIRECT_TOP = 4;                     // alternatives that are stored as they are found
-
+// ---- the values of TEAM lanes next to one another, joined
 template <int TEAM, typename V, typename F>
 __device__ __forceinline__ V lp_team(V v, F f) {
   if constexpr (TEAM >= 2) v = f(v, ccn_lane_xor<1>(v));
   if constexpr (TEAM >= 4) v = f(v, ccn_lane_xor<2>(v));
+  if constexpr (TEAM >= 8) v = f(v, ccn_lane_xor<4>(v));
+  if constexpr (TEAM >= 16) v = f(v, ccn_lane_xor<8>(v));
+  if constexpr (TEAM >= 32) v = f(v, ccn_lane_xor<16>(v));
+  if constexpr (TEAM >= 64) v = f(v, ccn_lane_xor<32>(v));
   return v;
 }
 
+// ---- rows of 25 to 512 classes: TEAM lanes hold a row in registers, 16 logits each, and join their results by lane moves; a
+// wave has 64 / TEAM rows.  Alternatives: `top` walks over the registers, each of which takes the largest logit that is left; TEAM of
+// them are kept, a lane each, and stored side by side.
 template <int T, int TEAM, bool TOP>
+__global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __restrict__ x, int64_t ld,
+                                                              const int64_t* __restrict__ target, int64_t rows, int C,
+                                                              int64_t ignore, int top, float* __restrict__ logprob,
+                                                              float* __restrict__ entropy, float2* __restrict__ stats,
+                                                              float* __restrict__ top_logprob, int64_t* __restrict__ top_index) {
+  constexpr int V = CcnVec16<T>::N, HOLD = 16, NJ = HOLD / V;
+  const int lane = threadIdx.x % TEAM;
+  const int64_t mine = (int64_t)blockIdx.x * (LP_TPB / TEAM) + threadIdx.x / TEAM, row = min(mine, rows - 1);
+  const bool live = mine < rows;                     // (every lane stays for the joins)
+  ccn_u32x4 raw[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, row * ld + (j * TEAM + lane) * V, C - (j * TEAM + lane) * V);
+  const int64_t t = target[row];
+  const float given = t >= 0 && t < C ? ld_el<T>(x, row * ld + t) : 0.f;
+  float m = -INFINITY, s = 0.f, w = 0.f;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+    if (j * TEAM * V < C) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = lp_max(m, get16<T>(raw[j], i));
+    }
+  m = lp_team<TEAM>(m, lp_max);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+    if (j * TEAM * V < C) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = lp_diff(get16<T>(raw[j], i), m), e = lp_exp(d);
+        s += e;
+        w = __builtin_fmaf(e, d, w);
+      }
+    }
+  s = lp_team<TEAM>(s, [](float a, float b) { return a + b; });
+  w = lp_team<TEAM>(w, [](float a, float b) { return a + b; });
+  const LpRow r = lp_finish(m, s, w);
+  if (live && lane == 0) {
+    logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
+    entropy[row] = r.entropy;
+    if (stats) stats[row] = make_float2(r.base, r.log_total);
+  }
+  if (!TOP) return;
+  int o[HOLD];                                       // the logits as whole numbers in the order of the alternatives
+#pragma unroll
+  for (int e = 0; e < HOLD; ++e) {
+    const float v = get16<T>(raw[e / V], e % V);
+    int b = __float_as_int(v + 0.0f);
+    if (v != v) b = 0x7f800001;
+    o[e] = ((e / V) * TEAM + lane) * V + e % V < C ? b ^ ((b >> 31) & 0x7fffffff) : INT_MIN;
+  }
+  float kept = 0.f;
+  int kept_class = 0;
+  for (int k = 0; k < top; ++k) {
+    int best = INT_MIN, at = 0;                      // (below every logit; taken ones become it)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (j * TEAM * V < C) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          at = o[j * V + i] > best ? j * TEAM * V + i : at;
+          best = max(best, o[j * V + i]);
+        }
+      }
+    // (value, then lower class, as one number)
+    uint64_t key = ((uint64_t)((uint32_t)best ^ 0x80000000u) << 32) | (uint32_t)~(at + lane * V);
+    key = lp_team<TEAM>(key, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    const int c = (int)(uint32_t)~(uint32_t)key, own = c - lane * V;
+    best = (int)((uint32_t)(key >> 32) ^ 0x80000000u);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (j * TEAM * V < C) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[j * V + i] = own == j * TEAM * V + i ? INT_MIN : o[j * V + i];
+      }
+    if (k % TEAM == lane) {
+      kept = (__int_as_float(best ^ ((best >> 31) & 0x7fffffff)) - r.base) - r.log_total;
+      kept_class = c;
+    }
+    if (k % TEAM == TEAM - 1 || k == top - 1) {
+      const int from = k / TEAM * TEAM;
+      if (live && from + lane <= k) {
+        top_logprob[row * top + from + lane] = kept;
+        top_index[row * top + from + lane] = kept_class;
+      }
+    }
+  }
+}
+
+// ---- rows of up to 24 classes: 128 rows go through shared memory (16-byte loads) and a thread walks each of them there; the odd pitch puts
+// the lanes of a wave on different banks.  (Two threads to a row, or the registers of logprob_team_kernel, take 12.0 and 12.3 us for
+// 400070 x 20 instead of 10.8.)
+// Alternatives: `top` walks, each of which takes the largest value that is left (of equal ones the lowest class).  Many of them leave
+// through shared memory: a thread's own are `top` values wide, 64 such stores side by side cost more than the walks (400070 x 20: 3 of
+// them 17.6 us without the detour and 20.1 with it, 5 23.2 and 23.5, 8 36.6 and 29.6; 500000 x 8: 5 of them 20.4 and 14.3).
+constexpr int LP_NARROW = 24;
+constexpr int LP_NARROW_TPB = 128;
+constexpr int LP_DIRECT_TOP = 4;                     // alternatives that are stored as they are found
+
+template <int T, bool TOP>
 __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const void* __restrict__ x, int64_t ld,
                                                                        const int64_t* __restrict__ target, int64_t rows, int C,
-                                                                       int pitch, int vecs, uint32_t magic, int64_t ignore, int top,
+                                                                       int vecs, uint32_t magic, int64_t ignore, int top,
                                                                        float* __restrict__ logprob, float* __restrict__ entropy,
                                                                        float2* __restrict__ stats,
                                                                        float* __restrict__ top_logprob,
                                                                        int64_t* __restrict__ top_index) {
   extern __shared__ float tile[];
-  constexpr int V = CcnVec16<T>::N, ROWS = LP_NARROW_TPB / TEAM;
+  constexpr int V = CcnVec16<T>::N, ROWS = LP_NARROW_TPB;
   const int64_t r0 = (int64_t)blockIdx.x * ROWS;
-  const int live = (int)min((int64_t)ROWS, rows - r0);
+  const int live = (int)min((int64_t)ROWS, rows - r0), pitch = C | 1;
   // 16-byte pieces, `vecs` to a row (i / vecs as a product: exact for i < 2^16, the error of magic is below 2^-16)
   const int n = live * vecs;
   for (int i = threadIdx.x; i < n; i += LP_NARROW_TPB) {
@@ -506,66 +599,54 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
       if (c + k < C) tile[q * pitch + c + k] = get16<T>(raw, k);
   }
   __syncthreads();
-  const int lane = threadIdx.x % TEAM, mine_row = min((int)threadIdx.x / TEAM, live - 1);       // (all lanes stay for the joins)
-  const bool writes = (int)threadIdx.x / TEAM < live && lane == 0;
-  float* const mine = tile + mine_row * pitch;
-  const int64_t row = r0 + mine_row, t = target[row];
-  float m = -INFINITY;
+  float* const out = tile + ROWS * pitch;
+  int* const out_class = reinterpret_cast<int*>(out + ROWS * top);
+  if ((int)threadIdx.x < live) {
+    float* const mine = tile + threadIdx.x * pitch;
+    const int64_t row = r0 + threadIdx.x, t = target[row];
+    float m = -INFINITY;
 #pragma unroll 4
-  for (int c = lane; c < C; c += TEAM) m = lp_max(m, mine[c]);
-  m = lp_team<TEAM>(m, lp_max);
-  const float given = t >= 0 && t < C ? mine[t] : 0.f;
-  float s = 0.f, w = 0.f;
+    for (int c = 0; c < C; ++c) m = lp_max(m, mine[c]);
+    const float given = t >= 0 && t < C ? mine[t] : 0.f;
+    float s = 0.f, w = 0.f;
 #pragma unroll 4
-  for (int c = lane; c < C; c += TEAM) {
-    const float v = mine[c], d = lp_diff(v, m), e = lp_exp(d);
-    s += e;
-    w = __builtin_fmaf(e, d, w);
-  }
-  s = lp_team<TEAM>(s, [](float a, float b) { return a + b; });
-  w = lp_team<TEAM>(w, [](float a, float b) { return a + b; });
-  const LpRow r = lp_finish(m, s, w);
-  if (writes) {
+    for (int c = 0; c < C; ++c) {
+      const float v = mine[c], d = lp_diff(v, m), e = lp_exp(d);
+      s += e;
+      w = __builtin_fmaf(e, d, w);
+      if (TOP) {                                     // from here on as a whole number in the order of the alternatives
+        int o = __float_as_int(v + 0.0f);
+        if (v != v) o = 0x7f800001;
+        mine[c] = __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+      }
+    }
+    const LpRow r = lp_finish(m, s, w);
     logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
     entropy[row] = r.entropy;
     if (stats) stats[row] = make_float2(r.base, r.log_total);
-  }
-  if (!TOP) return;
-  // (the given class's logit has been read by every thread of its wave, and a row's threads are of one wave)
-  int* const order = reinterpret_cast<int*>(mine);
-  float* const out = tile + ROWS * pitch;
-  int* const out_class = reinterpret_cast<int*>(out + ROWS * top);
-  const bool own = (int)threadIdx.x / TEAM < live;
-  for (int c = lane; c < C && own; c += TEAM) {      // as whole numbers in the order of the alternatives
-    const float v = mine[c];
-    int o = __float_as_int(v + 0.0f);
-    if (v != v) o = 0x7f800001;
-    order[c] = o ^ ((o >> 31) & 0x7fffffff);
-  }
-  for (int j = 0; j < top; ++j) {
-    int v = INT_MIN, at = 0;                         // (below every value; taken ones become it)
+    if (TOP) {
+      int* const order = reinterpret_cast<int*>(mine);
+      for (int j = 0; j < top; ++j) {
+        int v = INT_MIN, at = 0;                     // (below every value; taken ones become it)
 #pragma unroll 4
-    for (int c = lane; c < C; c += TEAM) {
-      const int o = order[c];
-      at = o > v ? c : at;
-      v = max(v, o);
-    }
-    // (value, then lower class, as one number)
-    const uint64_t k = lp_team<TEAM>(((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (uint32_t)~at,
-                                     [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-    at = (int)(uint32_t)~(uint32_t)k;
-    v = (int)((uint32_t)(k >> 32) ^ 0x80000000u);
-    if (own && at % TEAM == lane) order[at] = INT_MIN;
-    const float f = __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
-    if (writes && top <= LP_DIRECT_TOP) {
-      top_logprob[row * top + j] = (f - r.base) - r.log_total;
-      top_index[row * top + j] = at;
-    } else if (writes) {
-      out[mine_row * top + j] = (f - r.base) - r.log_total;
-      out_class[mine_row * top + j] = at;
+        for (int c = 0; c < C; ++c) {
+          const int o = order[c];
+          at = o > v ? c : at;
+          v = max(v, o);
+        }
+        order[at] = INT_MIN;
+        const float l = (__int_as_float(v ^ ((v >> 31) & 0x7fffffff)) - r.base) - r.log_total;
+        if (top <= LP_DIRECT_TOP) {
+          top_logprob[row * top + j] = l;
+          top_index[row * top + j] = at;
+        } else {
+          out[threadIdx.x * top + j] = l;
+          out_class[threadIdx.x * top + j] = at;
+        }
+      }
     }
   }
-  if (top <= LP_DIRECT_TOP) return;
+  if (!TOP || top <= LP_DIRECT_TOP) return;
   __syncthreads();
   for (int i = threadIdx.x; i < live * top; i += LP_NARROW_TPB) {
     top_logprob[r0 * top + i] = out[i];
@@ -579,11 +660,10 @@ struct LpGrad {
   int t;                                    // the given class, -1 where it is not scored
   float g;
 };
-__device__ __forceinline__ LpGrad lp_grad(int64_t row, const int64_t* __restrict__ target, int C, int64_t ignore, int top,
+__device__ __forceinline__ LpGrad lp_grad(int64_t row, const int64_t* __restrict__ target, int C, int64_t ignore,
                                           const float2* __restrict__ stats, const float* __restrict__ entropy,
                                           const float* __restrict__ g_logprob, int64_t g_logprob_stride,
-                                          const float* __restrict__ g_entropy, int64_t g_entropy_stride,
-                                          const float* __restrict__ g_top) {
+                                          const float* __restrict__ g_entropy, int64_t g_entropy_stride, float of_top) {
   LpGrad q;
   const int64_t t = target[row];
   const float2 st = stats[row];
@@ -594,8 +674,7 @@ __device__ __forceinline__ LpGrad lp_grad(int64_t row, const int64_t* __restrict
     if (t >= 0 && t < C) q.t = (int)t;
     q.g = q.t >= 0 ? g_logprob[row * g_logprob_stride] : NAN;
   }
-  float all = q.g;
-  for (int j = 0; j < top; ++j) all += g_top[row * top + j];
+  const float all = q.g + of_top;           // (of_top: the sum of the row's g_top)
   q.base = st.x;
   q.log_total = st.y;
   q.slope = -gh;
@@ -634,16 +713,11 @@ __device__ __forceinline__ ccn_u32x4 lp_grad16(const LpGrad& q, const ccn_u32x4&
   }
   return out;
 }
-// The value of an alternative: written again, with every one-hot term it takes part in (the same class twice gives the same value twice).
+// The value of an alternative: written again, with its one-hot term (a row's alternatives are distinct).
 template <int T>
 __device__ __forceinline__ void lp_grad_top(const LpGrad& q, const void* __restrict__ x, int64_t at, void* __restrict__ dx,
-                                            int64_t to, int64_t c, int top, const int64_t* __restrict__ top_index,
-                                            const float* __restrict__ g_top) {
-  float d = lp_smooth(q, ld_el<T>(x, at + c));
-  if (c == q.t) d += q.g;
-  for (int j = 0; j < top; ++j)
-    if (top_index[j] == c) d += g_top[j];
-  st_el<T>(dx, to + c, d);
+                                            int64_t to, int64_t c, float g) {
+  st_el<T>(dx, to + c, lp_smooth(q, ld_el<T>(x, at + c)) + (c == q.t ? q.g : 0.f) + g);
 }
 
 // A workgroup takes `group` rows of up to LP_GROUP_MAX classes, whose own values it computes once into shared memory; `vecs`: 16-byte
@@ -659,11 +733,19 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_rows_kernel(
     const float* __restrict__ g_entropy, int64_t g_entropy_stride, const float* __restrict__ g_top, void* __restrict__ dx, int64_t ldd) {
   constexpr int V = CcnVec16<T>::N;
   __shared__ LpGrad mine[LP_TPB];
+  extern __shared__ float gt[];                      // the group's g_top
   const int64_t r0 = (int64_t)blockIdx.x * group;
   const int live = (int)min((int64_t)group, rows - r0), n = live * vecs;
-  if ((int)threadIdx.x < live)
-    mine[threadIdx.x] = lp_grad(r0 + threadIdx.x, target, C, ignore, top, stats, entropy, g_logprob, g_logprob_stride, g_entropy,
-                                g_entropy_stride, g_top);
+  if (top) {
+    for (int i = threadIdx.x; i < live * top; i += LP_TPB) gt[i] = g_top[r0 * top + i];
+    __syncthreads();
+  }
+  if ((int)threadIdx.x < live) {
+    float of_top = 0.f;
+    for (int j = 0; j < top; ++j) of_top += gt[threadIdx.x * top + j];
+    mine[threadIdx.x] = lp_grad(r0 + threadIdx.x, target, C, ignore, stats, entropy, g_logprob, g_logprob_stride, g_entropy,
+                                g_entropy_stride, of_top);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += LP_TPB) {
     const int r = vecs == 1 ? i : (int)__umulhi((uint32_t)i, magic), c = (i - r * vecs) * V;
@@ -675,7 +757,7 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_rows_kernel(
   for (int i = threadIdx.x; i < live * top; i += LP_TPB) {
     const int r = i / top;
     const int64_t row = r0 + r, c = top_index[r0 * top + i];
-    if (c >= 0 && c < C) lp_grad_top<T>(mine[r], x, row * ld, dx, row * ldd, c, top, top_index + row * top, g_top + row * top);
+    if (c >= 0 && c < C) lp_grad_top<T>(mine[r], x, row * ld, dx, row * ldd, c, gt[i]);
   }
 }
 
@@ -697,7 +779,9 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
 #pragma unroll
     for (int j = 0; j < NJ; ++j) raw[j] = lp_load_part<T>(x, at + c0 + (j * LP_TPB + tid) * V, n - (j * LP_TPB + tid) * V);
   }
-  const LpGrad q = lp_grad(row, target, C, ignore, top, stats, entropy, g_logprob, g_logprob_stride, g_entropy, g_entropy_stride, g_top);
+  float of_top = 0.f;
+  for (int j = 0; j < top; ++j) of_top += g_top[row * top + j];
+  const LpGrad q = lp_grad(row, target, C, ignore, stats, entropy, g_logprob, g_logprob_stride, g_entropy, g_entropy_stride, of_top);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int c = (j * LP_TPB + tid) * V;
@@ -707,8 +791,18 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
   __syncthreads();
   if (tid < top) {
     const int64_t c = top_index[row * top + tid];
-    if (c >= c0 && c < c0 + n) lp_grad_top<T>(q, x, at, dx, to, c, top, top_index + row * top, g_top + row * top);
+    if (c >= c0 && c < c0 + n) lp_grad_top<T>(q, x, at, dx, to, c, g_top[row * top + tid]);
   }
+}
+
+// Lanes to a row of logprob_team_kernel, 0 where the row is logprob_wide_kernel's: that one's way to the alternatives costs the same for
+// many of them (us, 50000 x 500 bf16 with 0 / 4 / 8 / 16 of them: 16 / 38 / 54 / 90 here and 28 / 64 / 66 / 68 there; 50000 x 256 fp32 with
+// 0 / 16 / 32: 12 / 49 / 85 and 23 / 60 / 64; 100000 x 100 bf16 with 0 / 45: 11 / 108 and 52 / 210).
+int lp_team_of(int64_t C, int top) {
+  if (C <= 64) return 4;
+  if (C <= 128) return 8;
+  if (C > 512 || C * top > 4096) return 0;
+  return C <= 256 ? 16 : 32;
 }
 
 // How rows are cut into parts of about one length, a workgroup each, where there are too few rows to fill the card: 512 x 131072 bf16
@@ -750,32 +844,50 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
   CCN_REQUIRE(top == 0 || (top_logprob && top_index), "logprob_fwd: top > 0 without its outputs");
   hipStream_t s = (hipStream_t)stream;
   if (C <= LP_NARROW) {
-    const int team = C <= LP_TEAM1 ? 1 : C <= LP_TEAM2 ? 2 : 4, per = dtype == 0 ? 4 : 8;
-    const int vecs = (int)((C + per - 1) / per), n = LP_NARROW_TPB / team;
-    const int pitch = team == 1 ? (int)C | 1 : (int)((C + team - 1) / (2 * team) * 2 * team + team);     // team modulo 2 team
+    const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
-    const dim3 grid((unsigned)((rows + n - 1) / n)), block(LP_NARROW_TPB);
-    const size_t lds = (size_t)n * (pitch + (top > LP_DIRECT_TOP ? 2 * top : 0)) * sizeof(float);
-#define CCN_LP_NARROW(T, TEAM, TOP)                                                                                               \
-  hipLaunchKernelGGL((logprob_narrow_kernel<T, TEAM, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, pitch, vecs,    \
-                     magic, ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index)
-#define CCN_LP_TEAM(T, TOP)                                                                                                       \
-  do {                                                                                                                            \
-    if (team == 1) CCN_LP_NARROW(T, 1, TOP);                                                                                      \
-    else if (team == 2) CCN_LP_NARROW(T, 2, TOP);                                                                                 \
-    else CCN_LP_NARROW(T, 4, TOP);                                                                                                \
-  } while (0)
+    const dim3 grid((unsigned)((rows + LP_NARROW_TPB - 1) / LP_NARROW_TPB)), block(LP_NARROW_TPB);
+    const size_t lds = (size_t)LP_NARROW_TPB * ((C | 1) + (top > LP_DIRECT_TOP ? 2 * top : 0)) * sizeof(float);
+#define CCN_LP_NARROW(T, TOP)                                                                                                     \
+  hipLaunchKernelGGL((logprob_narrow_kernel<T, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, vecs, magic,          \
+                     ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index)
     if (top) {
-      if (dtype == 0) CCN_LP_TEAM(0, true);
-      else if (dtype == 1) CCN_LP_TEAM(1, true);
-      else CCN_LP_TEAM(2, true);
+      if (dtype == 0) CCN_LP_NARROW(0, true);
+      else if (dtype == 1) CCN_LP_NARROW(1, true);
+      else CCN_LP_NARROW(2, true);
     } else {
-      if (dtype == 0) CCN_LP_TEAM(0, false);
-      else if (dtype == 1) CCN_LP_TEAM(1, false);
-      else CCN_LP_TEAM(2, false);
+      if (dtype == 0) CCN_LP_NARROW(0, false);
+      else if (dtype == 1) CCN_LP_NARROW(1, false);
+      else CCN_LP_NARROW(2, false);
     }
-#undef CCN_LP_TEAM
 #undef CCN_LP_NARROW
+    CCN_LAUNCH_OK("logprob_fwd");
+    return CCN_OK;
+  }
+  const int team = lp_team_of(C, top);
+  if (team) {
+#define CCN_LP_TEAM(T, TEAM)                                                                                                      \
+  do {                                                                                                                            \
+    const dim3 grid((unsigned)((rows + LP_TPB / TEAM - 1) / (LP_TPB / TEAM))), block(LP_TPB);                                     \
+    if (top)                                                                                                                      \
+      hipLaunchKernelGGL((logprob_team_kernel<T, TEAM, true>), grid, block, 0, s, logits, ld, target, rows, (int)C,          \
+                         ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index);                            \
+    else                                                                                                                          \
+      hipLaunchKernelGGL((logprob_team_kernel<T, TEAM, false>), grid, block, 0, s, logits, ld, target, rows, (int)C,         \
+                         ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index);                            \
+  } while (0)
+#define CCN_LP_TEAMS(T)                                                                                                           \
+  do {                                                                                                                            \
+    if (team == 4) CCN_LP_TEAM(T, 4);                                                                                    \
+    else if (team == 8) CCN_LP_TEAM(T, 8);                                                                                    \
+    else if (team == 16) CCN_LP_TEAM(T, 16);                                                                                  \
+    else CCN_LP_TEAM(T, 32);                                                                                                  \
+  } while (0)
+    if (dtype == 0) CCN_LP_TEAMS(0);
+    else if (dtype == 1) CCN_LP_TEAMS(1);
+    else CCN_LP_TEAMS(2);
+#undef CCN_LP_TEAMS
+#undef CCN_LP_TEAM
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
@@ -832,7 +944,7 @@ extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const 
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
     const dim3 grid((unsigned)((rows + group - 1) / group)), block(LP_TPB);
 #define CCN_LP_BWD(T)                                                                                                             \
-  hipLaunchKernelGGL(logprob_bwd_rows_kernel<T>, grid, block, 0, s, logits, ld, target, rows, (int)C, ignore_index, top, group,    \
+  hipLaunchKernelGGL(logprob_bwd_rows_kernel<T>, grid, block, (size_t)group * top * sizeof(float), s, logits, ld, target, rows, (int)C, ignore_index, top, group,    \
                      vecs, magic, top_index, (const float2*)stats, entropy, g_logprob, g_logprob_stride, g_entropy,               \
                      g_entropy_stride, g_top, dlogits, ldd)
     if (dtype == 0) CCN_LP_BWD(0);

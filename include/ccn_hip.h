@@ -710,6 +710,7 @@ int ccn_adam_step(float* param, const float* grad, float* exp_avg, float* exp_av
  * class; top <= 64, top <= C).  A row of -inf only: logprob -inf, entropy 0.
  * bwd: dlogits (`dtype`, row stride ldd) = d / d logits of sum(g_logprob logprob) + sum(g_entropy entropy) + sum(g_top top_logprob);
  * g_logprob and g_entropy are read at row * their stride (0: one value for all rows) and may be null, g_top is rows x top.
+ * top_index as fwd gave it: a row's classes are distinct (of a class that is there twice one gradient is lost; outside [0, C): skipped).
  * Deterministic.  ws: ccn_logprob_workspace_bytes of device memory (0: none needed). */
 size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top);
 int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index,

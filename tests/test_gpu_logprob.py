@@ -135,8 +135,9 @@ def _target(rows, c, seed=0):
     return torch.randint(0, c, (rows,), generator=torch.Generator().manual_seed(seed + rows + c)).to(DEV)
 
 
-SIZES = [(1, 1), (1, 2), (2, 1), (3, 5), (257, 20), (1000, 20), (64, 55), (513, 55), (5, 63), (5, 64), (5, 65), (70, 66), (7, 127),
-         (9, 255), (9, 256), (9, 257), (33, 300), (5, 511), (5, 513), (4, 1000), (4, 1023), (4, 1025), (3, 2047), (3, 2048), (3, 2049),
+SIZES = [(1, 1), (1, 2), (2, 1), (3, 5), (257, 20), (1000, 20), (129, 23), (130, 24), (131, 25), (70, 26), (65, 33), (64, 55), (513, 55),
+         (5, 63), (5, 64), (5, 65), (70, 66), (7, 127), (33, 128), (33, 129), (9, 255), (9, 256), (17, 257), (33, 300), (5, 511), (9, 512),
+         (5, 513), (4, 1000), (4, 1023), (4, 1025), (3, 2047), (3, 2048), (3, 2049),
          (2, 4095), (2, 4097), (2, 8191), (2, 8193), (3, 16385), (1, 32769), (1, 50021), (2, 65535), (2, 65537), (300, 4099), (1, 262144),
          (1, 300007)]
 
@@ -151,13 +152,29 @@ def test_scores_and_gradient_over_sizes(rows, c, dtype):
     _check_gradient(x, t, min(c, 5))
 
 
-@pytest.mark.parametrize("rows,c", [(3, 64), (40, 64), (3, 65), (3, 100), (2, 2048), (3, 9000), (1, 70000)])
+@pytest.mark.parametrize("rows,c", [(3, 64), (40, 64), (3, 65), (3, 100), (40, 128), (17, 200), (18, 256), (9, 257), (10, 500), (9, 512),
+                                    (5, 513), (2, 2048), (3, 9000), (1, 70000)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_many_alternatives(rows, c, dtype):
     x, t = _logits(rows, c, dtype), _target(rows, c)
-    for top in (31, 32, 33, 63, 64):
+    for top in (2, 3, 4, 6, 8, 9, 12, 15, 16, 17, 18, 21, 31, 32, 33, 63, 64):
         _check(x, t, top)
+    _check_gradient(x, t, 17)
     _check_gradient(x, t, 64)
+
+
+@pytest.mark.parametrize("top", [1, 2, 3, 4, 5, 6, 9, 15, 16, 17, 20, 33])
+def test_a_row_that_is_taken_in_many_pieces(top):
+    """Random, rising and falling rows of a dozen pieces, in one part and in several, and rows whose first piece is the least."""
+    for rows, c in ((2, 100003), (800, 40001)):
+        x = _logits(rows, c, torch.float32)
+        x[0] = torch.arange(c, device=DEV) * (40.0 / c)
+        x[1] = x[0].flip(0)
+        if rows > 2:
+            x[2:200] += torch.arange(c, device=DEV) * (4.0 / c)
+            x[200:400, :9000] -= 30.0
+            x[400:500] = (x[400:500] * 2).round()
+        _check(x, _target(rows, c), top)
 
 
 def test_every_class_is_an_alternative():
