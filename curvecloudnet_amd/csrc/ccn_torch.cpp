@@ -290,15 +290,18 @@ std::vector<Tensor> grads_of(const std::vector<Tensor>& parameters) {
   return grads;
 }
 
-Tensor clip_grad_norm(const std::vector<Tensor>& grads, int kind, double max_norm) {
-  Table t = table_of(grads, "clip_grad_norm_");
+// None where no parameter has a gradient.
+py::object clip_grad_norm(const std::vector<Tensor>& parameters, int kind, double max_norm) {
+  const std::vector<Tensor> grads = grads_of(parameters);
+  if (grads.empty()) return py::none();
+  const Table t = table_of(grads, "clip_grad_norm_");
   NormOut o(t);
   launch("grad_clip", {t.n(), kind, o.bytes}, t.total, [&] {
     return entry.grad_clip(const_cast<void* const*>(t.at.data()), t.size.data(), t.code.data(), t.n(), kind, max_norm,
                            o.ws.mutable_data_ptr(), (size_t)o.bytes, o.norm.mutable_data_ptr<float>(), stream_of(t.one));
   });
   moved(grads);
-  return o.norm;
+  return py::cast(o.norm);
 }
 
 // ---- the update

@@ -274,15 +274,14 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     32 bits and rounded once to the gradient's type.  A norm that is not finite gives what the formula gives (0 or NaN), or raises with
     ``error_if_nonfinite`` (which waits for the GPU) before anything is scaled.  Gradients that share memory are refused."""
     kind, max_norm = _norm_kind(norm_type, "clip_grad_norm_"), _bound(max_norm, "clip_grad_norm_")
-    grads = binding().grads_of([parameters] if isinstance(parameters, torch.Tensor) else list(parameters))
-    if not grads:
-        return torch.zeros(())
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     _join_wgrad()
     if error_if_nonfinite:
-        norm = float(binding().grad_norm(grads, kind))
+        norm = float(grad_norm(binding().grads_of(parameters), norm_type))
         if not math.isfinite(norm):
             raise RuntimeError("clip_grad_norm_: the norm of the gradients is %r" % norm)
-    return binding().clip_grad_norm(grads, kind, max_norm)
+    norm = binding().clip_grad_norm(parameters, kind, max_norm)
+    return torch.zeros(()) if norm is None else norm
 
 
 def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, max_norm=None):
