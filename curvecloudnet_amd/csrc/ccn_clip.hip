@@ -152,8 +152,13 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double*
   }
 }
 
+// The factor is rounded to the gradients' type first, as a torch tensor's product with a scalar tensor rounds it: the same bits come out
+// as from clipping with torch, within half a step of the type more than from the factor in 32 bits.
 template <int T>
 __device__ __forceinline__ void clip_apply(char* p, int n, float scale) {
+  ccn_u32x4 of_type = {0, 0, 0, 0};
+  put16<T>(of_type, 0, scale);
+  scale = get16<T>(of_type, 0);
   constexpr int V = CcnVec16<T>::N, STEP = CLIP_TPB * V, U = 4;
   for (int i = threadIdx.x * V; i - (int)threadIdx.x * V < n; i += U * STEP) {
     ccn_u32x4 r[U];

@@ -129,14 +129,12 @@ __device__ __forceinline__ uint32_t lp_kth_lane(uint32_t sorted, int k) { return
 //
 // Alternatives: the threads' maxima give a lower bound of the top-th largest of the first logits held that few others reach
 // (lp_limit).  Those that do wait in shared memory, and so do later ones that beat the bound, about `top` of 8192 random logits.  Wave 0
-// puts them in order when another `top` would make them more than 64, and at the end; the last of the best is the new bound.  Where
-// more qualify than there is room for (equal logits, rising rows), the rest is looked at again after an ordering, against the new bound;
-// every turn settles LpShared::ROOM of them.
+// puts them in order when another `top` would make them more than 64, and at the end; the last of the best is the new bound.
 constexpr int LP_HOLD = 32;
 
 template <int NW>
 struct LpShared {
-  static constexpr int ROOM = NW == 4 ? 1024 : 256;
+  static constexpr int ROOM = NW == 4 ? 1024 : 512;
   uint64_t cand[ROOM];                      // waiting
   uint64_t best[64];                        // in order, descending
   uint64_t last_key;                        // the top-th of them, 0 where there are fewer
@@ -216,7 +214,7 @@ __device__ __forceinline__ int lp_class(int c0, int tid, int e) {
 }
 
 template <int T, int NW, bool TOP>
-__global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 ? 5 : 6) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
+__global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
                                                               const int64_t* __restrict__ target, int64_t rows, int C,
                                                               int64_t ignore, int top, int parts, int part_len,
                                                               float* __restrict__ logprob, float* __restrict__ entropy,
@@ -282,52 +280,79 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 ? 5 : 6) void logprob_wi
     if (TOP) {
       const bool first = c0 == beg;
       if (first) limit = lp_limit<NW>(tm, top, sh);
-      // (the first: not below the limit; later ones have to beat it, an equal logit of a higher class comes behind.  A NaN passes.)
-      uint32_t pending = 0;
+      // the logits of this thread that are not below v, or that beat it (a NaN is and does)
+      auto reach = [&](float v, bool beat) {
+        uint32_t some = 0;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        if (first ? !(vm[j] < limit) : !(vm[j] <= limit)) {
+        for (int j = 0; j < NJ; ++j)
+          if (beat ? !(vm[j] <= v) : !(vm[j] < v)) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float v = get16<T>(raw[j], i);
-            if (first ? !(v < limit) : !(v <= limit)) pending |= 1u << (j * V + i);
+            for (int i = 0; i < V; ++i) {
+              const float u = get16<T>(raw[j], i);
+              if (beat ? !(u <= v) : !(u < v)) some |= 1u << (j * V + i);
+            }
+            const int left = n - (j * NT + tid) * V; // (of this row)
+            if (left < V) some &= ~(~0u << (j * V + max(0, left)));
           }
-          const int left = n - (j * NT + tid) * V;   // (of this row)
-          if (left < V) pending &= ~(~0u << (j * V + max(0, left)));
-        }
-      auto push = [&]() {                            // (few: read again, from a cache, rather than picked out of registers)
-        if (pending) {
-          const int want = __builtin_popcount(pending), to = waiting + atomicAdd(&sh.count[turn], want);
+        return some;
+      };
+      // (later ones have to beat the limit: an equal logit of a higher class comes behind)
+      uint32_t pending = reach(limit, !first);
+      const uint32_t all = pending;
+      auto push = [&](uint32_t some) {               // (few: read again, from a cache, rather than picked out of registers)
+        if (some) {
+          const int want = __builtin_popcount(some), to = waiting + atomicAdd(&sh.count[turn], want);
           for (int k = to; k < min(to + want, LpShared<NW>::ROOM); ++k) {
-            const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(pending));
+            const int e = __builtin_ctz(some), c = lp_class<T, NT>(c0, tid, e);
             sh.cand[k] = lp_key(ld_el<T>(x, at + c), (uint32_t)c);
-            pending &= pending - 1;
+            some &= some - 1;
+            pending &= ~(1u << e);
           }
         }
       };
-      push();
+      const bool flood = __builtin_amdgcn_ballot_w64(__builtin_popcount(pending) > LP_HOLD / 2) != 0;
+      if (!flood) push(pending);
+      else if (lane == 0) atomicAdd(&sh.count[turn], LpShared<NW>::ROOM + 1);
       lp_sync<NW>();
-      waiting += sh.count[turn];
-      if ((have + waiting + top > 64 && c0 + TILE < end) || waiting > LpShared<NW>::ROOM) {
-        for (;;) {
-          const int got = min(waiting, LpShared<NW>::ROOM);
-          if (wave == 0) lp_order<NW>(sh, top, have, got);
-          have = min(top, have + got);
-          if (NW > 1 && waiting > got) lp_sync<NW>();        // (everyone has read the count that is cleared now)
-          if (waiting > got && tid == 0) sh.count[turn] = 0;
-          lp_sync<NW>();
-          limit = sh.last;
-          if (waiting == got) break;
+      const int came = sh.count[turn];
+      if (waiting + came > LpShared<NW>::ROOM) {
+        // equal logits or a rising row: over again, against what the logits held now promise by themselves; those of the first 64 classes
+        // go first, which settles any number of equal ones; then as many at a time as there is room for
+        // (one wave to a row has its logits at hand again in a cache, and no registers for two more looks at them)
+        auto drop = [&](auto out) {
           for (uint32_t left = pending; left; left &= left - 1) {
             const int c = lp_class<T, NT>(c0, tid, __builtin_ctz(left));
-            if (lp_key(ld_el<T>(x, at + c), (uint32_t)c) < sh.last_key) pending &= ~(left & -left);
+            if (out(ld_el<T>(x, at + c), c)) pending &= ~(left & -left);
           }
-          waiting = 0;
-          push();
+        };
+        pending = all;
+        const float own = lp_limit<NW>(tm, top, sh);
+        if (NW == 1) drop([&](float v, int) { return v < own; });
+        else pending &= reach(own, false);
+        for (bool opening = true;; opening = false) {
+          if (tid == 0) sh.count[turn] = 0;          // (everyone has read it: a barrier ago)
           lp_sync<NW>();
-          waiting = sh.count[turn];
+          push(!opening ? pending : tid * V < 64 ? pending & ((1u << V) - 1) : 0);
+          lp_sync<NW>();
+          const int now = waiting + sh.count[turn], got = min(now, LpShared<NW>::ROOM);
+          if (wave == 0) lp_order<NW>(sh, top, have, got);
+          have = min(top, have + got);
+          waiting = 0;
+          lp_sync<NW>();
+          limit = sh.last;
+          if (!opening && now == got) break;
+          if (NW > 1 && opening) pending &= reach(limit, true);
+          else drop([&](float v, int c) { return lp_key(v, (uint32_t)c) < sh.last_key; });
         }
-        waiting = 0;
+      } else {
+        waiting += came;
+        if (have + waiting + top > 64 && c0 + TILE < end) {
+          if (wave == 0) lp_order<NW>(sh, top, have, waiting);
+          have = min(top, have + waiting);
+          waiting = 0;
+          lp_sync<NW>();
+          limit = sh.last;
+        }
       }
       // (the count after next: read last before this tile's barrier, added to next behind the next one's)
       turn = turn == 2 ? 0 : turn + 1;

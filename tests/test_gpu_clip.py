@@ -1,8 +1,10 @@
 """parallel.grad_norm, clip_grad_norm_, adam_step_ and FlatAdam(max_norm=) on the GPU against their formulas in 64 bits.
 
 Tolerances, derived.  u = 2^-24.  Norms are summed in 64 bits (their error there, 2^-53 times the number of values, is nothing) and
-rounded once: u |norm|.  The factor is rounded once and the product once in 32 bits, then once to the gradient's type: a clipped
-value is off by (2 u + eps / 2) of itself, and by half a subnormal step of fp16 (2^-25) or bf16 / fp32 (2^-134 / 2^-150).
+rounded once: u |norm|.  The factor is rounded to 32 bits and to the gradient's type (as torch's product with a scalar tensor does), the
+product to 32 bits and to the type: (1 + u)^2 (1 + eps / 2)^2 - 1, a clipped value is off by (2 u + eps) of itself (2 u for fp32, whose type
+rounds nothing more) and eps^2 / 4 + 2 u eps, less than a hundredth of that; and by half a subnormal step of fp16 (2^-25; the factor's own
+may be subnormal too: 2^-25 of |g|) or bf16 / fp32 (2^-134 / 2^-150).
 """
 import math
 
@@ -63,13 +65,13 @@ def _check_clip(params, max_norm, kind=2.0):
     for p, g, b, a in zip(params, grads, before, at):
         assert p.grad is g and g.data_ptr() == a
         ref = b.cpu().double() * scale
-        eps = torch.finfo(g.dtype).eps / 2
-        tiny = 2.0 ** -25 if g.dtype == torch.float16 else 2.0 ** -134
+        eps = 0.0 if g.dtype == torch.float32 else torch.finfo(g.dtype).eps
+        tiny = 2.0 ** -25 * (1 + b.cpu().double().abs()) if g.dtype == torch.float16 else 2.0 ** -134
         if scale == 1.0:
             assert torch.equal(g, b)
             continue
         off = (g.cpu().double() - ref).abs()
-        assert bool((off <= ref.abs() * (2 * U + eps) * 1.001 + tiny).all())
+        assert bool((off <= ref.abs() * (2 * U + eps) * 1.01 + tiny).all())
     return norm
 
 
@@ -182,6 +184,18 @@ def test_shared_memory_is_refused():
     twice = float(grad_norm([p[1].grad, p[1].grad]))                    # (a norm only reads: counted as often as it is given)
     want = math.sqrt(2.0) * _norm64([p[1].grad], 2)
     assert abs(twice - want) <= 2 * U * want
+
+
+def test_same_bits_as_torch():
+    """torch.nn.utils.clip_grad_norm_ on the same gradients: for 16-bit types its factor is taken from the norm here, torch rounds its own
+    norm to the type."""
+    from curvecloudnet_amd.parallel import clip_grad_norm_
+    for d in DTYPES:
+        p = _params([(1000,), (77, 3), (5,)], [d] * 3)
+        q = _params([(1000,), (77, 3), (5,)], [d] * 3)
+        norm = clip_grad_norm_(p, 1.5)
+        torch._foreach_mul_([x.grad for x in q], (1.5 / (norm.double() + 1e-6)).float())
+        assert all(torch.equal(a.grad, b.grad) for a, b in zip(p, q))
 
 
 def test_versions_move_and_neighbours_stay():
