@@ -137,7 +137,7 @@ __device__ __forceinline__ double clip_total(const double* __restrict__ partial,
 }
 __device__ __forceinline__ float clip_scale(double norm, double max_norm) {
   const double s = max_norm / (norm + 1e-6);
-  return s != s ? NAN : s < 1.0 ? (float)s : 1.f;       // (a NaN norm makes every gradient NaN; an infinite one makes them 0)
+  return s != s ? NAN : s < 1.0 ? (float)s : 1.f;       // (a NaN norm makes every gradient NaN; an infinite one 0, and NaN where infinite)
 }
 
 // The norm, and the factor of the kernels that follow where there are many of their workgroups.
@@ -152,13 +152,16 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double*
   }
 }
 
-// The factor is rounded to the gradients' type first, as a torch tensor's product with a scalar tensor rounds it: the same bits come out
-// as from clipping with torch, within half a step of the type more than from the factor in 32 bits.
+// The factor is rounded to the gradients' type first, as a torch tensor's product with a scalar tensor rounds it: the same bits come out,
+// for half a step of the type more than with the factor in 32 bits.  Below the normal numbers of fp16, where half a step can be all of
+// the factor (a norm of 10^7 and a bound of 0.1), it stays in 32 bits.
 template <int T>
 __device__ __forceinline__ void clip_apply(char* p, int n, float scale) {
-  ccn_u32x4 of_type = {0, 0, 0, 0};
-  put16<T>(of_type, 0, scale);
-  scale = get16<T>(of_type, 0);
+  if (T != 2 || !(scale < 0x1p-14f)) {
+    ccn_u32x4 of_type = {0, 0, 0, 0};
+    put16<T>(of_type, 0, scale);
+    scale = get16<T>(of_type, 0);
+  }
   constexpr int V = CcnVec16<T>::N, STEP = CLIP_TPB * V, U = 4;
   for (int i = threadIdx.x * V; i - (int)threadIdx.x * V < n; i += U * STEP) {
     ccn_u32x4 r[U];
@@ -283,7 +286,7 @@ int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype
                 "%s: tensor %lld: null or not aligned to its type", who, (long long)i);
   }
   if (!writes) return CCN_OK;
-  bool ordered = true;                               // tensors of one buffer come in order, or in reverse: looked at before sorting
+  bool ordered = true;                               // (tensors of one buffer mostly come in order)
   std::vector<std::pair<uintptr_t, uintptr_t>> span;
   try {
     span.reserve((size_t)n);

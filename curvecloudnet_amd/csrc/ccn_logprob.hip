@@ -124,8 +124,9 @@ __device__ __forceinline__ uint64_t lp_merge64(uint64_t a, uint64_t b) {
 // Lane k - 1 of the lane values in descending order (NaN first).
 __device__ __forceinline__ uint32_t lp_kth_lane(uint32_t sorted, int k) { return (uint32_t)__builtin_amdgcn_readlane(sorted, k - 1); }
 
-// ---- rows of more than 512 classes (or many alternatives of fewer): NW waves hold NW * 2048 logits of a row at a time in registers (32 a thread), take their maximum,
-// and add weights relative to the maximum so far: one pass over the row, one rescaling per 32 logits of a thread.
+// ---- rows of more than 512 classes (or many alternatives of fewer): NW waves hold NW * 2048 logits of a row at a time in registers (32
+// a thread), take their maximum, and add weights relative to the maximum so far: one pass over the row, one rescaling per 32 logits of a
+// thread.
 //
 // Alternatives: the threads' maxima give a lower bound of the top-th largest of the first logits held that few others reach
 // (lp_limit).  Those that do wait in shared memory, and so do later ones that beat the bound, about `top` of 8192 random logits.  Wave 0
@@ -822,25 +823,15 @@ LpPlan lp_plan(int64_t rows, int64_t C, int top) {
   return p;
 }
 
-}  // namespace
+// A launch holds fewer than 2^32 threads: rows go in pieces (a workgroup of the widest takes one).
+constexpr int64_t LP_LAUNCH_ROWS = (int64_t)1 << 22;
+const void* lp_row(const void* x, int dtype, int64_t at) { return (const char*)x + at * (dtype == 0 ? 4 : 2); }
+int64_t lp_tiles(int64_t C) { return (C + LP_TPB * LP_HOLD - 1) / (LP_TPB * LP_HOLD); }
 
-extern "C" size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top) {
-  if (rows <= 0 || C <= LP_NARROW || top < 0) return 0;
-  const LpPlan p = lp_plan(rows, C, top);
-  if (p.parts == 1) return 0;
-  return ccn_align256((size_t)rows * p.parts * sizeof(float4)) + ccn_align256((size_t)rows * p.parts * top * sizeof(uint64_t));
-}
-
-extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C,
-                               int64_t ignore_index, int top, float* logprob, float* entropy, float* stats, float* top_logprob,
-                               int64_t* top_index, void* ws, size_t ws_bytes, void* stream) {
-  CCN_REQUIRE(logits && target && logprob && entropy, "logprob_fwd: null pointer");
-  CCN_REQUIRE(dtype >= 0 && dtype <= 2, "logprob_fwd: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
-  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 30) && (ld >= C || rows == 1),
-              "logprob_fwd: rows=%lld C=%lld ld=%lld", (long long)rows, (long long)C, (long long)ld);
-  CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_fwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
-  CCN_REQUIRE(top == 0 || (top_logprob && top_index), "logprob_fwd: top > 0 without its outputs");
-  hipStream_t s = (hipStream_t)stream;
+// The launches of one piece of the rows (p: of all of them).
+int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index, int top,
+           const LpPlan& p, float* logprob, float* entropy, float* stats, float* top_logprob, int64_t* top_index, void* ws,
+           hipStream_t s) {
   if (C <= LP_NARROW) {
     const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
@@ -862,8 +853,7 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
-  const int team = lp_team_of(C, top);
-  if (team) {
+  if (const int team = lp_team_of(C, top)) {
 #define CCN_LP_TEAM(T, TEAM)                                                                                                      \
   do {                                                                                                                            \
     const dim3 grid((unsigned)((rows + LP_TPB / TEAM - 1) / (LP_TPB / TEAM))), block(LP_TPB);                                     \
@@ -889,16 +879,9 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
-  const LpPlan p = lp_plan(rows, C, top);
-  const size_t need = ccn_logprob_workspace_bytes(rows, C, top);
-  if (need && (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < need)) {
-    ccn_set_error("logprob_fwd: workspace of %zu bytes, %zu are needed (16-byte aligned)", ws ? ws_bytes : (size_t)0, need);
-    return CCN_ERR_WORKSPACE;
-  }
   float4* const part_stats = (float4*)ws;
-  uint64_t* const part_keys = need ? (uint64_t*)((char*)ws + ccn_align256((size_t)rows * p.parts * sizeof(float4))) : nullptr;
+  uint64_t* const part_keys = ws ? (uint64_t*)((char*)ws + ccn_align256((size_t)rows * p.parts * sizeof(float4))) : nullptr;
   const int64_t blocks = p.nw == 1 ? (rows + 3) / 4 : rows * p.parts;
-  CCN_REQUIRE(blocks < ((int64_t)1 << 31), "logprob_fwd: rows=%lld", (long long)rows);
 #define CCN_LP_WIDE(T, NW, TOP)                                                                                                   \
   hipLaunchKernelGGL((logprob_wide_kernel<T, NW, TOP>), dim3((unsigned)blocks), dim3(LP_TPB), 0, s, logits, ld, target, rows,      \
                      (int)C, ignore_index, top, p.parts, p.part_len, logprob, entropy, (float2*)stats, top_logprob, top_index,   \
@@ -923,36 +906,24 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
   return CCN_OK;
 }
 
-extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C,
-                               int64_t ignore_index, int top, const int64_t* top_index, const float* stats, const float* entropy,
-                               const float* g_logprob, int64_t g_logprob_stride, const float* g_entropy, int64_t g_entropy_stride,
-                               const float* g_top, void* dlogits, int64_t ldd, void* stream) {
-  CCN_REQUIRE(logits && target && stats && entropy && dlogits, "logprob_bwd: null pointer");
-  CCN_REQUIRE(dtype >= 0 && dtype <= 2, "logprob_bwd: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
-  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 30) && (ld >= C || rows == 1) &&
-              (ldd >= C || rows == 1), "logprob_bwd: rows=%lld C=%lld ld=%lld ldd=%lld", (long long)rows, (long long)C,
-              (long long)ld, (long long)ldd);
-  CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_bwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
-  CCN_REQUIRE(top == 0 || (g_top && top_index), "logprob_bwd: top > 0 without its gradient and classes");
-  CCN_REQUIRE(g_logprob_stride >= 0 && g_entropy_stride >= 0, "logprob_bwd: negative gradient stride");
-  hipStream_t s = (hipStream_t)stream;
+int lp_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index, int top,
+           const int64_t* top_index, const float* stats, const float* entropy, const float* g_logprob, int64_t g_logprob_stride,
+           const float* g_entropy, int64_t g_entropy_stride, const float* g_top, void* dlogits, int64_t ldd, hipStream_t s) {
   if (C <= LP_GROUP_MAX) {
     const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
     const int group = (int)(LP_GROUP / C < 1 ? 1 : LP_GROUP / C > LP_TPB ? LP_TPB : LP_GROUP / C);
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
     const dim3 grid((unsigned)((rows + group - 1) / group)), block(LP_TPB);
 #define CCN_LP_BWD(T)                                                                                                             \
-  hipLaunchKernelGGL(logprob_bwd_rows_kernel<T>, grid, block, (size_t)group * top * sizeof(float), s, logits, ld, target, rows, (int)C, ignore_index, top, group,    \
-                     vecs, magic, top_index, (const float2*)stats, entropy, g_logprob, g_logprob_stride, g_entropy,               \
-                     g_entropy_stride, g_top, dlogits, ldd)
+  hipLaunchKernelGGL(logprob_bwd_rows_kernel<T>, grid, block, (size_t)group * top * sizeof(float), s, logits, ld, target, rows,   \
+                     (int)C, ignore_index, top, group, vecs, magic, top_index, (const float2*)stats, entropy, g_logprob,          \
+                     g_logprob_stride, g_entropy, g_entropy_stride, g_top, dlogits, ldd)
     if (dtype == 0) CCN_LP_BWD(0);
     else if (dtype == 1) CCN_LP_BWD(1);
     else CCN_LP_BWD(2);
 #undef CCN_LP_BWD
   } else {
-    const int64_t tiles = (C + LP_TPB * LP_HOLD - 1) / (LP_TPB * LP_HOLD);
-    CCN_REQUIRE(rows * tiles < ((int64_t)1 << 31), "logprob_bwd: rows=%lld C=%lld: too many for one launch", (long long)rows,
-                (long long)C);
+    const int64_t tiles = lp_tiles(C);
     const dim3 grid((unsigned)(rows * tiles)), block(LP_TPB);
 #define CCN_LP_BWD(T)                                                                                                             \
   hipLaunchKernelGGL(logprob_bwd_wide_kernel<T>, grid, block, 0, s, logits, ld, target, (int)C, ignore_index, top, (int)tiles,     \
@@ -964,5 +935,65 @@ extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const 
 #undef CCN_LP_BWD
   }
   CCN_LAUNCH_OK("logprob_bwd");
+  return CCN_OK;
+}
+
+}  // namespace
+
+extern "C" size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top) {
+  if (rows <= 0 || C <= LP_NARROW || top < 0) return 0;
+  const LpPlan p = lp_plan(rows, C, top);
+  if (p.parts == 1) return 0;
+  return ccn_align256((size_t)rows * p.parts * sizeof(float4)) + ccn_align256((size_t)rows * p.parts * top * sizeof(uint64_t));
+}
+
+extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C,
+                               int64_t ignore_index, int top, float* logprob, float* entropy, float* stats, float* top_logprob,
+                               int64_t* top_index, void* ws, size_t ws_bytes, void* stream) {
+  CCN_REQUIRE(logits && target && logprob && entropy, "logprob_fwd: null pointer");
+  CCN_REQUIRE((uintptr_t)stats % 8 == 0, "logprob_fwd: stats are not 8-byte aligned");
+  CCN_REQUIRE(dtype >= 0 && dtype <= 2, "logprob_fwd: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
+  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 30) && (ld >= C || rows == 1),
+              "logprob_fwd: rows=%lld C=%lld ld=%lld", (long long)rows, (long long)C, (long long)ld);
+  CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_fwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
+  CCN_REQUIRE(top == 0 || (top_logprob && top_index), "logprob_fwd: top > 0 without its outputs");
+  const LpPlan p = lp_plan(rows, C, top);
+  const size_t need = ccn_logprob_workspace_bytes(rows, C, top);
+  if (need && (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < need)) {
+    ccn_set_error("logprob_fwd: workspace of %zu bytes, %zu are needed (16-byte aligned)", ws ? ws_bytes : (size_t)0, need);
+    return CCN_ERR_WORKSPACE;
+  }
+  for (int64_t r = 0; r < rows; r += LP_LAUNCH_ROWS) {
+    const int rc = lp_fwd(lp_row(logits, dtype, r * ld), dtype, ld, target + r, rows - r < LP_LAUNCH_ROWS ? rows - r : LP_LAUNCH_ROWS, C,
+                          ignore_index, top, p, logprob + r, entropy + r, stats ? stats + 2 * r : nullptr,
+                          top ? top_logprob + r * top : nullptr, top ? top_index + r * top : nullptr, need ? ws : nullptr,
+                          (hipStream_t)stream);
+    if (rc) return rc;
+  }
+  return CCN_OK;
+}
+
+extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C,
+                               int64_t ignore_index, int top, const int64_t* top_index, const float* stats, const float* entropy,
+                               const float* g_logprob, int64_t g_logprob_stride, const float* g_entropy, int64_t g_entropy_stride,
+                               const float* g_top, void* dlogits, int64_t ldd, void* stream) {
+  CCN_REQUIRE(logits && target && stats && entropy && dlogits, "logprob_bwd: null pointer");
+  CCN_REQUIRE((uintptr_t)stats % 8 == 0, "logprob_bwd: stats are not 8-byte aligned");
+  CCN_REQUIRE(dtype >= 0 && dtype <= 2, "logprob_bwd: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", dtype);
+  CCN_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && C > 0 && C < ((int64_t)1 << 30) && (ld >= C || rows == 1) &&
+              (ldd >= C || rows == 1), "logprob_bwd: rows=%lld C=%lld ld=%lld ldd=%lld", (long long)rows, (long long)C,
+              (long long)ld, (long long)ldd);
+  CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_bwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
+  CCN_REQUIRE(top == 0 || (g_top && top_index), "logprob_bwd: top > 0 without its gradient and classes");
+  CCN_REQUIRE(g_logprob_stride >= 0 && g_entropy_stride >= 0, "logprob_bwd: negative gradient stride");
+  const int64_t most = C <= LP_GROUP_MAX ? LP_LAUNCH_ROWS : (LP_LAUNCH_ROWS + lp_tiles(C) - 1) / lp_tiles(C);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int rc = lp_bwd(lp_row(logits, dtype, r * ld), dtype, ld, target + r, rows - r < most ? rows - r : most, C, ignore_index, top,
+                          top ? top_index + r * top : nullptr, stats + 2 * r, entropy + r,
+                          g_logprob ? g_logprob + r * g_logprob_stride : nullptr, g_logprob_stride,
+                          g_entropy ? g_entropy + r * g_entropy_stride : nullptr, g_entropy_stride, top ? g_top + r * top : nullptr,
+                          const_cast<void*>(lp_row(dlogits, dtype, r * ldd)), ldd, (hipStream_t)stream);
+    if (rc) return rc;
+  }
   return CCN_OK;
 }

@@ -190,10 +190,11 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& target, int64_t top
   if (x.is_neg()) x = x.resolve_neg();
   // (one row: its stride is never used, and torch may report any)
   if ((x.stride(1) != 1 && c > 1) || (rows > 1 && x.stride(0) < c)) x = x.contiguous();
-  Tensor t = target;
+  Tensor t = target.is_neg() ? target.resolve_neg() : target;
   if (!flat || t.scalar_type() != at::kLong || !t.is_contiguous()) t = t.reshape({rows}).to(at::kLong).contiguous();
   Tensor logprob, entropy, best, index;
-  if (logits.requires_grad() && at::GradMode::is_enabled()) {
+  // (a tangent of forward mode goes the same way: the node refuses it)
+  if ((logits.requires_grad() && at::GradMode::is_enabled()) || logits._fw_grad(0).defined()) {
     const auto out = TokenLogProbs::apply(x, t, top, ignore);
     logprob = out[0];
     entropy = out[1];
@@ -234,7 +235,7 @@ struct Table {
   int64_t n() const { return (int64_t)at.size(); }
 };
 
-Table table_of(const std::vector<Tensor>& tensors, const char* who) {
+Table table_of(const std::vector<Tensor>& tensors, const char* who, bool writes) {
   Table t;
   t.at.reserve(tensors.size());
   t.size.reserve(tensors.size());
@@ -246,7 +247,7 @@ Table table_of(const std::vector<Tensor>& tensors, const char* who) {
     TORCH_CHECK_VALUE(x.is_non_overlapping_and_dense(), who, ": a tensor of strides ", x.strides(), " does not fill its memory");
     require_gpu(x);
     TORCH_CHECK_VALUE(x.device() == tensors[0].device(), who, ": tensors on ", tensors[0].device().str(), " and ", x.device().str());
-    t.at.push_back(x.const_data_ptr());
+    t.at.push_back(writes ? x.mutable_data_ptr() : x.const_data_ptr());
     t.size.push_back(x.numel());
     t.code.push_back(code);
     t.total += x.numel();
@@ -272,7 +273,7 @@ void moved(const std::vector<Tensor>& tensors) {             // written behind t
 }
 
 Tensor grad_norm(const std::vector<Tensor>& tensors, int kind) {
-  const Table t = table_of(tensors, "grad_norm");
+  const Table t = table_of(tensors, "grad_norm", false);
   NormOut o(t);
   launch("grad_norm", {t.n(), kind, o.bytes}, t.total, [&] {
     return entry.grad_norm(t.at.data(), t.size.data(), t.code.data(), t.n(), kind, o.ws.mutable_data_ptr(), (size_t)o.bytes,
@@ -294,7 +295,7 @@ std::vector<Tensor> grads_of(const std::vector<Tensor>& parameters) {
 py::object clip_grad_norm(const std::vector<Tensor>& parameters, int kind, double max_norm) {
   const std::vector<Tensor> grads = grads_of(parameters);
   if (grads.empty()) return py::none();
-  const Table t = table_of(grads, "clip_grad_norm_");
+  const Table t = table_of(grads, "clip_grad_norm_", true);
   NormOut o(t);
   launch("grad_clip", {t.n(), kind, o.bytes}, t.total, [&] {
     return entry.grad_clip(const_cast<void* const*>(t.at.data()), t.size.data(), t.code.data(), t.n(), kind, max_norm,
@@ -328,7 +329,7 @@ py::object adam_step(const std::vector<Tensor>& params, const std::vector<Tensor
       TORCH_CHECK_VALUE((uintptr_t)t.const_data_ptr() % 16 == 0, "adam_step_: a tensor does not start at a multiple of 16 bytes");
     }
   Table t[4];
-  for (int k = 0; k < 4; ++k) t[k] = table_of(*lists[k], "adam_step_");
+  for (int k = 0; k < 4; ++k) t[k] = table_of(*lists[k], "adam_step_", k != 1);
   py::object norm = py::none();
   if (max_norm) {
     NormOut o(t[1]);

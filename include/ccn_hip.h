@@ -706,7 +706,7 @@ int ccn_adam_step(float* param, const float* grad, float* exp_avg, float* exp_av
  * logits: rows x C of `dtype` (0 = fp32, 1 = bf16, 2 = fp16), row stride ld elements (any alignment of the type).  Outputs fp32.
  * C < 2^30, rows < 2^31.
  * fwd: logprob (rows) of target (0 where target == ignore_index, NaN for another target outside [0, C)), entropy (rows), stats
- * (2 x rows, nullable: what bwd needs), top_logprob / top_index (rows x top, the `top` largest logits, equal ones by ascending
+ * (2 x rows, 8-byte aligned, nullable: what bwd needs), top_logprob / top_index (rows x top, the `top` largest logits, equal ones by ascending
  * class; top <= 64, top <= C).  A row of -inf only: logprob -inf, entropy 0.
  * bwd: dlogits (`dtype`, row stride ldd) = d / d logits of sum(g_logprob logprob) + sum(g_entropy entropy) + sum(g_top top_logprob);
  * g_logprob and g_entropy are read at row * their stride (0: one value for all rows) and may be null, g_top is rows x top.
@@ -724,9 +724,11 @@ int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const int64_t* ta
 /* The global norm of n gradients and their clipping.  grads / sizes / dtypes are HOST arrays (addresses of device buffers, their
  * lengths in values, 0 = fp32 | 1 = bf16 | 2 = fp16; dtypes may be null: all fp32); they are read before the call returns.  kind: 1 =
  * sum of magnitudes, 2 = square root of the sum of squares, 3 = largest magnitude.  norm: fp32 device scalar, the norm BEFORE
- * clipping.  clip: every value times min(1, max_norm / (norm + 1e-6)), in place; tensors that share memory are refused.
+ * clipping.  clip: every value times min(1, max_norm / (norm + 1e-6)), in place, the factor rounded to the tensor's type first
+ * (fp16: unless it is below 2^-14); tensors that share memory are refused.
  * adam_clip: torch.optim.Adam(amsgrad=False, maximize=False) over n runs of parameters (fp32, 16-byte aligned) with the gradients
- * scaled the same way as they are read; they are not written.  Norms are summed in double in a fixed order.  ws: ccn_grad_norm_workspace_bytes(n) of device memory. */
+ * scaled the same way as they are read; they are not written.  Norms are summed in double in a fixed order.
+ * ws: ccn_grad_norm_workspace_bytes(n) of device memory. */
 size_t ccn_grad_norm_workspace_bytes(int64_t n);
 int ccn_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, void* ws,
                   size_t ws_bytes, float* norm, void* stream);

@@ -198,6 +198,31 @@ def test_same_bits_as_torch():
         assert all(torch.equal(a.grad, b.grad) for a, b in zip(p, q))
 
 
+def test_small_factors_of_fp16():
+    """A factor below 2^-14 is no normal fp16 number: rounded to one it would be off by up to all of itself.  In 32 bits a value is off by
+    the norm's and the factor's roundings (2 u), the product's (u) and half a step of its type, 2^-25 at least."""
+    from curvecloudnet_amd.parallel import clip_grad_norm_
+    for bound in (1e-4, 2e-3, 0.03, 0.9):
+        (p,) = _params([(100000,)], [torch.float16])
+        before = p.grad.mul_(300).double()
+        norm = clip_grad_norm_([p], bound)
+        ref = before * (bound / (float(before.square().sum().sqrt()) + 1e-6))
+        assert float(norm) > 5e4 and bound / float(norm) < 2.0 ** -14
+        off = (p.grad.double() - ref).abs()
+        assert bool((off <= ref.abs() * (2.0 ** -11 + 4 * U) + 2.0 ** -25).all())
+    assert float(p.grad.abs().max()) > 0
+
+
+def test_gradients_whose_memory_is_not_their_own_yet():
+    from curvecloudnet_amd.parallel import clip_grad_norm_
+    (p,) = _params([(1000,)], [torch.float32])
+    origin = p.grad
+    before = origin.clone()
+    p.grad = torch._lazy_clone(origin)                                  # (copied when it is first written)
+    clip_grad_norm_([p], 0.5)
+    assert torch.equal(origin, before) and not torch.equal(p.grad, before)
+
+
 def test_versions_move_and_neighbours_stay():
     from curvecloudnet_amd.parallel import clip_grad_norm_
     buf = torch.ones(3000, device=DEV)

@@ -524,3 +524,34 @@ def test_other_kinds_of_tensors():
         leaf.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         r.logprob.sum().backward()
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as forward
+    x, t = _logits(4, 30, torch.float32), _target(4, 30)
+    with forward.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+        _score(forward.make_dual(x, torch.ones_like(x)), t)
+
+
+@pytest.mark.parametrize("c,top", [(3, 2), (33, 2), (600, 0), (4097, 0)])
+def test_more_rows_than_a_launch_holds(c, top):
+    rows, border = (1 << 22) + 5, 1 << 22
+    x = torch.zeros(rows, c, dtype=torch.float16, device=DEV)
+    t = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    for at in (0, border - 4):                                          # (the first rows, and those on both sides of the border)
+        x[at: at + 9] = _logits(9, c, torch.float16, seed=at)
+        t[at: at + 9] = _target(9, c, seed=at)
+    x.requires_grad_(True)
+    r = _score(x, t, top=top)
+    (d,) = torch.autograd.grad(r.logprob.sum() + 2 * r.entropy.sum(), x)
+    for at in (0, border - 4):
+        part = slice(at, at + 9)
+        small = x.detach()[part].clone().requires_grad_(True)
+        q = _score(small, t[part], top=top)
+        _check(small, t[part], top, r=q)
+        (e,) = torch.autograd.grad(q.logprob.sum() + 2 * q.entropy.sum(), small)
+        assert torch.equal(d[part], e)
+        assert all(torch.equal(a[part], b) for a, b in zip(r, q) if a is not None)
+    rest = r.logprob.detach()[9: border - 4]
+    _near(rest[:: 1 << 18], torch.full((rest[:: 1 << 18].numel(),), -math.log(c)), _e(torch.tensor(math.log(c)), c), "rows of zeros")
+    assert bool((rest == rest[0]).all())

@@ -101,7 +101,8 @@ def test_c_entries_of_the_scores_refuse():
                        (lambda: bwd(x=null), "null"), (lambda: bwd(stats=null), "null"), (lambda: bwd(d=null), "null"),
                        (lambda: bwd(dtype=7), "dtype"), (lambda: bwd(ldd=7), "ldd"), (lambda: bwd(ld=7), "ld"), (lambda: bwd(rows=-1), "rows"),
                        (lambda: bwd(top=2, gt=null), "top"), (lambda: bwd(top=2, index=null), "top"), (lambda: bwd(top=9), "top"),
-                       (lambda: bwd(s1=-1), "stride"), (lambda: bwd(s2=-1), "stride")):
+                       (lambda: bwd(s1=-1), "stride"), (lambda: bwd(s2=-1), "stride"),
+                       (lambda: bwd(stats=ctypes.c_void_p(0x1004)), "stats")):
         assert call() < 0 and word in err(), (word, err())
     sizes = [(r, c, k) for r in (1, 96, 1 << 20) for c in (1, 64, 65, 50021, 262144, (1 << 30) - 1) for k in (0, 64)]
     assert all(0 <= lib.ccn_logprob_workspace_bytes(*s) < 1 << 42 for s in sizes)
