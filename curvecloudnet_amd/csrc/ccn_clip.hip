@@ -156,12 +156,15 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double*
 // for half a step of the type more than with the factor in 32 bits.  Below the normal numbers of fp16, where half a step can be all of
 // the factor (a norm of 10^7 and a bound of 0.1), it stays in 32 bits.
 template <int T>
+__device__ __forceinline__ float clip_factor_of(float scale) {
+  if (T == 2 && scale < 0x1p-14f) return scale;
+  ccn_u32x4 of_type = {0, 0, 0, 0};
+  put16<T>(of_type, 0, scale);
+  return get16<T>(of_type, 0);
+}
+template <int T>
 __device__ __forceinline__ void clip_apply(char* p, int n, float scale) {
-  if (T != 2 || !(scale < 0x1p-14f)) {
-    ccn_u32x4 of_type = {0, 0, 0, 0};
-    put16<T>(of_type, 0, scale);
-    scale = get16<T>(of_type, 0);
-  }
+  scale = clip_factor_of<T>(scale);
   constexpr int V = CcnVec16<T>::N, STEP = CLIP_TPB * V, U = 4;
   for (int i = threadIdx.x * V; i - (int)threadIdx.x * V < n; i += U * STEP) {
     ccn_u32x4 r[U];
@@ -206,6 +209,92 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, 
     else if (type == 1) clip_apply<1>(p, n, scale);
     else clip_apply<2>(p, n, scale);
   }
+}
+
+// ---- few values (pieces of SMALL_PIECE of a tensor, two to a wave at most): one workgroup keeps them in registers between the norm and
+// the product, one launch does both.  max_norm < 0: the norm alone.
+constexpr int SMALL_TPB = 1024, SMALL_PIECE = 2048, SMALL_EACH = 2, SMALL_MAX = SMALL_EACH * SMALL_TPB / 64;
+static_assert(SMALL_MAX <= 64, "found by one look of a wave");
+
+struct SmallHeld {
+  ccn_u32x4 whole[SMALL_PIECE / 256];
+  float rest;                                      // (a lane's share of the values behind the last 16 whole bytes)
+};
+template <int KIND, int T>
+__device__ __forceinline__ void small_read(ClipAcc<KIND>& a, SmallHeld& h, const char* p, int n) {
+  constexpr int V = CcnVec16<T>::N, NJ = SMALL_PIECE / 64 / V;
+  const int lane = threadIdx.x & 63, whole = n / V * V;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    h.whole[j] = ccn_u32x4{0, 0, 0, 0};
+    if ((j * 64 + lane) * V < whole) h.whole[j] = ld16<T>(p, (j * 64 + lane) * V);
+  }
+  h.rest = lane < n - whole ? ld_el<T>(p, whole + lane) : 0.f;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+    if (j * 64 * V < whole) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) clip_add<KIND, T>(a, get16<T>(h.whole[j], k));
+    }
+  clip_add<KIND, T>(a, h.rest);
+}
+template <int T>
+__device__ __forceinline__ void small_write(const SmallHeld& h, char* p, int n, float scale) {
+  constexpr int V = CcnVec16<T>::N, NJ = SMALL_PIECE / 64 / V;
+  const int lane = threadIdx.x & 63, whole = n / V * V;
+  scale = clip_factor_of<T>(scale);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+    if ((j * 64 + lane) * V < whole) {
+      ccn_u32x4 o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) put16<T>(o, k, get16<T>(h.whole[j], k) * scale);
+      st16<T>(p, (j * 64 + lane) * V, o);
+    }
+  if (lane < n - whole) st_el<T>(p, whole + lane, h.rest * scale);
+}
+
+template <int KIND>
+__global__ __launch_bounds__(SMALL_TPB) void grad_small_kernel(const ClipTable t, double max_norm, float* __restrict__ norm) {
+  __shared__ double red[SMALL_TPB / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pieces = t.first[t.n];
+  SmallHeld held[SMALL_EACH];
+  char* p[SMALL_EACH];
+  int n[SMALL_EACH], type[SMALL_EACH];
+  ClipAcc<KIND> a;
+#pragma unroll
+  for (int u = 0; u < SMALL_EACH; ++u) {
+    const int c = wave + u * (SMALL_TPB / 64);
+    n[u] = type[u] = 0;
+    p[u] = nullptr;
+    if (c < pieces) {
+      const int i = __builtin_amdgcn_readfirstlane(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < t.n && t.first[lane] <= c))) - 1;
+      const uint64_t at = t.at[i];
+      n[u] = c + 1 == t.first[i + 1] ? (int)((at >> 48) & 0x3fff) + 1 : SMALL_PIECE;
+      type[u] = (int)(at >> 62);
+      p[u] = reinterpret_cast<char*>(at & 0xffffffffffffull) + (c - t.first[i]) * SMALL_PIECE * (type[u] ? 2 : 4);
+      if (type[u] == 0) small_read<KIND, 0>(a, held[u], p[u], n[u]);
+      else if (type[u] == 1) small_read<KIND, 1>(a, held[u], p[u], n[u]);
+      else small_read<KIND, 2>(a, held[u], p[u], n[u]);
+    }
+  }
+  double v = ccn_wave_join(clip_value<KIND>(a), [](double x, double y) { return clip_join<KIND>(x, y); });
+  if (lane == 0) red[wave] = v;
+  __syncthreads();
+  v = red[0];
+  for (int k = 1; k < SMALL_TPB / 64; ++k) v = clip_join<KIND>(v, red[k]);
+  if (KIND == NORM_TWO) v = sqrt(v);
+  if (threadIdx.x == 0) *norm = (float)v;
+  if (max_norm < 0.0) return;
+  const float scale = clip_scale(v, max_norm);
+  if (scale == 1.f) return;
+#pragma unroll
+  for (int u = 0; u < SMALL_EACH; ++u)
+    if (n[u]) {
+      if (type[u] == 0) small_write<0>(held[u], p[u], n[u], scale);
+      else if (type[u] == 1) small_write<1>(held[u], p[u], n[u], scale);
+      else small_write<2>(held[u], p[u], n[u], scale);
+    }
 }
 
 // ---- Adam over several runs of parameters with the gradients scaled on the way
@@ -309,15 +398,15 @@ int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype
 int clip_chunks(int64_t size, int chunk) { return (int)((size + chunk - 1) / chunk); }
 
 // The tables of the launches that a list of tensors takes: f(table) for each.
-template <typename F>
+template <int CHUNK = CLIP_CHUNK, typename F>
 int clip_tables(const void* const* ptr, const int64_t* size, const int32_t* dtype, int64_t n, F f) {
   ClipTable t;
   t.n = 0;
   t.first[0] = 0;
   for (int64_t i = 0; i < n; ++i) {
     if (size[i] == 0) continue;
-    t.at[t.n] = (uint64_t)(uintptr_t)ptr[i] | ((uint64_t)((size[i] - 1) % CLIP_CHUNK) << 48) | ((uint64_t)(dtype ? dtype[i] : 0) << 62);
-    t.first[t.n + 1] = t.first[t.n] + clip_chunks(size[i], CLIP_CHUNK);
+    t.at[t.n] = (uint64_t)(uintptr_t)ptr[i] | ((uint64_t)((size[i] - 1) % CHUNK) << 48) | ((uint64_t)(dtype ? dtype[i] : 0) << 62);
+    t.first[t.n + 1] = t.first[t.n] + clip_chunks(size[i], CHUNK);
     if (++t.n == CLIP_MAX) {
       if (int rc = f(t)) return rc;
       t.n = 0;
@@ -343,6 +432,20 @@ int clip_norm_launches(const void* const* ptr, const int64_t* size, const int32_
     const int grid = clip_grid(t.first[t.n], CLIP_PART_MAX);
     CLIP_KINDS(kind, grad_norm_kernel, dim3(grid), dim3(CLIP_TPB), 0, s, t, partial + *count);
     *count += grid;
+    return CCN_OK;
+  });
+}
+
+// Whether grad_small_kernel does it all.
+bool clip_is_small(const int64_t* size, int64_t n) {
+  int64_t pieces = 0;
+  for (int64_t i = 0; i < n && pieces <= SMALL_MAX; ++i) pieces += (size[i] + SMALL_PIECE - 1) / SMALL_PIECE;
+  return pieces > 0 && pieces <= SMALL_MAX;
+}
+int clip_small(const void* const* ptr, const int64_t* size, const int32_t* dtype, int64_t n, int kind, double max_norm, float* norm,
+               hipStream_t s) {
+  return clip_tables<SMALL_PIECE>(ptr, size, dtype, n, [&](const ClipTable& t) {
+    CLIP_KINDS(kind, grad_small_kernel, dim3(1), dim3(SMALL_TPB), 0, s, t, max_norm, norm);
     return CCN_OK;
   });
 }
@@ -382,6 +485,11 @@ extern "C" int ccn_grad_norm(const void* const* grads, const int64_t* sizes, con
   double* const partial = (double*)ws;
   int count = 0;
   hipStream_t s = (hipStream_t)stream;
+  if (clip_is_small(sizes, n)) {
+    if (int rc = clip_small(grads, sizes, dtypes, n, kind, -1.0, norm, s)) return rc;
+    CCN_LAUNCH_OK("grad_norm");
+    return CCN_OK;
+  }
   if (int rc = clip_norm_launches(grads, sizes, dtypes, n, kind, partial, &count, s)) return rc;
   CLIP_KINDS(kind, grad_norm_final_kernel, dim3(1), dim3(CLIP_TPB), 0, s, partial, count, 0.0, norm, nullptr);
   CCN_LAUNCH_OK("grad_norm");
@@ -399,6 +507,11 @@ extern "C" int ccn_grad_clip(void* const* grads, const int64_t* sizes, const int
   int64_t chunks = 0;
   for (int64_t i = 0; i < n; ++i) chunks += clip_chunks(sizes[i], CLIP_CHUNK);
   hipStream_t s = (hipStream_t)stream;
+  if (clip_is_small(sizes, n)) {
+    if (int rc = clip_small(grads, sizes, dtypes, n, kind, max_norm, norm, s)) return rc;
+    CCN_LAUNCH_OK("grad_clip");
+    return CCN_OK;
+  }
   if (int rc = clip_norm_launches(grads, sizes, dtypes, n, kind, partial, &count, s)) return rc;
   const float* const factor = clip_factor(kind, partial, count, max_norm, norm, chunks, s);
   float* out = factor ? nullptr : norm;

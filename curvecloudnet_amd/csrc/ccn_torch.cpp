@@ -7,6 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
 #include <cmath>
@@ -241,16 +242,18 @@ Table table_of(const std::vector<Tensor>& tensors, const char* who, bool writes)
   t.size.reserve(tensors.size());
   t.code.reserve(tensors.size());
   for (const Tensor& x : tensors) {
-    TORCH_CHECK_TYPE(x.layout() == at::kStrided, who, ": sparse tensors are not built");
+    c10::TensorImpl* const impl = x.unsafeGetTensorImpl();
+    TORCH_CHECK_TYPE(impl->layout() == at::kStrided, who, ": sparse tensors are not built");
     const int code = code_of(x.scalar_type());
     TORCH_CHECK_TYPE(code >= 0, who, ": ", name_of(x.scalar_type()), "; fp32, bf16 or fp16 is wanted");
-    TORCH_CHECK_VALUE(x.is_non_overlapping_and_dense(), who, ": a tensor of strides ", x.strides(), " does not fill its memory");
+    TORCH_CHECK_VALUE(impl->is_non_overlapping_and_dense(), who, ": a tensor of strides ", x.strides(), " does not fill its memory");
     require_gpu(x);
-    TORCH_CHECK_VALUE(x.device() == tensors[0].device(), who, ": tensors on ", tensors[0].device().str(), " and ", x.device().str());
-    t.at.push_back(writes ? x.mutable_data_ptr() : x.const_data_ptr());
-    t.size.push_back(x.numel());
+    TORCH_CHECK_VALUE(impl->device() == tensors[0].device(), who, ": tensors on ", tensors[0].device().str(), " and ", x.device().str());
+    const int64_t size = impl->numel();
+    t.at.push_back(writes ? impl->mutable_data() : impl->data());
+    t.size.push_back(size);
     t.code.push_back(code);
-    t.total += x.numel();
+    t.total += size;
   }
   t.one = tensors[0];
   return t;
@@ -272,7 +275,17 @@ void moved(const std::vector<Tensor>& tensors) {             // written behind t
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-Tensor grad_norm(const std::vector<Tensor>& tensors, int kind) {
+// The i-th of a list; hundreds are looked at in place, without one Python object or count of references more than it takes.
+const Tensor& tensor_at(const py::list& list, size_t i, const char* who) {
+  PyObject* const o = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
+  TORCH_CHECK_TYPE(THPVariable_Check(o), who, ": ", Py_TYPE(o)->tp_name, " is no tensor");
+  return THPVariable_Unpack(o);
+}
+
+Tensor grad_norm(const py::list& list, int kind) {
+  std::vector<Tensor> tensors;
+  tensors.reserve(list.size());
+  for (size_t i = 0; i < list.size(); ++i) tensors.push_back(tensor_at(list, i, "grad_norm"));
   const Table t = table_of(tensors, "grad_norm", false);
   NormOut o(t);
   launch("grad_norm", {t.n(), kind, o.bytes}, t.total, [&] {
@@ -283,16 +296,18 @@ Tensor grad_norm(const std::vector<Tensor>& tensors, int kind) {
 }
 
 // The gradients of `parameters`, those that have one.
-std::vector<Tensor> grads_of(const std::vector<Tensor>& parameters) {
+std::vector<Tensor> grads_of(const py::list& parameters) {
   std::vector<Tensor> grads;
   grads.reserve(parameters.size());
-  for (const Tensor& p : parameters)
-    if (p.grad().defined()) grads.push_back(p.grad());
+  for (size_t i = 0; i < parameters.size(); ++i) {
+    const Tensor& g = tensor_at(parameters, i, "clip_grad_norm_").unsafeGetTensorImpl()->grad();
+    if (g.defined()) grads.push_back(g);
+  }
   return grads;
 }
 
 // None where no parameter has a gradient.
-py::object clip_grad_norm(const std::vector<Tensor>& parameters, int kind, double max_norm) {
+py::object clip_grad_norm(const py::list& parameters, int kind, double max_norm) {
   const std::vector<Tensor> grads = grads_of(parameters);
   if (grads.empty()) return py::none();
   const Table t = table_of(grads, "clip_grad_norm_", true);
