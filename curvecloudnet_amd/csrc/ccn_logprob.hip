@@ -281,9 +281,10 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
     if (TOP) {
       const bool first = c0 == beg;
       if (first) limit = lp_limit<NW>(tm, top, sh);
-      // the logits of this thread that are not below v, or that beat it (a NaN is and does)
+      // the logits of this thread that are not below v, or that beat it (a NaN is and does, but for a v of NaN, which none beats)
       auto reach = [&](float v, bool beat) {
         uint32_t some = 0;
+        if (beat && v != v) return some;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
           if (beat ? !(vm[j] <= v) : !(vm[j] < v)) {

@@ -306,6 +306,21 @@ def test_nan_and_infinity_stay_in_their_rows(c):
     assert torch.isfinite(d[[0, 5]]).all() and torch.isnan(d[1:5]).any(1).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["fp32", "fp16"])
+@pytest.mark.parametrize("c", [20, 100, 1500, 5000, 40000])
+def test_rows_of_many_nan(c, dtype):
+    """More of them than alternatives: everywhere, on odd classes, behind the first piece, in the last class and few before it."""
+    x, t = _logits(5, c, dtype), _target(5, c)
+    x[0] = math.nan
+    x[1, 1::2] = math.nan
+    x[2, c // 2:] = math.nan
+    x[3, -1] = x[3, c // 3] = math.nan
+    x[4, 0] = math.inf
+    x[4, 3::5] = math.nan
+    for top in (1, 3, min(c, 20)):
+        _check(x, t, top)
+
+
 def test_targets_that_are_not_scored():
     for c in (20, 65, 3000):
         rows = 9
