@@ -150,3 +150,12 @@ def test_c_entries_of_the_norm_refuse():
         assert call() < 0 and word in err(), (word, err())
     sizes = [lib.ccn_grad_norm_workspace_bytes(n) for n in (0, 1, 160, 161, 320, 321, 1000, 1 << 20)]
     assert sizes == sorted(sizes) and 0 < sizes[0] and sizes[-1] < 1 << 30 and lib.ccn_grad_norm_workspace_bytes(-1) == 0
+
+
+def test_lists_of_other_things_are_refused():
+    from curvecloudnet_amd.parallel import clip_grad_norm_, grad_norm
+    for bad in (1.0, None, "weight", [torch.zeros(3)]):
+        with pytest.raises(TypeError, match="is no tensor"):
+            grad_norm([bad])
+        with pytest.raises(TypeError, match="is no tensor"):
+            clip_grad_norm_([torch.nn.Parameter(torch.zeros(3)), bad], 1.0)
