@@ -378,11 +378,12 @@ int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype
     CCN_REQUIRE(!dtype || (dtype[i] >= 0 && dtype[i] <= 2), "%s: tensor %lld: dtype %d is not 0 (fp32), 1 (bf16) or 2 (fp16)", who,
                 (long long)i, dtype ? dtype[i] : 0);
     CCN_REQUIRE(size[i] >= 0 && size[i] < ((int64_t)1 << 36), "%s: tensor %lld has %lld values", who, (long long)i, (long long)size[i]);
-    CCN_REQUIRE(size[i] == 0 || (ptr[i] && (uintptr_t)ptr[i] % el == 0 && (uintptr_t)ptr[i] < (uintptr_t)1 << 48),
+    CCN_REQUIRE(size[i] == 0 || (ptr[i] && ((uintptr_t)ptr[i] & (uintptr_t)(el - 1)) == 0 && (uintptr_t)ptr[i] < (uintptr_t)1 << 48),
                 "%s: tensor %lld: null or not aligned to its type", who, (long long)i);
   }
   if (!writes) return CCN_OK;
-  bool ordered = true;                               // (tensors of one buffer mostly come in order)
+  int runs = 0;                                      // tensors of one buffer mostly come in order: few ascending runs are merged
+  size_t run[8];                                     // (where the second and later ones start)
   std::vector<std::pair<uintptr_t, uintptr_t>> span;
   try {
     span.reserve((size_t)n);
@@ -393,10 +394,13 @@ int clip_check(const void* const* ptr, const int64_t* size, const int32_t* dtype
   for (int64_t i = 0; i < n; ++i) {
     if (size[i] == 0) continue;
     const uintptr_t a = (uintptr_t)ptr[i], b = a + (uintptr_t)size[i] * (dtype && dtype[i] ? 2 : 4);
-    ordered = ordered && (span.empty() || span.back().first <= a);
+    if (!span.empty() && a < span.back().first && runs++ < 8) run[runs - 1] = span.size();
     span.emplace_back(a, b);
   }
-  if (!ordered) std::sort(span.begin(), span.end());
+  if (runs > 8) std::sort(span.begin(), span.end());
+  else
+    for (int k = 0; k < runs; ++k)
+      std::inplace_merge(span.begin(), span.begin() + run[k], k + 1 < runs ? span.begin() + run[k + 1] : span.end());
   for (size_t i = 1; i < span.size(); ++i)
     CCN_REQUIRE(span[i - 1].second <= span[i].first, "%s: two of the tensors share memory (the same one given twice?)", who);
   return CCN_OK;
@@ -545,14 +549,16 @@ extern "C" int ccn_adam_clip(float* const* params, const float* const* grads, fl
   std::vector<int64_t> every;
   int64_t chunks = 0;
   try {                                              // nothing that is written may share memory with anything else that is used
-    for (int64_t i = 0; i < n; ++i) {
-      chunks += clip_chunks(sizes[i], ADAM_CHUNK);
-      for (const void* p : {(const void*)params[i], (const void*)grads[i], (const void*)exp_avgs[i], (const void*)exp_avg_sqs[i]}) {
-        CCN_REQUIRE((uintptr_t)p % 16 == 0, "adam_clip: buffers must be 16-byte aligned");
-        all.push_back(p);
+    all.reserve((size_t)(4 * n));
+    every.reserve((size_t)(4 * n));
+    for (const void* const* list : {(const void* const*)params, (const void* const*)grads, (const void* const*)exp_avgs,
+                                    (const void* const*)exp_avg_sqs})
+      for (int64_t i = 0; i < n; ++i) {
+        CCN_REQUIRE((uintptr_t)list[i] % 16 == 0, "adam_clip: buffers must be 16-byte aligned");
+        all.push_back(list[i]);
         every.push_back(sizes[i]);
       }
-    }
+    for (int64_t i = 0; i < n; ++i) chunks += clip_chunks(sizes[i], ADAM_CHUNK);
   } catch (...) {
     ccn_set_error("adam_clip: out of host memory");
     return CCN_ERR_ARG;

@@ -282,10 +282,15 @@ const Tensor& tensor_at(const py::list& list, size_t i, const char* who) {
   return THPVariable_Unpack(o);
 }
 
-Tensor grad_norm(const py::list& list, int kind) {
+std::vector<Tensor> tensors_of(const py::list& list, const char* who) {
   std::vector<Tensor> tensors;
   tensors.reserve(list.size());
-  for (size_t i = 0; i < list.size(); ++i) tensors.push_back(tensor_at(list, i, "grad_norm"));
+  for (size_t i = 0; i < list.size(); ++i) tensors.push_back(tensor_at(list, i, who));
+  return tensors;
+}
+
+Tensor grad_norm(const py::list& list, int kind) {
+  const std::vector<Tensor> tensors = tensors_of(list, "grad_norm");
   const Table t = table_of(tensors, "grad_norm", false);
   NormOut o(t);
   launch("grad_norm", {t.n(), kind, o.bytes}, t.total, [&] {
@@ -322,9 +327,10 @@ py::object clip_grad_norm(const py::list& parameters, int kind, double max_norm)
 
 // ---- the update
 
-py::object adam_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs,
-                     const std::vector<Tensor>& exp_avg_sqs, int64_t step, double lr, double beta1, double beta2, double eps,
-                     double weight_decay, std::optional<double> max_norm) {
+py::object adam_step(const py::list& of_params, const py::list& of_grads, const py::list& of_exp_avgs, const py::list& of_exp_avg_sqs,
+                     int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay, std::optional<double> max_norm) {
+  const std::vector<Tensor> params = tensors_of(of_params, "adam_step_"), grads = tensors_of(of_grads, "adam_step_"),
+                            exp_avgs = tensors_of(of_exp_avgs, "adam_step_"), exp_avg_sqs = tensors_of(of_exp_avg_sqs, "adam_step_");
   const std::vector<Tensor>* lists[4] = {&params, &grads, &exp_avgs, &exp_avg_sqs};
   for (int k = 1; k < 4; ++k)
     TORCH_CHECK_VALUE(lists[k]->size() == params.size(), "adam_step_: ", params.size(), " parameters, ", grads.size(), " gradients, ",
