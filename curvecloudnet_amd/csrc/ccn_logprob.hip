@@ -42,6 +42,20 @@ __device__ __forceinline__ float lp_key_value(uint64_t k) {
   const uint32_t b = (uint32_t)(k >> 32);
   return __uint_as_float((b & 0x80000000u) ? (b & 0x7fffffffu) : ~b);
 }
+// The same order for the i-th 16-bit value of r, in 16 bits.
+template <int T>
+__device__ __forceinline__ uint32_t lp_key16(const ccn_u32x4& r, int i) {
+  constexpr uint32_t INF = T == 1 ? 0x7f80 : 0x7c00;
+  uint32_t h = (r[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+  if ((h & 0x7fffu) > INF) h = INF + 1;
+  if (h == 0x8000u) h = 0;
+  return h & 0x8000u ? h ^ 0xffffu : h | 0x8000u;
+}
+template <int T>
+__device__ __forceinline__ float lp_key16_value(uint32_t k) {
+  const uint32_t h = k & 0x8000u ? k & 0x7fffu : k ^ 0xffffu;
+  return T == 1 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
 __device__ __forceinline__ int64_t lp_key_class(uint64_t k) { return (int64_t)(uint32_t)~(uint32_t)k; }
 
 // The row's results from its statistics.  m: the maximum, NaN where a logit is.
@@ -481,7 +495,8 @@ __device__ __forceinline__ V lp_team(V v, F f) {
 // ---- rows of 25 to 512 classes: TEAM lanes hold a row in registers, 16 logits each, and join their results by lane moves; a
 // wave has 64 / TEAM rows.  Alternatives: `top` walks over the registers, each of which takes the largest logit that is left; TEAM of
 // them are kept, a lane each, and stored side by side.  220011 x 55 fp32: 14.0 us, 3.8 TB/s, half of it the latency of one round of loads;
-// with alternatives the walks bound it (100000 x 100 bf16 11 us, with 5 of them 23).
+// with alternatives the walks bound it, each of them 0.4 us for 100000 x 50 fp32 and 1.2 for 50000 x 256 (100000 x 100 bf16 10 us, with 5 of
+// them 20).
 template <int T, int TEAM, bool TOP>
 __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __restrict__ x, int64_t ld,
                                                               const int64_t* __restrict__ target, int64_t rows, int C,
@@ -524,40 +539,59 @@ __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __rest
     if (stats) stats[row] = make_float2(r.base, r.log_total);
   }
   if (!TOP) return;
-  int o[HOLD];                                       // the logits as whole numbers in the order of the alternatives
+  // the logits as whole numbers in the order of the alternatives; in 16 bits with the class below them, so that no two are equal
+  uint32_t o[HOLD];
 #pragma unroll
   for (int e = 0; e < HOLD; ++e) {
     const float v = get16<T>(raw[e / V], e % V);
-    int b = __float_as_int(v + 0.0f);
-    if (v != v) b = 0x7f800001;
-    o[e] = ((e / V) * TEAM + lane) * V + e % V < C ? b ^ ((b >> 31) & 0x7fffffff) : INT_MIN;
+    const int c = ((e / V) * TEAM + lane) * V + e % V;
+    o[e] = c >= C ? 0 : T == 0 ? (uint32_t)(lp_key(v, 0) >> 32) : lp_key16<T>(raw[e / V], e % V) << 16 | (0xffffu - c);
   }
+  uint32_t last = 0;
   float kept = 0.f;
   int kept_class = 0;
   for (int k = 0; k < top; ++k) {
-    int best = INT_MIN, at = 0;                      // (below every logit; taken ones become it)
+    uint32_t best = 0;                               // (below every logit; taken ones become it)
+    int c;
+    float value;
+    if constexpr (T == 0) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (j * TEAM * V < C) {
+      for (int j = 0; j < NJ; ++j)
+        if (j * TEAM * V < C) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          at = o[j * V + i] > best ? j * TEAM * V + i : at;
-          best = max(best, o[j * V + i]);
+          for (int i = 0; i < V; ++i) best = max(best, o[j * V + i]);
         }
-      }
-    // (value, then lower class, as one number)
-    uint64_t key = ((uint64_t)((uint32_t)best ^ 0x80000000u) << 32) | (uint32_t)~(at + lane * V);
-    key = lp_team<TEAM>(key, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-    const int c = (int)(uint32_t)~(uint32_t)key, own = c - lane * V;
-    best = (int)((uint32_t)(key >> 32) ^ 0x80000000u);
+      best = lp_team<TEAM>(best, [](uint32_t x, uint32_t y) { return max(x, y); });
+      int at = INT_MAX / 2;                          // the lowest class that has it
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (j * TEAM * V < C) {
+      for (int j = NJ - 1; j >= 0; --j)
+        if (j * TEAM * V < C) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[j * V + i] = own == j * TEAM * V + i ? INT_MIN : o[j * V + i];
-      }
+          for (int i = V - 1; i >= 0; --i) at = o[j * V + i] == best ? j * TEAM * V + i : at;
+        }
+      c = (int)lp_team<TEAM>((uint32_t)(at + lane * V), [](uint32_t x, uint32_t y) { return min(x, y); });
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        if (j * TEAM * V < C) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[j * V + i] = c - lane * V == j * TEAM * V + i ? 0 : o[j * V + i];
+        }
+      value = lp_key_value((uint64_t)best << 32);
+    } else {
+      // those below the last one wrap around when it is subtracted, and so are larger than those that are not: the largest difference is
+      // the next one's
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        if (j * TEAM * V < C) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) best = max(best, o[j * V + i] - last);
+        }
+      last += lp_team<TEAM>(best, [](uint32_t x, uint32_t y) { return max(x, y); });
+      c = 0xffff - (int)(last & 0xffffu);
+      value = lp_key16_value<T>(last >> 16);
+    }
     if (k % TEAM == lane) {
-      kept = (__int_as_float(best ^ ((best >> 31) & 0x7fffffff)) - r.base) - r.log_total;
+      kept = (value - r.base) - r.log_total;
       kept_class = c;
     }
     if (k % TEAM == TEAM - 1 || k == top - 1) {
@@ -801,12 +835,12 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
 }
 
 // Lanes to a row of logprob_team_kernel, 0 where the row is logprob_wide_kernel's: that one's way to the alternatives costs the same for
-// many of them (us, 50000 x 500 bf16 with 0 / 4 / 8 / 16 of them: 16 / 38 / 54 / 90 here and 28 / 64 / 66 / 68 there; 50000 x 256 fp32 with
-// 0 / 16 / 32: 12 / 49 / 85 and 23 / 60 / 64; 100000 x 100 bf16 with 0 / 45: 11 / 108 and 52 / 210).
-int lp_team_of(int64_t C, int top) {
+// many of them, and a walk here costs less in 16 bits (us, 50000 rows, here / there: 500 bf16 with 12 of them 44 / 57, with 20 58 / 60; 256 fp16
+// with 32 44 / 66; 500 fp32 with 8 53 / 58, with 12 70 / 61; 256 fp32 with 20 55 / 61).
+int lp_team_of(int64_t C, int top, bool wide_type) {
   if (C <= 64) return 4;
   if (C <= 128) return 8;
-  if (C > 512 || C * top > 4096) return 0;
+  if (C > 512 || C * top > (wide_type ? 5120 : 10240)) return 0;
   return C <= 256 ? 16 : 32;
 }
 
@@ -859,7 +893,7 @@ int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
-  if (const int team = lp_team_of(C, top)) {
+  if (const int team = lp_team_of(C, top, dtype == 0)) {
 #define CCN_LP_TEAM(T, TEAM)                                                                                                      \
   do {                                                                                                                            \
     const dim3 grid((unsigned)((rows + LP_TPB / TEAM - 1) / (LP_TPB / TEAM))), block(LP_TPB);                                     \
