@@ -13,6 +13,8 @@
 // and no gradient from it; any other target outside [0, C) -> NaN for both, and nothing is read there.
 #include <limits.h>
 
+#include <type_traits>
+
 #include "ccn_common.h"
 
 namespace {
@@ -160,6 +162,13 @@ struct LpShared {
   float red[2][NW];
 };
 
+// (no alternatives, or the best class alone)
+template <int NW>
+struct LpSharedFew {
+  uint64_t best[NW];
+  float red[2][NW];
+};
+
 template <int NW>
 __device__ __forceinline__ void lp_sync() {
   if (NW == 1) {
@@ -172,12 +181,12 @@ __device__ __forceinline__ void lp_sync() {
 
 // A value that at least `top` of the logits held reach, from the threads' maxima m: of every wave's 64 in order, the larger of the
 // top-th of one wave and of the (top / NW)-th, the least over the waves.  (The least of the maxima of `top` or more groups of threads needs
-// no order, but more logits reach it: 20000 x 1000 fp32 with 1 / 8 / 16 alternatives 27.0 / 33.4 / 39.1 us, in order 28.6 / 32.3 / 34.3.)
+// no order, but more logits reach it: 20000 x 1000 fp32 with 8 / 16 alternatives 33.4 / 39.1 us, in order 32.3 / 34.3.)
 template <int NW>
 __device__ __forceinline__ float lp_limit(float m, int top, LpShared<NW>& sh) {
   const int lane = threadIdx.x & 63, wave = NW == 4 ? threadIdx.x >> 6 : 0;
   uint32_t v = (uint32_t)(lp_key(m, 0) >> 32);
-  v = top == 1 ? ccn_wave_join(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; }) : lp_sort64(v);
+  v = lp_sort64(v);
   uint32_t bound = lp_kth_lane(v, top);
   if (NW > 1) {
     const uint32_t share = lp_kth_lane(v, (top + NW - 1) / NW);
@@ -229,8 +238,11 @@ __device__ __forceinline__ int lp_class(int c0, int tid, int e) {
   return c0 + ((e / V) * NT + tid) * V + e % V;
 }
 
-template <int T, int NW, bool TOP>
-__global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
+// TOP: 0 no alternatives, 1 the best class alone, 2 any number of them.  The best class needs no list: a wave looks for the class of its
+// largest logit where a piece of the row holds a larger one than those before (20000 x 1000 bf16: 13.3 us without, 16.4 with the best class,
+// 21.8 as a list of one; 600 x 20000 bf16 10.1, 12.2, 16.2).
+template <int T, int NW, int TOP>
+__global__ __launch_bounds__(LP_TPB, TOP < 2 ? 8 : NW == 1 || T == 0 ? 5 : 6) void logprob_wide_kernel(const void* __restrict__ x, int64_t ld,
                                                               const int64_t* __restrict__ target, int64_t rows, int C,
                                                               int64_t ignore, int top, int parts, int part_len,
                                                               float* __restrict__ logprob, float* __restrict__ entropy,
@@ -238,8 +250,9 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
                                                               int64_t* __restrict__ top_index, float4* __restrict__ part_stats,
                                                               uint64_t* __restrict__ part_keys) {
   constexpr int NT = NW * 64, V = CcnVec16<T>::N, NJ = LP_HOLD / V, TILE = NT * LP_HOLD;
-  __shared__ LpShared<NW> shared[4 / NW];
-  LpShared<NW>& sh = shared[NW == 4 ? 0 : threadIdx.x >> 6];
+  typedef std::conditional_t<TOP == 2, LpShared<NW>, LpSharedFew<NW>> Shared;
+  __shared__ Shared shared[4 / NW];
+  Shared& sh = shared[NW == 4 ? 0 : threadIdx.x >> 6];
   const int tid = NW == 4 ? threadIdx.x : threadIdx.x & 63, lane = threadIdx.x & 63, wave = NW == 4 ? threadIdx.x >> 6 : 0;
   const int64_t unit = NW == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t row = NW == 4 ? blockIdx.x / (unsigned)parts : unit;
@@ -255,7 +268,9 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
   float m = -INFINITY, s = 0.f, w = 0.f;
   int turn = 0, have = 0, waiting = 0;               // (the same in every thread)
   float limit = -INFINITY;
-  if (TOP) {
+  float first_value = -INFINITY;                     // (a row of -inf: its first class)
+  uint32_t first_class = beg;
+  if constexpr (TOP == 2) {
     if (tid < 3) sh.count[tid] = 0;
     lp_sync<NW>();
   }
@@ -293,7 +308,24 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
           w = __builtin_fmaf(e, d, w);
         }
       }
-    if (TOP) {
+    if constexpr (TOP == 1) {
+      const float of_wave = ccn_wave_join(tm, lp_max);
+      if (!(of_wave <= first_value) && first_value == first_value) {
+        uint32_t at = ~0u;
+#pragma unroll
+        for (int j = NJ - 1; j >= 0; --j)
+          if (vm[j] == of_wave || vm[j] != vm[j]) {
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i) {
+              const float u = get16<T>(raw[j], i);
+              if (u == of_wave || u != u) at = c0 + (j * NT + tid) * V + i;
+            }
+          }
+        first_class = ccn_wave_join(at, [](uint32_t a, uint32_t b) { return min(a, b); });
+        first_value = of_wave;
+      }
+    }
+    if constexpr (TOP == 2) {
       const bool first = c0 == beg;
       if (first) limit = lp_limit<NW>(tm, top, sh);
       // the logits of this thread that are not below v, or that beat it (a NaN is and does, but for a v of NaN, which none beats)
@@ -376,9 +408,13 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
       if (tid == 0) sh.count[turn == 2 ? 0 : turn + 1] = 0;
     }
   }
-  if (TOP) {
+  uint64_t best = 0;
+  if constexpr (TOP == 2) {
     if (waiting && wave == 0) lp_order<NW>(sh, top, have, waiting);
     have = min(top, have + waiting);
+  } else if (TOP == 1) {
+    best = lp_key(first_value, first_class);
+    if (NW > 1 && lane == 0) sh.best[wave] = best;
   }
   // the threads' statistics joined
   float all = m;
@@ -409,9 +445,14 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
     }
   }
   if (wave != 0) return;
+  if (TOP == 1 && NW > 1) {                          // (written two barriers ago)
+#pragma unroll
+    for (int k = 1; k < NW; ++k) best = best > sh.best[k] ? best : sh.best[k];
+  }
+  if (TOP == 2 && lane < have) best = sh.best[lane];
   if (parts > 1) {
     if (lane == 0) part_stats[unit] = make_float4(all, s, w, 0.f);
-    if (TOP && lane < top) part_keys[unit * top + lane] = lane < have ? sh.best[lane] : 0;
+    if (TOP && lane < top) part_keys[unit * top + lane] = best;
     return;
   }
   const LpRow r = lp_finish(all, s, w);
@@ -421,7 +462,6 @@ __global__ __launch_bounds__(LP_TPB, !TOP ? 8 : NW == 1 || T == 0 ? 5 : 6) void 
     if (stats) stats[row] = make_float2(r.base, r.log_total);
   }
   if (TOP && lane < top) {
-    const uint64_t best = sh.best[lane];
     top_logprob[row * top + lane] = (lp_key_value(best) - r.base) - r.log_total;
     top_index[row * top + lane] = lp_key_class(best);
   }
@@ -495,9 +535,8 @@ __device__ __forceinline__ V lp_team(V v, F f) {
 // ---- rows of 25 to 512 classes: TEAM lanes hold a row in registers, 16 logits each, and join their results by lane moves; a
 // wave has 64 / TEAM rows.  Alternatives: `top` walks over the registers, each of which takes the largest logit that is left; TEAM of
 // them are kept, a lane each, and stored side by side.  220011 x 55 fp32: 14.0 us, 3.8 TB/s, half of it the latency of one round of loads;
-// with alternatives the walks bound it, each of them 0.4 us for 100000 x 50 fp32 and 1.2 for 50000 x 256 (100000 x 100 bf16 10 us, with 5 of
-// them 20).
-template <int T, int TEAM, bool TOP>
+// with alternatives the walks bound it, each of them 1.2 us for 100000 x 50 fp32, 2.1 for 50000 x 256 fp32 and 1.1 in 16 bits.
+template <int T, int TEAM, int TOP>
 __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __restrict__ x, int64_t ld,
                                                               const int64_t* __restrict__ target, int64_t rows, int C,
                                                               int64_t ignore, int top, float* __restrict__ logprob,
@@ -538,7 +577,25 @@ __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __rest
     entropy[row] = r.entropy;
     if (stats) stats[row] = make_float2(r.base, r.log_total);
   }
-  if (!TOP) return;
+  if (TOP == 0) return;
+  if constexpr (TOP == 1) {                          // the lowest class of the largest logit (or of a NaN)
+    int at = INT_MAX / 2;
+#pragma unroll
+    for (int j = NJ - 1; j >= 0; --j)
+      if (j * TEAM * V < C) {
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) {
+          const float v = get16<T>(raw[j], i);
+          if (v == m || v != v) at = j * TEAM * V + i;
+        }
+      }
+    const uint32_t c = lp_team<TEAM>((uint32_t)(at + lane * V), [](uint32_t x, uint32_t y) { return min(x, y); });
+    if (live && lane == 0) {
+      top_logprob[row] = (m - r.base) - r.log_total;
+      top_index[row] = c;
+    }
+    return;
+  }
   // the logits as whole numbers in the order of the alternatives; in 16 bits with the class below them, so that no two are equal
   uint32_t o[HOLD];
 #pragma unroll
@@ -615,7 +672,7 @@ constexpr int LP_NARROW = 24;
 constexpr int LP_NARROW_TPB = 128;
 constexpr int LP_DIRECT_TOP = 4;                     // alternatives that are stored as they are found
 
-template <int T, bool TOP>
+template <int T, int TOP>
 __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const void* __restrict__ x, int64_t ld,
                                                                        const int64_t* __restrict__ target, int64_t rows, int C,
                                                                        int vecs, uint32_t magic, int64_t ignore, int top,
@@ -647,12 +704,14 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
     for (int c = 0; c < C; ++c) m = lp_max(m, mine[c]);
     const float given = t >= 0 && t < C ? mine[t] : 0.f;
     float s = 0.f, w = 0.f;
+    int first = C;                                   // the lowest class of the largest logit (or of a NaN)
 #pragma unroll 4
     for (int c = 0; c < C; ++c) {
       const float v = mine[c], d = lp_diff(v, m), e = lp_exp(d);
       s += e;
       w = __builtin_fmaf(e, d, w);
-      if (TOP) {                                     // from here on as a whole number in the order of the alternatives
+      if (TOP == 1) first = v == m || v != v ? min(first, c) : first;
+      if (TOP == 2) {                                // from here on as a whole number in the order of the alternatives
         int o = __float_as_int(v + 0.0f);
         if (v != v) o = 0x7f800001;
         mine[c] = __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
@@ -662,7 +721,11 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
     logprob[row] = t == ignore ? 0.f : t >= 0 && t < C ? (given - r.base) - r.log_total : NAN;
     entropy[row] = r.entropy;
     if (stats) stats[row] = make_float2(r.base, r.log_total);
-    if (TOP) {
+    if (TOP == 1) {
+      top_logprob[row] = (m - r.base) - r.log_total;
+      top_index[row] = first;
+    }
+    if (TOP == 2) {
       int* const order = reinterpret_cast<int*>(mine);
       for (int j = 0; j < top; ++j) {
         int v = INT_MIN, at = 0;                     // (below every value; taken ones become it)
@@ -684,7 +747,7 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
       }
     }
   }
-  if (!TOP || top <= LP_DIRECT_TOP) return;
+  if (TOP < 2 || top <= LP_DIRECT_TOP) return;
   __syncthreads();
   for (int i = threadIdx.x; i < live * top; i += LP_NARROW_TPB) {
     top_logprob[r0 * top + i] = out[i];
@@ -854,7 +917,7 @@ struct LpPlan {
 };
 LpPlan lp_plan(int64_t rows, int64_t C, int top) {
   LpPlan p = {C <= 64 * LP_HOLD ? 1 : 4, 1, (int)C};
-  if (p.nw == 1 || rows >= (top ? LP_FULL_TOP : LP_FULL)) return p;
+  if (p.nw == 1 || rows >= (top > 1 ? LP_FULL_TOP : LP_FULL)) return p;
   int64_t parts = (LP_WORKGROUPS + rows - 1) / rows;
   if (parts > (C + LP_PART - 1) / LP_PART) parts = (C + LP_PART - 1) / LP_PART;
   if (parts > LP_PARTS_MAX) parts = LP_PARTS_MAX;
@@ -880,29 +943,30 @@ int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
 #define CCN_LP_NARROW(T, TOP)                                                                                                     \
   hipLaunchKernelGGL((logprob_narrow_kernel<T, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, vecs, magic,          \
                      ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index)
-    if (top) {
-      if (dtype == 0) CCN_LP_NARROW(0, true);
-      else if (dtype == 1) CCN_LP_NARROW(1, true);
-      else CCN_LP_NARROW(2, true);
-    } else {
-      if (dtype == 0) CCN_LP_NARROW(0, false);
-      else if (dtype == 1) CCN_LP_NARROW(1, false);
-      else CCN_LP_NARROW(2, false);
-    }
+#define CCN_LP_NARROWS(T)              \
+  do {                                 \
+    if (top > 1) CCN_LP_NARROW(T, 2);  \
+    else if (top) CCN_LP_NARROW(T, 1); \
+    else CCN_LP_NARROW(T, 0);          \
+  } while (0)
+    if (dtype == 0) CCN_LP_NARROWS(0);
+    else if (dtype == 1) CCN_LP_NARROWS(1);
+    else CCN_LP_NARROWS(2);
+#undef CCN_LP_NARROWS
 #undef CCN_LP_NARROW
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
   if (const int team = lp_team_of(C, top, dtype == 0)) {
+#define CCN_LP_TEAM_TOP(T, TEAM, TOP)                                                                                             \
+  hipLaunchKernelGGL((logprob_team_kernel<T, TEAM, TOP>), grid, block, 0, s, logits, ld, target, rows, (int)C, ignore_index, top, \
+                     logprob, entropy, (float2*)stats, top_logprob, top_index)
 #define CCN_LP_TEAM(T, TEAM)                                                                                                      \
   do {                                                                                                                            \
     const dim3 grid((unsigned)((rows + LP_TPB / TEAM - 1) / (LP_TPB / TEAM))), block(LP_TPB);                                     \
-    if (top)                                                                                                                      \
-      hipLaunchKernelGGL((logprob_team_kernel<T, TEAM, true>), grid, block, 0, s, logits, ld, target, rows, (int)C,          \
-                         ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index);                            \
-    else                                                                                                                          \
-      hipLaunchKernelGGL((logprob_team_kernel<T, TEAM, false>), grid, block, 0, s, logits, ld, target, rows, (int)C,         \
-                         ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index);                            \
+    if (top > 1) CCN_LP_TEAM_TOP(T, TEAM, 2);                                                                                     \
+    else if (top) CCN_LP_TEAM_TOP(T, TEAM, 1);                                                                                    \
+    else CCN_LP_TEAM_TOP(T, TEAM, 0);                                                                                             \
   } while (0)
 #define CCN_LP_TEAMS(T)                                                                                                           \
   do {                                                                                                                            \
@@ -916,6 +980,7 @@ int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
     else CCN_LP_TEAMS(2);
 #undef CCN_LP_TEAMS
 #undef CCN_LP_TEAM
+#undef CCN_LP_TEAM_TOP
     CCN_LAUNCH_OK("logprob_fwd");
     return CCN_OK;
   }
@@ -928,10 +993,12 @@ int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
                      part_stats, part_keys)
 #define CCN_LP_FWD(T)                                                                                                             \
   do {                                                                                                                            \
-    if (p.nw == 1 && top) CCN_LP_WIDE(T, 1, true);                                                                                \
-    else if (p.nw == 1) CCN_LP_WIDE(T, 1, false);                                                                                 \
-    else if (top) CCN_LP_WIDE(T, 4, true);                                                                                        \
-    else CCN_LP_WIDE(T, 4, false);                                                                                                \
+    if (p.nw == 1 && top > 1) CCN_LP_WIDE(T, 1, 2);                                                                               \
+    else if (p.nw == 1 && top) CCN_LP_WIDE(T, 1, 1);                                                                              \
+    else if (p.nw == 1) CCN_LP_WIDE(T, 1, 0);                                                                                     \
+    else if (top > 1) CCN_LP_WIDE(T, 4, 2);                                                                                       \
+    else if (top) CCN_LP_WIDE(T, 4, 1);                                                                                           \
+    else CCN_LP_WIDE(T, 4, 0);                                                                                                    \
     if (p.parts > 1)                                                                                                              \
       hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)rows), dim3(LP_TPB), 0, s, logits, ld, target, (int)C,             \
                          ignore_index, top, p.parts, part_stats, part_keys, logprob, entropy, (float2*)stats, top_logprob,        \

@@ -321,6 +321,27 @@ def test_rows_of_many_nan(c, dtype):
         _check(x, t, top)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("c", [1, 2, 20, 24, 25, 55, 64, 65, 128, 129, 300, 512, 513, 1000, 2048, 2049, 5000, 40000, 200003])
+def test_the_best_class_alone(c, dtype):
+    x, t = _logits(12, c, dtype), _target(12, c)
+    x[0] = 1.5                                                          # equal ones: the lowest class
+    x[1] = -math.inf
+    x[2, : c - 1] = -math.inf
+    x[3, c // 2:] = 40.0
+    x[4, -1] = x[4, c // 3] = math.nan
+    x[5, -1] = math.inf
+    x[6] = torch.linspace(-20, 20, c, device=DEV).to(dtype)
+    x[7] = torch.linspace(20, -20, c, device=DEV).to(dtype)
+    x[8] = 0.0
+    x[8, 1::2] = -0.0
+    x[9] = -0.0
+    x[9, c // 2] = 0.0
+    _check(x, t, 1)
+    some = x[torch.tensor([0, 3, 6, 7, 8, 9, 10, 11], device=DEV)]
+    _check_gradient(some, _target(8, c), 1)
+
+
 def test_targets_that_are_not_scored():
     for c in (20, 65, 3000):
         rows = 9
