@@ -825,6 +825,7 @@ __device__ __forceinline__ void lp_grad_top(const LpGrad& q, const void* __restr
 // pieces of a row.  220011 x 55 fp32: 21.3 us, 4.7 TB/s read and written.
 constexpr int LP_GROUP = 4096;              // logits of a group of rows, about
 constexpr int LP_GROUP_MAX = 4096;
+constexpr int LP_GROUPS = 1024;             // groups, about, where rows are few (1500 x 20 fp32 with 20 alternatives: 14.8 us in 8 groups, 7.7)
 
 template <int T>
 __global__ __launch_bounds__(LP_TPB) void logprob_bwd_rows_kernel(
@@ -897,6 +898,15 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
   }
 }
 
+// Whether the row is logprob_narrow_kernel's.  Its walks wait for shared memory: where rows are few the team's registers are faster from three
+// alternatives on (us, narrow / team, 1500 x 20 with 3 / 10 / 20 of them: fp32 8.2 / 6.8, 12.0 / 9.3, 17.6 / 12.3, bf16 9.1 / 6.8, 13.1 / 7.5,
+// 19.0 / 8.9), and where they are many in 16 bits with many alternatives (400000 x 20 with 5 / 10: bf16 24.6 / 24.2, 35 / 30, fp32 22 / 29, 33 / 42).
+bool lp_is_narrow(int64_t rows, int64_t C, int top, bool wide_type) {
+  if (C > LP_NARROW) return false;
+  if (C < 12 || top < 3) return true;
+  return rows > 65536 && (wide_type || C < 20 || top < 8);
+}
+
 // Lanes to a row of logprob_team_kernel, 0 where the row is logprob_wide_kernel's: that one's way to the alternatives costs the same for
 // many of them, and a walk here costs less in 16 bits (us, 50000 rows, here / there: 500 bf16 with 12 of them 44 / 57, with 20 58 / 60; 256 fp16
 // with 32 44 / 66; 500 fp32 with 8 53 / 58, with 12 70 / 61; 256 fp32 with 20 55 / 61).
@@ -907,6 +917,16 @@ int lp_team_of(int64_t C, int top, bool wide_type) {
   return C <= 256 ? 16 : 32;
 }
 
+// Waves to a row of logprob_wide_kernel.  One is enough up to 2048 classes; where rows are many it goes on longer alone, since four spend more
+// on joining what they found (us, four / one, 20000 rows of 2050: bf16 with 0 / 5 alternatives 40 / 23, 86 / 38, fp32 40 / 29, 98 / 43; of 4100: 48 /
+// 34, 96 / 55, fp32 52 / 56, 117 / 70; of 8192: 55 / 60, 125 / 93, fp32 107 / 118, 131 / 124; 4000 rows of 2050 bf16 with 5 22 / 13, of 8192 26.5 /
+// 25.2; 1000 of 2050 11.1 / 10.8, of 4100 11.3 / 13.1).
+int lp_waves(int64_t rows, int64_t C, int top, bool wide_type) {
+  if (C <= 64 * LP_HOLD) return 1;
+  if (rows < (C <= 4096 ? 2048 : 4096)) return 4;
+  return (top > 1 ? C <= 8192 : C * (wide_type ? 4 : 2) <= 12000) ? 1 : 4;
+}
+
 // How rows are cut into parts of about one length, a workgroup each, where there are too few rows to fill the card: 512 x 131072 bf16
 // with 8 alternatives takes 58 us in one part to a row and 45 in three, 512 x 50000 31 and 27, but 1000 x 50000 38 and 44 in two (each
 // part orders its own); without alternatives 256 x 50000 12.2 and 13.0, 512 x 20000 fp32 11.3 and 13.6 (the joining launch).  Parts of less
@@ -915,8 +935,8 @@ constexpr int64_t LP_FULL = 256, LP_FULL_TOP = 768, LP_WORKGROUPS = 1536, LP_PAR
 struct LpPlan {
   int nw, parts, part_len;
 };
-LpPlan lp_plan(int64_t rows, int64_t C, int top) {
-  LpPlan p = {C <= 64 * LP_HOLD ? 1 : 4, 1, (int)C};
+LpPlan lp_plan(int64_t rows, int64_t C, int top, bool wide_type) {
+  LpPlan p = {lp_waves(rows, C, top, wide_type), 1, (int)C};
   if (p.nw == 1 || rows >= (top > 1 ? LP_FULL_TOP : LP_FULL)) return p;
   int64_t parts = (LP_WORKGROUPS + rows - 1) / rows;
   if (parts > (C + LP_PART - 1) / LP_PART) parts = (C + LP_PART - 1) / LP_PART;
@@ -935,7 +955,7 @@ int64_t lp_tiles(int64_t C) { return (C + LP_TPB * LP_HOLD - 1) / (LP_TPB * LP_H
 int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index, int top,
            const LpPlan& p, float* logprob, float* entropy, float* stats, float* top_logprob, int64_t* top_index, void* ws,
            hipStream_t s) {
-  if (C <= LP_NARROW) {
+  if (lp_is_narrow(rows, C, top, dtype == 0)) {
     const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
     const dim3 grid((unsigned)((rows + LP_NARROW_TPB - 1) / LP_NARROW_TPB)), block(LP_NARROW_TPB);
@@ -1018,7 +1038,8 @@ int lp_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
            const float* g_entropy, int64_t g_entropy_stride, const float* g_top, void* dlogits, int64_t ldd, hipStream_t s) {
   if (C <= LP_GROUP_MAX) {
     const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
-    const int group = (int)(LP_GROUP / C < 1 ? 1 : LP_GROUP / C > LP_TPB ? LP_TPB : LP_GROUP / C);
+    const int64_t share = rows / LP_GROUPS, most = LP_GROUP / C > LP_TPB ? LP_TPB : LP_GROUP / C;
+    const int group = (int)(share < 1 || most < 1 ? 1 : share < most ? share : most);
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
     const dim3 grid((unsigned)((rows + group - 1) / group)), block(LP_TPB);
 #define CCN_LP_BWD(T)                                                                                                             \
@@ -1049,7 +1070,7 @@ int lp_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
 
 extern "C" size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top) {
   if (rows <= 0 || C <= LP_NARROW || top < 0) return 0;
-  const LpPlan p = lp_plan(rows, C, top);
+  const LpPlan p = lp_plan(rows, C, top, false);     // (rows that are cut are too few for their type to matter)
   if (p.parts == 1) return 0;
   return ccn_align256((size_t)rows * p.parts * sizeof(float4)) + ccn_align256((size_t)rows * p.parts * top * sizeof(uint64_t));
 }
@@ -1064,7 +1085,7 @@ extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const 
               "logprob_fwd: rows=%lld C=%lld ld=%lld", (long long)rows, (long long)C, (long long)ld);
   CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_fwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
   CCN_REQUIRE(top == 0 || (top_logprob && top_index), "logprob_fwd: top > 0 without its outputs");
-  const LpPlan p = lp_plan(rows, C, top);
+  const LpPlan p = lp_plan(rows, C, top, dtype == 0);
   const size_t need = ccn_logprob_workspace_bytes(rows, C, top);
   if (need && (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < need)) {
     ccn_set_error("logprob_fwd: workspace of %zu bytes, %zu are needed (16-byte aligned)", ws ? ws_bytes : (size_t)0, need);

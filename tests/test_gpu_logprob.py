@@ -433,6 +433,35 @@ def test_many_rows():
         assert bool(((d.double() - ref).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,c,tops", [(65541, 3, (3,)), (65541, 11, (3, 5, 11)), (65541, 12, (3, 5, 12)), (65541, 20, (4, 5, 7, 8, 20)),
+                                         (65541, 24, (3, 7, 8, 24)), (2050, 2049, (0, 1, 2, 20, 64)), (2050, 2999, (0, 1, 5)),
+                                         (2050, 4095, (0, 1, 5, 33)), (4100, 4097, (0, 1, 5)), (4100, 6001, (0, 1, 3)), (4100, 8192, (2, 20, 64))])
+def test_many_rows_of_every_kind(rows, c, tops, dtype):
+    """Kernels that are taken where rows are many: odd rows among ordinary ones, at the start, in the middle and at the end."""
+    gen = torch.Generator(device=DEV).manual_seed(c)
+    x = (torch.randn(rows, c, generator=gen, device=DEV) * 3).to(dtype)
+    t = torch.randint(0, c, (rows,), generator=gen, device=DEV)
+    parts = [slice(0, 13), slice(rows // 2, rows // 2 + 13), slice(rows - 13, rows)]
+    for p in parts:
+        y = x[p]
+        y[0] = 1.5
+        y[1] = -math.inf
+        y[2, : c - 1] = -math.inf
+        y[3, c // 2:] = 40.0
+        y[4, -1] = y[4, c // 3] = math.nan
+        y[5, -1] = math.inf
+        y[6] = torch.linspace(-20, 20, c, device=DEV).to(dtype)
+        y[7] = torch.linspace(20, -20, c, device=DEV).to(dtype)
+        y[8] = math.nan
+        y[9, torch.arange(c, device=DEV) % 50 != 7 % c] = -math.inf
+        y[10, c - c // 3:] += 20.0
+    for top in tops:
+        r = _score(x, t, top=top)
+        for p in parts:
+            _check(x[p], t[p], top, r=type(r)(*(None if v is None else v[p] for v in r)))
+
+
 def test_same_bits_every_time_and_two_streams_at_once():
     x, t = _logits(37, 40001, torch.bfloat16), _target(37, 40001)
     y, k = _logits(5000, 20, torch.float32), _target(5000, 20)
@@ -582,12 +611,15 @@ def test_more_rows_than_a_launch_holds(c, top):
     (d,) = torch.autograd.grad(r.logprob.sum() + 2 * r.entropy.sum(), x)
     for at in (0, border - 4):
         part = slice(at, at + 9)
-        small = x.detach()[part].clone().requires_grad_(True)
-        q = _score(small, t[part], top=top)
-        _check(small, t[part], top, r=q)
+        # (as many rows as take the same kernels)
+        small, given = torch.zeros(5000, c, dtype=x.dtype, device=DEV), torch.zeros(5000, dtype=torch.int64, device=DEV)
+        small[:9], given[:9] = x.detach()[part], t[part]
+        small.requires_grad_(True)
+        q = _score(small, given, top=top)
+        _check(small[:9].detach(), given[:9], top, r=type(q)(*(None if a is None else a[:9] for a in q)))
         (e,) = torch.autograd.grad(q.logprob.sum() + 2 * q.entropy.sum(), small)
-        assert torch.equal(d[part], e)
-        assert all(torch.equal(a[part], b) for a, b in zip(r, q) if a is not None)
+        assert torch.equal(d[part], e[:9])
+        assert all(torch.equal(a[part], b[:9]) for a, b in zip(r, q) if a is not None)
     rest = r.logprob.detach()[9: border - 4]
     _near(rest[:: 1 << 18], torch.full((rest[:: 1 << 18].numel(),), -math.log(c)), _e(torch.tensor(math.log(c)), c), "rows of zeros")
     assert bool((rest == rest[0]).all())
