@@ -930,14 +930,18 @@ int lp_waves(int64_t rows, int64_t C, int top, bool wide_type) {
 // How rows are cut into parts of about one length, a workgroup each, where there are too few rows to fill the card: 512 x 131072 bf16
 // with 8 alternatives takes 58 us in one part to a row and 45 in three, 512 x 50000 31 and 27, but 1000 x 50000 38 and 44 in two (each
 // part orders its own); without alternatives 256 x 50000 12.2 and 13.0, 512 x 20000 fp32 11.3 and 13.6 (the joining launch).  Parts of less
-// than LP_PART cost more than they gain (96 x 131072 fp16 with 20: 23.9, with parts of half that 34.6).
-constexpr int64_t LP_FULL = 256, LP_FULL_TOP = 768, LP_WORKGROUPS = 1536, LP_PART = LP_TPB * LP_HOLD, LP_PARTS_MAX = 64;
+// than LP_PART cost more than they gain (96 x 131072 fp16 with 20: 23.9, with parts of half that 34.6).  Rows of a few parts' length stay
+// whole, since the joining launch costs more than the workgroup's next turns (us, in parts / whole, 1 or 30 rows of bf16: 32000 classes 9.2 / 7.6,
+// 20000 and the best class 9.1 / 8.0, of 32000 9.4 / 9.4, 12000 with 5 alternatives 12.4 / 12.1, 20000 12.8 / 14.4); with alternatives also those of
+// 600 rows and up to 32768 classes (24000 with 5 19.6 / 18.4, of 300 14.5 / 16.2).
+constexpr int64_t LP_FULL = 256, LP_FULL_TOP = 768, LP_FULL_SHORT = 512, LP_WORKGROUPS = 1536, LP_PART = LP_TPB * LP_HOLD, LP_PARTS_MAX = 64;
 struct LpPlan {
   int nw, parts, part_len;
 };
 LpPlan lp_plan(int64_t rows, int64_t C, int top, bool wide_type) {
   LpPlan p = {lp_waves(rows, C, top, wide_type), 1, (int)C};
-  if (p.nw == 1 || rows >= (top > 1 ? LP_FULL_TOP : LP_FULL)) return p;
+  if (p.nw == 1 || C <= LP_PART * (top > 1 ? 2 : top ? 3 : 4)) return p;
+  if (rows >= (top <= 1 ? LP_FULL : C <= 4 * LP_PART ? LP_FULL_SHORT : LP_FULL_TOP)) return p;
   int64_t parts = (LP_WORKGROUPS + rows - 1) / rows;
   if (parts > (C + LP_PART - 1) / LP_PART) parts = (C + LP_PART - 1) / LP_PART;
   if (parts > LP_PARTS_MAX) parts = LP_PARTS_MAX;
