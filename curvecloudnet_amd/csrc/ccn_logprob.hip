@@ -930,21 +930,27 @@ int lp_waves(int64_t rows, int64_t C, int top, bool wide_type) {
 // How rows are cut into parts of about one length, a workgroup each, where there are too few rows to fill the card: 512 x 131072 bf16
 // with 8 alternatives takes 58 us in one part to a row and 45 in three, 512 x 50000 31 and 27, but 1000 x 50000 38 and 44 in two (each
 // part orders its own); without alternatives 256 x 50000 12.2 and 13.0, 512 x 20000 fp32 11.3 and 13.6 (the joining launch).  Parts of less
-// than LP_PART cost more than they gain (96 x 131072 fp16 with 20: 23.9, with parts of half that 34.6).  Rows of a few parts' length stay
+// than a piece cost more than they gain (96 x 131072 fp16 with 20: 23.9, with parts of half that 34.6).  Rows of a few pieces stay
 // whole, since the joining launch costs more than the workgroup's next turns (us, in parts / whole, 1 or 30 rows of bf16: 32000 classes 9.2 / 7.6,
 // 20000 and the best class 9.1 / 8.0, of 32000 9.4 / 9.4, 12000 with 5 alternatives 12.4 / 12.1, 20000 12.8 / 14.4); with alternatives also those of
 // 600 rows and up to 32768 classes (24000 with 5 19.6 / 18.4, of 300 14.5 / 16.2).
-constexpr int64_t LP_FULL = 256, LP_FULL_TOP = 768, LP_FULL_SHORT = 512, LP_WORKGROUPS = 1536, LP_PART = LP_TPB * LP_HOLD, LP_PARTS_MAX = 64;
+// Parts of one piece where a quarter more workgroups than fit at once do that; else as many as fit, and no more than take as many pieces each
+// (bf16 with 5: 266 x 51831 in 4 / 5 / 6 / 7 parts 18.8 / 19.8 / 22.5 / 20.1 us, 180 x 131072 in 7 / 8 / 9 23.5 / 21.5 / 25.8, 100 x 131072 in 15 / 16
+// 19.6 / 18.2; fp32, of which fewer fit, 400 x 51831 in 3 / 4 25.2 / 26.6).
+constexpr int64_t LP_FULL = 256, LP_FULL_TOP = 768, LP_FULL_SHORT = 512, LP_PIECE = LP_TPB * LP_HOLD, LP_PARTS_MAX = 64;
+int64_t lp_pieces(int64_t C) { return (C + LP_PIECE - 1) / LP_PIECE; }
 struct LpPlan {
   int nw, parts, part_len;
 };
 LpPlan lp_plan(int64_t rows, int64_t C, int top, bool wide_type) {
   LpPlan p = {lp_waves(rows, C, top, wide_type), 1, (int)C};
-  if (p.nw == 1 || C <= LP_PART * (top > 1 ? 2 : top ? 3 : 4)) return p;
-  if (rows >= (top <= 1 ? LP_FULL : C <= 4 * LP_PART ? LP_FULL_SHORT : LP_FULL_TOP)) return p;
-  int64_t parts = (LP_WORKGROUPS + rows - 1) / rows;
-  if (parts > (C + LP_PART - 1) / LP_PART) parts = (C + LP_PART - 1) / LP_PART;
+  if (p.nw == 1 || C <= LP_PIECE * (top > 1 ? 2 : top ? 3 : 4)) return p;
+  if (rows >= (top <= 1 ? LP_FULL : C <= 4 * LP_PIECE ? LP_FULL_SHORT : LP_FULL_TOP)) return p;
+  const int64_t fit = 256 * (top <= 1 ? 8 : wide_type ? 5 : 6);       // (the launch bounds of logprob_wide_kernel)
+  int64_t parts = lp_pieces(C);
+  if (rows * parts > fit + fit / 4) parts = fit / rows < 1 ? 1 : fit / rows;
   if (parts > LP_PARTS_MAX) parts = LP_PARTS_MAX;
+  parts = (lp_pieces(C) + lp_pieces((C + parts - 1) / parts) - 1) / lp_pieces((C + parts - 1) / parts);
   p.part_len = (int)(((C + parts - 1) / parts + 7) / 8 * 8);
   p.parts = (int)((C + p.part_len - 1) / p.part_len);
   return p;
@@ -953,7 +959,6 @@ LpPlan lp_plan(int64_t rows, int64_t C, int top, bool wide_type) {
 // A launch holds fewer than 2^32 threads: rows go in pieces (a workgroup of the widest takes one).
 constexpr int64_t LP_LAUNCH_ROWS = (int64_t)1 << 22;
 const void* lp_row(const void* x, int dtype, int64_t at) { return (const char*)x + at * (dtype == 0 ? 4 : 2); }
-int64_t lp_tiles(int64_t C) { return (C + LP_TPB * LP_HOLD - 1) / (LP_TPB * LP_HOLD); }
 
 // The launches of one piece of the rows (p: of all of them).
 int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C, int64_t ignore_index, int top,
@@ -1055,7 +1060,7 @@ int lp_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
     else CCN_LP_BWD(2);
 #undef CCN_LP_BWD
   } else {
-    const int64_t tiles = lp_tiles(C);
+    const int64_t tiles = lp_pieces(C);
     const dim3 grid((unsigned)(rows * tiles)), block(LP_TPB);
 #define CCN_LP_BWD(T)                                                                                                             \
   hipLaunchKernelGGL(logprob_bwd_wide_kernel<T>, grid, block, 0, s, logits, ld, target, (int)C, ignore_index, top, (int)tiles,     \
@@ -1074,9 +1079,9 @@ int lp_bwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
 
 extern "C" size_t ccn_logprob_workspace_bytes(int64_t rows, int64_t C, int top) {
   if (rows <= 0 || C <= LP_NARROW || top < 0) return 0;
-  const LpPlan p = lp_plan(rows, C, top, false);     // (rows that are cut are too few for their type to matter)
-  if (p.parts == 1) return 0;
-  return ccn_align256((size_t)rows * p.parts * sizeof(float4)) + ccn_align256((size_t)rows * p.parts * top * sizeof(uint64_t));
+  const int a = lp_plan(rows, C, top, false).parts, b = lp_plan(rows, C, top, true).parts, parts = a > b ? a : b;      // (for any type)
+  if (parts == 1) return 0;
+  return ccn_align256((size_t)rows * parts * sizeof(float4)) + ccn_align256((size_t)rows * parts * top * sizeof(uint64_t));
 }
 
 extern "C" int ccn_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int64_t rows, int64_t C,
@@ -1118,7 +1123,7 @@ extern "C" int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const 
   CCN_REQUIRE(top >= 0 && top <= LP_TOP_MAX && top <= C, "logprob_bwd: top=%d (at most %d, and at most C)", top, LP_TOP_MAX);
   CCN_REQUIRE(top == 0 || (g_top && top_index), "logprob_bwd: top > 0 without its gradient and classes");
   CCN_REQUIRE(g_logprob_stride >= 0 && g_entropy_stride >= 0, "logprob_bwd: negative gradient stride");
-  const int64_t most = C <= LP_GROUP_MAX ? LP_LAUNCH_ROWS : (LP_LAUNCH_ROWS + lp_tiles(C) - 1) / lp_tiles(C);
+  const int64_t most = C <= LP_GROUP_MAX ? LP_LAUNCH_ROWS : (LP_LAUNCH_ROWS + lp_pieces(C) - 1) / lp_pieces(C);
   for (int64_t r = 0; r < rows; r += most) {
     const int rc = lp_bwd(lp_row(logits, dtype, r * ld), dtype, ld, target + r, rows - r < most ? rows - r : most, C, ignore_index, top,
                           top ? top_index + r * top : nullptr, stats + 2 * r, entropy + r,
