@@ -661,16 +661,20 @@ __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __rest
   }
 }
 
-// ---- rows of up to 24 classes: 128 rows go through shared memory (16-byte loads) and a thread walks each of them there; the odd pitch puts
-// the lanes of a wave on different banks.  (Two threads to a row, or the registers of logprob_team_kernel, take 12.0 and 12.3 us for
-// 400070 x 20 instead of 10.8.)
-// Bound by the latency from load to store of a workgroup's rows (400070 x 20 fp32 10.8 us, 3.6 TB/s; with 3 alternatives 14.2 us).
-// Alternatives: `top` walks, each of which takes the largest value that is left (of equal ones the lowest class).  Many of them leave
-// through shared memory: a thread's own are `top` values wide, 64 such stores side by side cost more than the walks (400070 x 20: 3 of
-// them 17.6 us without the detour and 20.1 with it, 5 23.2 and 23.5, 8 36.6 and 29.6; 500000 x 8: 5 of them 20.4 and 14.3).
+// ---- rows of up to 24 classes: 128 rows go through shared memory (16-byte loads) and a thread walks each of them there.  (Two threads to a
+// row, or the registers of logprob_team_kernel, take 12.0 and 12.3 us for 400070 x 20 instead of 10.8.)  Bound by the latency from load to
+// store of a workgroup's rows, and by its stores (400000 x 20 fp32: 9.9 us, 3.9 TB/s; with 3 alternatives 15.1, 3.5).
+// Up to LP_FEW_MAX alternatives come out of the two walks that the row takes anyway: the first keeps the K largest values in order, the second,
+// from the last class to the first, notes where they are.  They leave through the row's own place in shared memory: a thread's own are K values
+// wide, 64 such stores side by side cost more.  More of them: a walk for each, which takes the largest that is left (400000 x 20 fp32 with 3 / 5
+// of them 16.1 / 22.3 us by walks and 15.1 / 18.3 so, x 12 12.4 / 16.6 and 12.2 / 14.1).
 constexpr int LP_NARROW = 24;
 constexpr int LP_NARROW_TPB = 128;
-constexpr int LP_DIRECT_TOP = 4;                     // alternatives that are stored as they are found
+
+// TOP: 0 none, 1 the best class alone, LP_FEW + K: K of them, LP_WALK any number.
+constexpr int LP_FEW = 100, LP_FEW_MAX = 5, LP_WALK = 2;
+// A row's place in shared memory, which takes its few alternatives as well; odd, so that the lanes of a wave meet different banks.
+__host__ __device__ inline int lp_pitch(int C, int few) { return (C > 2 * few ? C : 2 * few) | 1; }
 
 template <int T, int TOP>
 __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const void* __restrict__ x, int64_t ld,
@@ -681,9 +685,9 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
                                                                        float* __restrict__ top_logprob,
                                                                        int64_t* __restrict__ top_index) {
   extern __shared__ float tile[];
-  constexpr int V = CcnVec16<T>::N, ROWS = LP_NARROW_TPB;
+  constexpr int V = CcnVec16<T>::N, ROWS = LP_NARROW_TPB, K = TOP > LP_FEW ? TOP - LP_FEW : 1;
   const int64_t r0 = (int64_t)blockIdx.x * ROWS;
-  const int live = (int)min((int64_t)ROWS, rows - r0), pitch = C | 1;
+  const int live = (int)min((int64_t)ROWS, rows - r0), pitch = lp_pitch(C, TOP > LP_FEW ? K : 0);
   // 16-byte pieces, `vecs` to a row (i / vecs as a product: exact for i < 2^16, the error of magic is below 2^-16)
   const int n = live * vecs;
   for (int i = threadIdx.x; i < n; i += LP_NARROW_TPB) {
@@ -699,22 +703,33 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
   if ((int)threadIdx.x < live) {
     float* const mine = tile + threadIdx.x * pitch;
     const int64_t row = r0 + threadIdx.x, t = target[row];
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int c = 0; c < C; ++c) m = lp_max(m, mine[c]);
     const float given = t >= 0 && t < C ? mine[t] : 0.f;
-    float s = 0.f, w = 0.f;
-    int first = C;                                   // the lowest class of the largest logit (or of a NaN)
+    // the K largest in order: a new one pushes those below it down by one
+    float best[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) best[k] = -INFINITY;
 #pragma unroll 4
     for (int c = 0; c < C; ++c) {
+      const float v = mine[c];
+#pragma unroll
+      for (int k = K - 1; k > 0; --k) best[k] = __builtin_amdgcn_fmed3f(v, best[k - 1], best[k]);
+      best[0] = lp_max(best[0], v);
+    }
+    const float m = best[0];
+    float s = 0.f, w = 0.f;
+    int at[K];                                       // their classes; from the last class to the first, equal ones by ascending class
+#pragma unroll
+    for (int k = 0; k < K; ++k) at[k] = 0;
+#pragma unroll 4
+    for (int c = C - 1; c >= 0; --c) {
       const float v = mine[c], d = lp_diff(v, m), e = lp_exp(d);
       s += e;
       w = __builtin_fmaf(e, d, w);
-      if (TOP == 1) first = v == m || v != v ? min(first, c) : first;
-      if (TOP == 2) {                                // from here on as a whole number in the order of the alternatives
-        int o = __float_as_int(v + 0.0f);
-        if (v != v) o = 0x7f800001;
-        mine[c] = __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+      if (TOP == 1) at[0] = v == m || v != v ? c : at[0];
+      if (TOP > LP_FEW) {
+#pragma unroll
+        for (int k = K - 1; k > 0; --k) at[k] = v == best[k] ? (best[k] == best[k - 1] ? at[k - 1] : c) : at[k];
+        at[0] = v == m ? c : at[0];
       }
     }
     const LpRow r = lp_finish(m, s, w);
@@ -723,35 +738,62 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
     if (stats) stats[row] = make_float2(r.base, r.log_total);
     if (TOP == 1) {
       top_logprob[row] = (m - r.base) - r.log_total;
-      top_index[row] = first;
+      top_index[row] = at[0];
     }
-    if (TOP == 2) {
-      int* const order = reinterpret_cast<int*>(mine);
-      for (int j = 0; j < top; ++j) {
-        int v = INT_MIN, at = 0;                     // (below every value; taken ones become it)
+    // (the K largest are not found among NaN: the few waves that have any walk)
+    if (TOP == LP_WALK || (TOP > LP_FEW && __builtin_amdgcn_ballot_w64(m != m) != 0)) {
+      int* const order = reinterpret_cast<int*>(mine);   // whole numbers in the order of the alternatives
 #pragma unroll 4
-        for (int c = 0; c < C; ++c) {
-          const int o = order[c];
-          at = o > v ? c : at;
+      for (int c = 0; c < C; ++c) {
+        const float v = mine[c];
+        int o = __float_as_int(v + 0.0f);
+        if (v != v) o = 0x7f800001;
+        order[c] = o ^ ((o >> 31) & 0x7fffffff);
+      }
+      auto walk = [&](float& value, int& c) {
+        int v = INT_MIN;                             // (below every value; taken ones become it)
+        c = 0;
+#pragma unroll 4
+        for (int i = 0; i < C; ++i) {
+          const int o = order[i];
+          c = o > v ? i : c;
           v = max(v, o);
         }
-        order[at] = INT_MIN;
-        const float l = (__int_as_float(v ^ ((v >> 31) & 0x7fffffff)) - r.base) - r.log_total;
-        if (top <= LP_DIRECT_TOP) {
-          top_logprob[row * top + j] = l;
-          top_index[row * top + j] = at;
-        } else {
-          out[threadIdx.x * top + j] = l;
-          out_class[threadIdx.x * top + j] = at;
+        order[c] = INT_MIN;
+        value = __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
+      };
+      if constexpr (TOP == LP_WALK) {
+        for (int j = 0; j < top; ++j) {
+          float v;
+          walk(v, out_class[threadIdx.x * top + j]);
+          out[threadIdx.x * top + j] = (v - r.base) - r.log_total;
         }
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k) walk(best[k], at[k]);
+      }
+    }
+    if (TOP > LP_FEW) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        mine[k] = (best[k] - r.base) - r.log_total;  // (the row itself is not needed any more)
+        mine[K + k] = __int_as_float(at[k]);
       }
     }
   }
-  if (TOP < 2 || top <= LP_DIRECT_TOP) return;
+  if (TOP < 2) return;
   __syncthreads();
-  for (int i = threadIdx.x; i < live * top; i += LP_NARROW_TPB) {
-    top_logprob[r0 * top + i] = out[i];
-    top_index[r0 * top + i] = out_class[i];
+  if constexpr (TOP > LP_FEW) {
+    for (int i = threadIdx.x; i < live * K; i += LP_NARROW_TPB) {
+      const float* const from = tile + i / K * pitch + i % K;
+      top_logprob[r0 * K + i] = from[0];
+      top_index[r0 * K + i] = __float_as_int(from[K]);
+    }
+  } else {
+    for (int i = threadIdx.x; i < live * top; i += LP_NARROW_TPB) {
+      top_logprob[r0 * top + i] = out[i];
+      top_index[r0 * top + i] = out_class[i];
+    }
   }
 }
 
@@ -899,8 +941,8 @@ __global__ __launch_bounds__(LP_TPB) void logprob_bwd_wide_kernel(
 }
 
 // Whether the row is logprob_narrow_kernel's.  Its walks wait for shared memory: where rows are few the team's registers are faster from three
-// alternatives on (us, narrow / team, 1500 x 20 with 3 / 10 / 20 of them: fp32 8.2 / 6.8, 12.0 / 9.3, 17.6 / 12.3, bf16 9.1 / 6.8, 13.1 / 7.5,
-// 19.0 / 8.9), and where they are many in 16 bits with many alternatives (400000 x 20 with 5 / 10: bf16 24.6 / 24.2, 35 / 30, fp32 22 / 29, 33 / 42).
+// alternatives on (us, narrow / team, 1500 x 20 with 3 / 10 / 20 of them: fp32 7.7 / 6.7, 12.0 / 9.3, 17.6 / 12.3, bf16 8.6 / 6.4, 13.1 / 7.5,
+// 19.0 / 8.9), and where they are many in 16 bits with many alternatives (400000 x 20 with 5 / 10: bf16 19.1 / 24.2, 35 / 30, fp32 18.3 / 29, 33 / 42).
 bool lp_is_narrow(int64_t rows, int64_t C, int top, bool wide_type) {
   if (C > LP_NARROW) return false;
   if (C < 12 || top < 3) return true;
@@ -968,16 +1010,21 @@ int lp_fwd(const void* logits, int dtype, int64_t ld, const int64_t* target, int
     const int per = dtype == 0 ? 4 : 8, vecs = (int)((C + per - 1) / per);
     const uint32_t magic = vecs == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs);
     const dim3 grid((unsigned)((rows + LP_NARROW_TPB - 1) / LP_NARROW_TPB)), block(LP_NARROW_TPB);
-    const size_t lds = (size_t)LP_NARROW_TPB * ((C | 1) + (top > LP_DIRECT_TOP ? 2 * top : 0)) * sizeof(float);
+    const size_t lds = (size_t)LP_NARROW_TPB * (lp_pitch((int)C, top > 1 && top <= LP_FEW_MAX ? top : 0) + (top > LP_FEW_MAX ? 2 * top : 0)) * sizeof(float);
 #define CCN_LP_NARROW(T, TOP)                                                                                                     \
   hipLaunchKernelGGL((logprob_narrow_kernel<T, TOP>), grid, block, lds, s, logits, ld, target, rows, (int)C, vecs, magic,          \
                      ignore_index, top, logprob, entropy, (float2*)stats, top_logprob, top_index)
-#define CCN_LP_NARROWS(T)              \
-  do {                                 \
-    if (top > 1) CCN_LP_NARROW(T, 2);  \
-    else if (top) CCN_LP_NARROW(T, 1); \
-    else CCN_LP_NARROW(T, 0);          \
+#define CCN_LP_NARROWS(T)                                 \
+  do {                                                    \
+    if (top == 0) CCN_LP_NARROW(T, 0);                    \
+    else if (top == 1) CCN_LP_NARROW(T, 1);               \
+    else if (top == 2) CCN_LP_NARROW(T, LP_FEW + 2);      \
+    else if (top == 3) CCN_LP_NARROW(T, LP_FEW + 3);      \
+    else if (top == 4) CCN_LP_NARROW(T, LP_FEW + 4);      \
+    else if (top == 5) CCN_LP_NARROW(T, LP_FEW + 5);      \
+    else CCN_LP_NARROW(T, LP_WALK);                       \
   } while (0)
+    static_assert(LP_FEW_MAX == 5, "the launches below");
     if (dtype == 0) CCN_LP_NARROWS(0);
     else if (dtype == 1) CCN_LP_NARROWS(1);
     else CCN_LP_NARROWS(2);
