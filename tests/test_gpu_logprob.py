@@ -342,6 +342,22 @@ def test_the_best_class_alone(c, dtype):
     _check_gradient(some, _target(8, c), 1)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("c", [4, 8, 20, 64, 300, 1000, 5000, 20000])
+def test_subnormal_logits_and_zeros_of_both_signs(c, dtype):
+    """Told apart by the alternatives, though they weigh the same."""
+    step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    x = torch.zeros(4, c, dtype=dtype, device=DEV)
+    x[0] = (torch.arange(c, device=DEV) % 7 * step).to(dtype)
+    x[1] = (-(torch.arange(c, device=DEV) % 5) * step).to(dtype)
+    x[2, 1::2] = -0.0
+    x[3] = -0.0
+    x[3, c // 2] = step
+    assert float(x[0, 1]) == step > 0
+    for top in (1, 2, 3, min(c, 5), min(c, 9)):
+        _check(x, _target(4, c), top)
+
+
 def test_targets_that_are_not_scored():
     for c in (20, 65, 3000):
         rows = 9
