@@ -86,6 +86,10 @@ void require_gpu(const Tensor& t) {
 
 constexpr int64_t TOP_MAX = 64;
 
+// A gradient as the kernels read it: the engine hands some down with their sign still to be turned (those of imaginary parts), which
+// contiguous() leaves as it is.
+Tensor settled(const Tensor& g) { return g.defined() ? g.resolve_neg() : g; }
+
 template <typename T>
 T* data(const Tensor& t) {
   return t.defined() ? t.mutable_data_ptr<T>() : nullptr;
@@ -136,7 +140,8 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   static Tensor gradient(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &target = saved[1], &index = saved[2], &stats = saved[3], &entropy = saved[4];
-    const Tensor g_logprob = grads[0], g_entropy = grads[1], g_top = grads.size() > 2 && grads[2].defined() ? grads[2].contiguous() : Tensor();
+    const Tensor g_logprob = settled(grads[0]), g_entropy = settled(grads[1]);
+    const Tensor g_top = grads.size() > 2 && grads[2].defined() ? settled(grads[2]).contiguous() : Tensor();
     const int64_t rows = logits.size(0), c = logits.size(1), top = g_top.defined() ? g_top.size(1) : 0;
     const int64_t ignore = ctx->saved_data["ignore"].toInt(), per = logits.scalar_type() == at::kFloat ? 4 : 8;
     const int64_t ld = (c + per - 1) / per * per;            // rows start 16-byte aligned

@@ -639,3 +639,28 @@ def test_more_rows_than_a_launch_holds(c, top):
     rest = r.logprob.detach()[9: border - 4]
     _near(rest[:: 1 << 18], torch.full((rest[:: 1 << 18].numel(),), -math.log(c)), _e(torch.tensor(math.log(c)), c), "rows of zeros")
     assert bool((rest == rest[0]).all())
+
+
+@pytest.mark.parametrize("c", [20, 300, 5000])
+def test_gradients_whose_sign_is_still_to_be_turned(c):
+    """Gradients with torch's negative bit, contiguous and strided, give the bits of the negated ones; so does the engine's own: the
+    imaginary part of a conjugated complex number hands its gradient down that way."""
+    x, t = _logits(33, c, torch.float32).requires_grad_(True), _target(33, c)
+    gen = torch.Generator().manual_seed(c)
+    for k, shape in enumerate(((33,), (33,), (33, 7))):
+        g = torch.randn(shape, generator=gen).to(DEV)
+        far = torch.stack([g, g + 1], -1)[..., 0]
+        for lazy in (torch._neg_view(g), torch._neg_view(far)):
+            assert lazy.is_neg()
+            r = _score(x, t, top=7)
+            (want,) = torch.autograd.grad(r[k], x, -g, retain_graph=True)
+            (got,) = torch.autograd.grad(r[k], x, lazy)
+            assert float(want.abs().max()) > 0 and torch.equal(got, want)
+    seen = []
+    r = _score(x, t)
+    r.entropy.register_hook(lambda g: seen.append(g.is_neg()))
+    both = torch.view_as_real(torch.complex(r.logprob, r.entropy).conj().resolve_conj())
+    (got,) = torch.autograd.grad(both.sum(), x, retain_graph=True)
+    assert seen == [True]
+    (want,) = torch.autograd.grad([r.logprob, r.entropy], x, [torch.ones_like(r.logprob), -torch.ones_like(r.entropy)])
+    assert torch.equal(got, want)
