@@ -27,7 +27,6 @@ struct Entries {
   decltype(&ccn_grad_norm) grad_norm;
   decltype(&ccn_grad_clip) grad_clip;
   decltype(&ccn_adam_clip) adam_clip;
-  decltype(&ccn_adam_step) adam_step;
 } entry;
 
 template <typename F>
@@ -44,7 +43,6 @@ void bind(const py::dict& addresses) {
   take(entry.grad_norm, addresses, "ccn_grad_norm");
   take(entry.grad_clip, addresses, "ccn_grad_clip");
   take(entry.adam_clip, addresses, "ccn_adam_clip");
-  take(entry.adam_step, addresses, "ccn_adam_step");
 }
 
 // What _lib.call does around a launch (timing, the log of launches) is done there for these too, where it is asked for: `observer`
@@ -356,22 +354,21 @@ py::object adam_step(const py::list& of_params, const py::list& of_grads, const 
     }
   Table t[4];
   for (int k = 0; k < 4; ++k) t[k] = table_of(*lists[k], "adam_step_", k != 1);
+  const auto run = [&](double bound, void* ws, int64_t bytes, float* norm) {
+    launch("adam_clip", {t[1].n(), step, bytes}, t[1].total, [&] {
+      return entry.adam_clip((float* const*)t[0].at.data(), (const float* const*)t[1].at.data(), (float* const*)t[2].at.data(),
+                             (float* const*)t[3].at.data(), t[1].size.data(), t[1].n(), lr, beta1, beta2, eps, weight_decay, step, bound,
+                             ws, (size_t)bytes, norm, stream_of(t[1].one));
+    });
+  };
   py::object norm = py::none();
   if (max_norm) {
     NormOut o(t[1]);
-    launch("adam_clip", {t[1].n(), step, o.bytes}, t[1].total, [&] {
-      return entry.adam_clip((float* const*)t[0].at.data(), (const float* const*)t[1].at.data(), (float* const*)t[2].at.data(),
-                             (float* const*)t[3].at.data(), t[1].size.data(), t[1].n(), lr, beta1, beta2, eps, weight_decay, step,
-                             *max_norm, o.ws.mutable_data_ptr(), (size_t)o.bytes, o.norm.mutable_data_ptr<float>(), stream_of(t[1].one));
-    });
+    run(*max_norm, o.ws.mutable_data_ptr(), o.bytes, o.norm.mutable_data_ptr<float>());
     norm = py::cast(o.norm);
   } else {
     c10::DeviceGuard guard(t[1].one.device());
-    for (size_t i = 0; i < params.size(); ++i)
-      launch("adam_step", {t[1].size[i], step}, t[1].size[i], [&] {
-        return entry.adam_step((float*)t[0].at[i], (const float*)t[1].at[i], (float*)t[2].at[i], (float*)t[3].at[i], t[1].size[i],
-                               (float)lr, (float)beta1, (float)beta2, (float)eps, (float)weight_decay, step, stream_of(t[1].one));
-      });
+    run(INFINITY, nullptr, 0, nullptr);
   }
   moved(params);
   moved(exp_avgs);

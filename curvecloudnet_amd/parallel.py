@@ -288,7 +288,8 @@ def adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     """One ``torch.optim.Adam`` update, in place, of several contiguous 16-byte aligned fp32 tensors (the flat buckets of FlatAdam).
     ``max_norm``: the gradients' global norm is bounded as by clip_grad_norm_, but each is scaled as it is read (ccn_adam_clip): they keep
     their values, and the read and write of a separate clipping pass are saved.  Returns the norm before clipping (an fp32 scalar on the
-    device), or None without ``max_norm``.  ``step``: the 1-based count of this update."""
+    device), or None without ``max_norm``: the same update with nothing scaled and no norm taken.  Tensors that share memory are refused
+    either way.  ``step``: the 1-based count of this update."""
     step, max_norm = int(step), None if max_norm is None else _bound(max_norm, "adam_step_")
     if step < 1:
         raise ValueError("adam_step_: step %d; the first update is step 1" % step)

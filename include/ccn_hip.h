@@ -727,7 +727,8 @@ int ccn_logprob_bwd(const void* logits, int dtype, int64_t ld, const int64_t* ta
  * clipping.  clip: every value times min(1, max_norm / (norm + 1e-6)), in place, the factor rounded to the tensor's type first
  * (fp16: unless it is below 2^-14); tensors that share memory are refused.
  * adam_clip: torch.optim.Adam(amsgrad=False, maximize=False) over n runs of parameters (fp32, 16-byte aligned) with the gradients
- * scaled the same way as they are read; they are not written.  Norms are summed in double in a fixed order.
+ * scaled the same way as they are read; they are not written.  Without norm and ws and with an infinite max_norm no norm is taken and
+ * nothing is scaled.  What it writes may share memory with nothing else it is given.  Norms are summed in double in a fixed order.
  * ws: ccn_grad_norm_workspace_bytes(n) of device memory. */
 size_t ccn_grad_norm_workspace_bytes(int64_t n);
 int ccn_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t n, int kind, void* ws,

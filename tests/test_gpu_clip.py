@@ -440,3 +440,60 @@ def test_a_run_of_all_of_them():
     before = float(grad_norm([p.grad for p in mlp.parameters()]))
     assert abs(float(clip_grad_norm_(mlp.parameters(), before / 2)) - before) <= U * before
     assert abs(float(grad_norm([p.grad for p in mlp.parameters()])) - before / 2) <= before * (4 * U) + 1e-6
+
+
+@pytest.mark.parametrize("sizes", [(1,), (5, 1, 3), (1000, 7, 16385, 4096), (300001, 20), (37,) * 70, (0, 9, 0)])
+def test_adam_step_without_a_bound(sizes):
+    """Parameters and both moments, the bits of an infinite bound, another stream, and a captured update.  The errors are those of the update
+    that clips, but for v's: the gradient with decay is off by 4 u (|g| + |decay p|), its square by 8 u of their square, which
+    1 - beta2 takes along."""
+    from curvecloudnet_amd.parallel import adam_step_
+    how = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+    gen = torch.Generator().manual_seed(sum(sizes))
+    draw = lambda s: [(torch.randn(n, generator=gen) * s) for n in sizes]      # noqa: E731
+    for step, spread in ((1, 0.0), (50, 0.3)):
+        p, g, m = draw(1.0), draw(0.5), draw(spread)
+        v = [x.square() * spread for x in draw(0.5)]
+        _, want = _adam64(*[[x.double() for x in k] for k in (p, g, m, v)], step, 1e-2, (0.9, 0.999), 1e-8, 0.02, None)
+        dev, other, away, kept = ([[x.to(DEV) for x in k] for k in (p, g, m, v)] for _ in range(4))
+        assert adam_step_(*dev, step, **how) is None
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(dev[1], g))
+        for k, (wp, wm, wv, wg, den) in enumerate(want):
+            g0 = wg.abs() + (0.02 * p[k].double()).abs() * 2
+            em = 8 * U * (m[k].double().abs() + g0)
+            ev = 12 * U * wv + 8 * U * 0.001 * g0 * g0
+            assert bool(((dev[2][k].cpu().double() - wm).abs() <= em).all())
+            assert bool(((dev[3][k].cpu().double() - wv).abs() <= ev).all())
+            up = 1e-2 / (1 - 0.9 ** step) * ((em + 16 * U * wm.abs()) / den + wm.abs() / den * ev / (wv + 1e-300))
+            assert bool(((dev[0][k].cpu().double() - wp).abs() <= up + 2 * U * wp.abs()).all())
+        adam_step_(*other, step, max_norm=math.inf, **how)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            adam_step_(*away, step, **how)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            adam_step_(*kept, step, **how)
+        for turn in range(3):
+            for a, b in zip(kept, (p, g, m, v)):
+                for x, y in zip(a, b):
+                    x.copy_(y)
+            graph.replay()
+            torch.cuda.synchronize()
+            for also in (other, away, kept):
+                assert all(torch.equal(a, b) for x, y in zip(also, dev) for a, b in zip(x, y)), turn
+
+
+def test_adam_step_without_a_bound_refuses_shared_memory():
+    from curvecloudnet_amd.parallel import adam_step_
+    make = lambda n=64: [torch.ones(n, device=DEV)]        # noqa: E731
+    p, wide = make(), torch.ones(100, device=DEV)
+    for lists in ((p, make(), p, make()), (p, p, make(), make()), (p, make(), make(), p), (p + p, make() + make(), make() + make(), make() + make()),
+                  ([wide[:64]], make(), [wide[36:]], make())):
+        with pytest.raises(RuntimeError, match="share memory"):
+            adam_step_(*lists, 1)
+    torch.cuda.synchronize()
+    assert bool((p[0] == 1).all()) and bool((wide == 1).all())
+    with pytest.raises(ValueError, match="multiple of 16"):
+        adam_step_([torch.ones(65, device=DEV)[1:]], make(), make(), make(), 1)

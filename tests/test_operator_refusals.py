@@ -159,3 +159,24 @@ def test_lists_of_other_things_are_refused():
             grad_norm([bad])
         with pytest.raises(TypeError, match="is no tensor"):
             clip_grad_norm_([torch.nn.Parameter(torch.zeros(3)), bad], 1.0)
+
+
+def test_the_update_without_a_bound_refuses_from_c():
+    """Neither norm nor workspace, and an infinite bound: everything else is looked at all the same.  One of the two alone is refused."""
+    from curvecloudnet_amd import _lib
+    lib = _lib.lib()
+    null, fake = ctypes.c_void_p(None), ctypes.c_void_p(0x10000)
+    err = lambda: lib.ccn_last_error().decode()                      # noqa: E731
+    table = lambda *v: (ctypes.c_int64 * len(v))(*v)                 # noqa: E731
+
+    def adam(p=(0x1000,), g=(0x2000,), m=(0x3000,), v=(0x4000,), s=(4,), step=1, bound=math.inf, ws=null, wn=0, out=null):
+        return lib.ccn_adam_clip(table(*p), table(*g), table(*m), table(*v), table(*s), len(s), 1e-3, 0.9, 0.999, 1e-8, 0.0, step, bound,
+                                 ws, wn, out, null)
+
+    for call, word in ((lambda: adam(m=(0x1000,)), "share"), (lambda: adam(p=(0x2000,)), "share"), (lambda: adam(v=(0x3000,)), "share"),
+                       (lambda: adam(p=(0x1000, 0x1010), g=(0x2000, 0x2100), m=(0x3000, 0x3100), v=(0x4000, 0x4100), s=(8, 4)), "share"),
+                       (lambda: adam(p=(0x1008,)), "16-byte"), (lambda: adam(p=(0,)), "null"), (lambda: adam(s=(-1,)), "values"),
+                       (lambda: adam(step=0), "step"), (lambda: adam(bound=1.0), "null"), (lambda: adam(bound=math.nan), "max_norm"),
+                       (lambda: adam(out=fake), "null"), (lambda: adam(ws=fake, wn=1 << 20), "null"),
+                       (lambda: adam(out=fake, ws=fake, wn=8), "workspace")):
+        assert call() < 0 and word in err(), (word, err())
