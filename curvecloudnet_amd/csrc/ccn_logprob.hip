@@ -699,7 +699,7 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
   }
   __syncthreads();
   float* const out = tile + ROWS * pitch;
-  int* const out_class = reinterpret_cast<int*>(out + ROWS * top);
+  float* const out_class = out + ROWS * top;         // (classes and, below, keys: bits of whole numbers; this memory holds floats throughout)
   if ((int)threadIdx.x < live) {
     float* const mine = tile + threadIdx.x * pitch;
     const int64_t row = r0 + threadIdx.x, t = target[row];
@@ -742,31 +742,32 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
     }
     // (the K largest are not found among NaN: the few waves that have any walk)
     if (TOP == LP_WALK || (TOP > LP_FEW && __builtin_amdgcn_ballot_w64(m != m) != 0)) {
-      int* const order = reinterpret_cast<int*>(mine);   // whole numbers in the order of the alternatives
 #pragma unroll 4
-      for (int c = 0; c < C; ++c) {
+      for (int c = 0; c < C; ++c) {                      // whole numbers in the order of the alternatives
         const float v = mine[c];
         int o = __float_as_int(v + 0.0f);
         if (v != v) o = 0x7f800001;
-        order[c] = o ^ ((o >> 31) & 0x7fffffff);
+        mine[c] = __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
       }
       auto walk = [&](float& value, int& c) {
         int v = INT_MIN;                             // (below every value; taken ones become it)
         c = 0;
 #pragma unroll 4
         for (int i = 0; i < C; ++i) {
-          const int o = order[i];
+          const int o = __float_as_int(mine[i]);
           c = o > v ? i : c;
           v = max(v, o);
         }
-        order[c] = INT_MIN;
+        mine[c] = __int_as_float(INT_MIN);
         value = __int_as_float(v ^ ((v >> 31) & 0x7fffffff));
       };
       if constexpr (TOP == LP_WALK) {
         for (int j = 0; j < top; ++j) {
           float v;
-          walk(v, out_class[threadIdx.x * top + j]);
+          int c;
+          walk(v, c);
           out[threadIdx.x * top + j] = (v - r.base) - r.log_total;
+          out_class[threadIdx.x * top + j] = __int_as_float(c);
         }
       } else {
 #pragma unroll
@@ -792,7 +793,7 @@ __global__ __launch_bounds__(LP_NARROW_TPB) void logprob_narrow_kernel(const voi
   } else {
     for (int i = threadIdx.x; i < live * top; i += LP_NARROW_TPB) {
       top_logprob[r0 * top + i] = out[i];
-      top_index[r0 * top + i] = out_class[i];
+      top_index[r0 * top + i] = __float_as_int(out_class[i]);
     }
   }
 }

@@ -664,3 +664,24 @@ def test_gradients_whose_sign_is_still_to_be_turned(c):
     assert seen == [True]
     (want,) = torch.autograd.grad([r.logprob, r.entropy], x, [torch.ones_like(r.logprob), -torch.ones_like(r.entropy)])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["fp32", "fp16"])
+@pytest.mark.parametrize("c", list(range(1, 25)))
+def test_every_number_of_alternatives_of_short_rows(c, dtype):
+    """Rows that a thread walks in shared memory, where results and keys take the place of the logits: waves of ordinary rows and waves with
+    rows of NaN, infinities, equal logits and zeros of both signs, for every number of alternatives."""
+    x, t = _logits(300, c, dtype), _target(300, c)
+    for at in (0, 130, 140, 299 - 9):
+        x[at], x[at + 1], x[at + 2, c // 2] = math.nan, -math.inf, math.nan
+        x[at + 3], x[at + 4, -1], x[at + 5, 0] = 0.25, math.inf, -math.inf
+        x[at + 6, ::2], x[at + 6, 1::2], x[at + 7, 1:] = -0.0, 0.0, -math.inf
+        x[at + 8, ::3] = math.nan
+    for top in range(c + 1):
+        _check(x, t, top)
+    many = x.repeat(220, 1)                                             # (as many rows as keep to that form)
+    given = t.repeat(220)
+    for top in sorted({c // 2, c}):
+        r = _score(many, given, top=top)
+        for part in (slice(0, 300), slice(300 * 219, 300 * 220)):
+            _check(x, t, top, r=type(r)(*(None if v is None else v[part] for v in r)))
