@@ -88,6 +88,14 @@ constexpr int64_t TOP_MAX = 64;
 // contiguous() leaves as it is.
 Tensor settled(const Tensor& g) { return g.defined() ? g.resolve_neg() : g; }
 
+// Logits (rows, C) as the kernels read them: columns adjacent, rows in order and apart.
+Tensor rows_of(Tensor x) {
+  if (x.is_neg()) x = x.resolve_neg();
+  // (one row: its stride is never used, and torch may report any)
+  if ((x.stride(1) != 1 && x.size(1) > 1) || (x.size(0) > 1 && x.stride(0) < x.size(1))) x = x.contiguous();
+  return x;
+}
+
 template <typename T>
 T* data(const Tensor& t) {
   return t.defined() ? t.mutable_data_ptr<T>() : nullptr;
@@ -130,17 +138,31 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({logits, target, s.index, s.stats, s.entropy});
     ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["rows"] = logits.size(0);
+    ctx->saved_data["classes"] = logits.size(1);
+    ctx->saved_data["device"] = (int64_t)logits.get_device();
     if (!top) return {s.logprob, s.entropy};
     ctx->mark_non_differentiable({s.index});
     return {s.logprob, s.entropy, s.best, s.index};
   }
 
   static Tensor gradient(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &target = saved[1], &index = saved[2], &stats = saved[3], &entropy = saved[4];
     const Tensor g_logprob = settled(grads[0]), g_entropy = settled(grads[1]);
     const Tensor g_top = grads.size() > 2 && grads[2].defined() ? settled(grads[2]).contiguous() : Tensor();
-    const int64_t rows = logits.size(0), c = logits.size(1), top = g_top.defined() ? g_top.size(1) : 0;
+    const int64_t rows = ctx->saved_data["rows"].toInt(), c = ctx->saved_data["classes"].toInt();
+    const int64_t device = ctx->saved_data["device"].toInt(), top = g_top.defined() ? g_top.size(1) : 0;
+    // (a hook on saved tensors may have laid them out anew, and torch does not look at what it gives back)
+    const auto saved = ctx->get_saved_variables();
+    const auto kept = [&](size_t i, at::ScalarType type, at::IntArrayRef shape) {
+      const Tensor& t = saved[i];
+      TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == shape && t.is_cuda() && t.get_device() == device &&
+                      (t.scalar_type() == type || (i == 0 && code_of(t.scalar_type()) >= 0)),
+                  "token_logprobs: a hook on saved tensors gave back another tensor than was saved");
+      return i == 0 ? rows_of(t) : t.resolve_neg().contiguous();
+    };
+    const Tensor logits = kept(0, at::kFloat, {rows, c}), target = kept(1, at::kLong, {rows});
+    const Tensor index = top ? kept(2, at::kLong, {rows, top}) : Tensor();
+    const Tensor stats = kept(3, at::kFloat, {rows, 2}), entropy = kept(4, at::kFloat, {rows});
     const int64_t ignore = ctx->saved_data["ignore"].toInt(), per = logits.scalar_type() == at::kFloat ? 4 : 8;
     const int64_t ld = (c + per - 1) / per * per;            // rows start 16-byte aligned
     c10::DeviceGuard guard(logits.device());
@@ -190,10 +212,7 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& target, int64_t top
   TORCH_CHECK_VALUE(logits.device() == target.device(), "token_logprobs: logits on ", logits.device().str(), ", target on ",
                     target.device().str());
   const bool flat = logits.dim() == 2;
-  Tensor x = flat ? logits : logits.reshape({rows, c});
-  if (x.is_neg()) x = x.resolve_neg();
-  // (one row: its stride is never used, and torch may report any)
-  if ((x.stride(1) != 1 && c > 1) || (rows > 1 && x.stride(0) < c)) x = x.contiguous();
+  const Tensor x = rows_of(flat ? logits : logits.reshape({rows, c}));
   Tensor t = target.is_neg() ? target.resolve_neg() : target;
   if (!flat || t.scalar_type() != at::kLong || !t.is_contiguous()) t = t.reshape({rows}).to(at::kLong).contiguous();
   Tensor logprob, entropy, best, index;

@@ -685,3 +685,67 @@ def test_every_number_of_alternatives_of_short_rows(c, dtype):
         r = _score(many, given, top=top)
         for part in (slice(0, 300), slice(300 * 219, 300 * 220)):
             _check(x, t, top, r=type(r)(*(None if v is None else v[part] for v in r)))
+
+
+def _gradient_under_hooks(x, t, g, pack, unpack):
+    from torch.autograd.graph import saved_tensors_hooks
+    with saved_tensors_hooks(pack, unpack):
+        r = _score(x, t, top=3)
+    return torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], x, g)[0]
+
+
+@pytest.mark.parametrize("c", [20, 300, 5000])
+def test_saved_tensors_that_come_back_in_another_layout(c):
+    """Hooks on saved tensors: copies, on the host meanwhile, spread out, transposed, with their sign still to be turned; checkpointing."""
+    x, t = _logits(33, c, torch.float32).requires_grad_(True), _target(33, c)
+    gen = torch.Generator().manual_seed(c)
+    g = [torch.randn(s, generator=gen).to(DEV) for s in ((33,), (33,), (33, 3))]
+    r = _score(x, t, top=3)
+    (want,) = torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], x, g)
+    same = lambda v: v                                                  # noqa: E731
+    for pack, unpack in ((torch.clone, same), (lambda v: v.cpu(), lambda v: v.to(DEV)), (torch.clone, lambda v: torch.stack([v, v], -1)[..., 0]),
+                         (torch.clone, lambda v: v.t().contiguous().t()), (torch.neg, torch._neg_view)):
+        assert torch.equal(_gradient_under_hooks(x, t, g, pack, unpack), want)
+    from torch.utils.checkpoint import checkpoint
+    r = checkpoint(lambda y: _score(y, t, top=3), x, use_reentrant=False)
+    (got,) = torch.autograd.grad([r.logprob, r.entropy, r.top_logprob], x, g)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("unpack", [lambda v: v[:5], lambda v: v[..., None], lambda v: v.double() if v.is_floating_point() else v.int(),
+                                    lambda v: v.cpu(), lambda v: v.cpu() if v.dim() == 1 else v, lambda v: v[:, :1] if v.dim() == 2 else v],
+                         ids=["rows", "axes", "types", "host", "host-in-part", "columns"])
+def test_saved_tensors_that_come_back_as_others_are_refused(unpack):
+    x, t = _logits(33, 300, torch.float32).requires_grad_(True), _target(33, 300)
+    g = [torch.ones(s, device=DEV) for s in ((33,), (33,), (33, 3))]
+    with pytest.raises(RuntimeError, match="hook"):
+        _gradient_under_hooks(x, t, g, torch.clone, unpack)
+
+
+class _Nothing(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, v):
+        return v.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+@pytest.mark.parametrize("c", [20, 300, 5000])
+def test_outputs_that_get_no_gradient_at_all(c):
+    """What follows gives none to any output: zeros come out."""
+    x, t = _logits(7, c, torch.float32).requires_grad_(True), _target(7, c)
+    r = _score(x, t, top=3)
+    (d,) = torch.autograd.grad(sum(_Nothing.apply(v).sum() for v in r[:3]), x)
+    assert d.shape == x.shape and not bool(d.any())
+
+
+def test_saved_rows_that_come_back_expanded():
+    """Every value of a row is the same, and comes back as one."""
+    x, t = torch.full((1, 300), 0.5, device=DEV).requires_grad_(True), _target(1, 300)
+    r = _score(x, t, top=3)
+    g = [torch.ones_like(v) for v in r[:3]]
+    (want,) = torch.autograd.grad(r[:3], x, g)
+    got = _gradient_under_hooks(x, t, g, torch.clone, lambda v: v[:, :1].clone().expand(1, 300) if v.shape == (1, 300) else v)
+    assert torch.equal(got, want)
