@@ -157,8 +157,9 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_norm_final_kernel(const double*
 }
 
 // The factor is rounded to the gradients' type first, as a torch tensor's product with a scalar tensor rounds it: the same bits come out,
-// for half a step of the type more than with the factor in 32 bits.  Below the normal numbers of fp16, where half a step can be all of
-// the factor (a norm of 10^7 and a bound of 0.1), it stays in 32 bits.
+// for half a step of the type more than with the factor in 32 bits.  That half step is common to all values, so the norm that is left is
+// off by it too, 2^-8 of max_norm at most for bf16 (2^-11 for fp16) in either direction, and a bf16 factor above 1 - 2^-9 is 1.  Below the
+// normal numbers of fp16, where half a step can be all of the factor (a norm of 10^7 and a bound of 0.1), it stays in 32 bits.
 template <int T>
 __device__ __forceinline__ float clip_factor_of(float scale) {
   if (T == 2 && scale < 0x1p-14f) return scale;
@@ -189,8 +190,8 @@ __device__ __forceinline__ void clip_apply(char* p, int n, float scale) {
   if ((int)threadIdx.x < n - whole) st_el<T>(p, whole + threadIdx.x, ld_el<T>(p, whole + threadIdx.x) * scale);
 }
 
-// The second pass, bound by memory: 400M bf16 values 257 us (6.2 TB/s of reads and writes), 310 tensors of 5.3M fp32 14 us (3 TB/s, in chunks
-// of 2048 as of 16384).
+// The second pass, bound by memory: 400M bf16 values 257 us (6.2 TB/s of reads and writes); 310 tensors of 5.3M fp32 14 us (3 TB/s, in chunks
+// of 2048 as of 16384), the waves waiting for 83 % of that: for the partial results, then for their values.
 template <int KIND>
 __global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, const double* __restrict__ partial, int count,
                                                              double max_norm, float* __restrict__ norm,
@@ -219,7 +220,8 @@ __global__ __launch_bounds__(CLIP_TPB) void grad_clip_kernel(const ClipTable t, 
 
 // ---- few values (pieces of SMALL_PIECE of a tensor, two to a wave at most): one workgroup keeps them in registers between the norm and
 // the product, one launch does both: 6 tensors of 9001 fp32 values take 6.2 us with their call, 9.8 in two launches; 65536 values 9.6 and
-// 9.8, of bf16 7.5 and 10.0.  max_norm < 0: the norm alone.
+// 9.8, of bf16 7.5 and 10.0.  max_norm < 0: the norm alone.  (1024 threads leave 128 registers each: four of them spill, but for the largest
+// magnitude.)
 constexpr int SMALL_TPB = 1024, SMALL_PIECE = 2048, SMALL_EACH = 2, SMALL_MAX = SMALL_EACH * SMALL_TPB / 64;
 static_assert(SMALL_MAX <= 64, "found by one look of a wave");
 

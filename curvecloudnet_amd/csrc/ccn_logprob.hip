@@ -535,7 +535,8 @@ __device__ __forceinline__ V lp_team(V v, F f) {
 // ---- rows of 25 to 512 classes: TEAM lanes hold a row in registers, 16 logits each, and join their results by lane moves; a
 // wave has 64 / TEAM rows.  Alternatives: `top` walks over the registers, each of which takes the largest logit that is left; TEAM of
 // them are kept, a lane each, and stored side by side.  220011 x 55 fp32: 14.0 us, 3.8 TB/s, half of it the latency of one round of loads;
-// with alternatives the walks bound it, each of them 1.2 us for 100000 x 50 fp32, 2.1 for 50000 x 256 fp32 and 1.1 in 16 bits.
+// with alternatives the walks' vector arithmetic bounds it (busy for 87 % of the time and more), each of them 1.2 us for 100000 x 50 fp32, 2.1 for
+// 50000 x 256 fp32 and 1.1 in 16 bits.
 template <int T, int TEAM, int TOP>
 __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __restrict__ x, int64_t ld,
                                                               const int64_t* __restrict__ target, int64_t rows, int C,
@@ -663,7 +664,8 @@ __global__ __launch_bounds__(LP_TPB) void logprob_team_kernel(const void* __rest
 
 // ---- rows of up to 24 classes: 128 rows go through shared memory (16-byte loads) and a thread walks each of them there.  (Two threads to a
 // row, or the registers of logprob_team_kernel, take 12.0 and 12.3 us for 400070 x 20 instead of 10.8.)  Bound by the latency from load to
-// store of a workgroup's rows, and by its stores (400000 x 20 fp32: 9.9 us, 3.9 TB/s; with 3 alternatives 15.1, 3.5).
+// store of a workgroup's rows, its stores and, with alternatives, by vector arithmetic, which is busy for 71 % of the time (400000 x 20 fp32: 9.9 us,
+// 3.9 TB/s; with 3 alternatives 15.1, 3.5).
 // Up to LP_FEW_MAX alternatives come out of the two walks that the row takes anyway: the first keeps the K largest values in order, the second,
 // from the last class to the first, notes where they are.  They leave through the row's own place in shared memory: a thread's own are K values
 // wide, 64 such stores side by side cost more.  More of them: a walk for each, which takes the largest that is left (400000 x 20 fp32 with 3 / 5

@@ -271,7 +271,9 @@ def grad_norm(tensors, norm_type=2.0):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """``torch.nn.utils.clip_grad_norm_`` in one call of the library (ccn_grad_clip): every gradient of ``parameters`` is multiplied
     in place by min(1, max_norm / (norm + 1e-6)); returns the norm before clipping, an fp32 scalar on the device.  As there, the factor is
-    rounded to a 16-bit gradient's type before the product, and that once (for fp16 a factor below 2^-14 is not: it could vanish).  A norm that is not finite gives what the formula gives (0 or NaN), or raises with
+    rounded to a 16-bit gradient's type before the product, and that once (for fp16 a factor below 2^-14 is not: it could vanish).  That
+    alone may leave the norm up to 2^-8 of ``max_norm`` off it for bf16, 2^-11 for fp16, and a bf16 factor above 1 - 2^-9 is 1.  adam_step_
+    holds the factor in 32 bits.  A norm that is not finite gives what the formula gives (0 or NaN), or raises with
     ``error_if_nonfinite`` (which waits for the GPU) before anything is scaled.  Gradients that share memory are refused."""
     kind, max_norm = _norm_kind(norm_type, "clip_grad_norm_"), _bound(max_norm, "clip_grad_norm_")
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
