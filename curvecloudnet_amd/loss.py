@@ -55,7 +55,8 @@ def token_logprobs(logits, target, top=0, ignore_index=-100):
     ``target == ignore_index``: logprob 0, no gradient from it; entropy and alternatives are the row's all the same.  Any other
     target outside [0, C): NaN, in logprob and (where logprob takes part in the loss) in the row's gradient.  Logits of -inf are
     classes without probability; a row of nothing else has logprob -inf, entropy 0 and gradient 0 but for the given class's own.
-    The gradient has the logits' type, its rows 16-byte aligned (their stride padded where C is odd)."""
+    The gradient has the logits' type, its rows 16-byte aligned (their stride padded where C is odd).  Where a backward pass is captured
+    into a graph, no eager autograd graph of the same leaves may be alive, as for any torch operator."""
     return Scores(*binding().token_logprobs(logits, target, top, ignore_index))
 
 
